@@ -125,9 +125,79 @@ int sabah_moe_decode(int n_layers, const void *const *gate_banks, const void *co
                      int ff, int n_used, int n_tokens, int qt_gate, int qt_up, int qt_down, void *stream);
 
 /* Reads and clears the device error word: 1 when a kernel reading a
- * device-resident bank met an expert id outside [0, n_experts), else 0.
+ * device-resident bank met an expert id outside [0, n_experts), 4 when an
+ * attention-side kernel met a cache page, slot, length or position out of
+ * range, else 0.
  * New in this build (the device-resident path has no synchronous id check). */
 int sabah_rt_device_error(void);
+
+/* ---- the step around the experts: attention over a paged cache, the router ---- */
+
+/* New in this build (the reference leaves these to its host application).
+ * Element types are ggml's codes: 0 = f32, 1 = f16, 30 = bf16. Strides are in
+ * bytes; the last dimension is dense. Everything is asynchronous on stream
+ * (NULL: the compute stream) and allocates nothing. An index out of range
+ * (named at each call) is never followed: it gives NaN in what depends on it
+ * and the device error word. */
+
+/* Per-head norms of q [n_tokens][n_q_heads][head_dim] and k [..][n_kv_heads][..],
+ * the position rotation, and the write of k and v into a paged cache:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight          (weight NULL: y = x)
+ *   pair i < rope_dim / 2 of y is (i, i + rope_dim / 2), or (2i, 2i + 1) with
+ *   pairs_mode; (a, b) -> (a c - b s, a s + b c), (c, s) = table[pos][i],
+ *   pos = positions[pair_axis ? pair_axis[i] : 0][token]
+ * table is [n_positions][rope_dim / 2][2] floats, positions [n_axes][n_tokens]
+ * (n_axes <= 4), pair_axis [rope_dim / 2] or NULL. head_dim is even and at most
+ * 256; rope_dim is even, 0 for no rotation.
+ * q_out and k_out are dense [n_tokens][heads][head_dim] of act_type; q_out may
+ * be q and k_out k where those are dense. With d_slots, k (as rotated) and v
+ * (as it is) also go to row slots[t] % page_size of page slots[t] / page_size,
+ * rounded to cache_type (f16 or bf16); a negative slot writes nothing, two
+ * tokens of one call must not share a slot, and k_out may be NULL. Without
+ * d_slots, v and the cache arguments are not read. A slot past the cache writes
+ * nothing and sets the device error; a position or axis out of range gives NaN. */
+int sabah_qk_norm_rope(const void *d_q, size_t q_token_stride, size_t q_head_stride, int n_q_heads, const void *d_k,
+                       size_t k_token_stride, size_t k_head_stride, const void *d_v, size_t v_token_stride,
+                       size_t v_head_stride, int n_kv_heads, int n_tokens, int head_dim, int act_type,
+                       const float *d_q_weight, const float *d_k_weight, float eps, const float *d_table,
+                       int n_positions, int rope_dim, int pairs_mode, const int32_t *d_positions, int n_axes,
+                       const uint8_t *d_pair_axis, void *d_q_out, void *d_k_out, void *d_k_cache,
+                       size_t k_page_stride, size_t k_slot_stride, size_t k_cache_head_stride, void *d_v_cache,
+                       size_t v_page_stride, size_t v_slot_stride, size_t v_cache_head_stride, int n_pages,
+                       int page_size, int cache_type, const int64_t *d_slots, void *stream);
+
+/* Attention of one new token per sequence over a paged cache:
+ *   out[b][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale <q[b][h], k_j> - m)
+ *   for max(0, lens[b] - window) <= j < lens[b] (window 0: all of them)
+ * Key j is row j % page_size of page block_table[b][j / page_size], and query
+ * head h reads key-value head h / (n_q_heads / n_kv_heads). The new token's own
+ * key is in the cache and counted in lens[b]. head_dim is a multiple of 8 up to
+ * 256. act_type is that of q and out (dense [n_seqs][n_q_heads][head_dim]): f32,
+ * or the cache's type (f16 or bf16). Cache pointers and strides are multiples
+ * of 16 bytes. d_lse (or NULL) gets m + ln sum p, [n_seqs][n_q_heads] floats.
+ * A sequence of length 0 gives zeros and an lse of -inf. Cache rows, pages and
+ * table entries outside the window are not read. A length outside
+ * [0, table_width * page_size] or a page outside [0, n_pages) gives that
+ * sequence NaN, and the device error word.
+ * d_workspace holds sabah_attend_paged_workspace(...) bytes, 16-byte aligned,
+ * of any content; calls that may overlap on the GPU must not share it. */
+size_t sabah_attend_paged_workspace(int n_q_heads, int n_kv_heads, int head_dim);
+int sabah_attend_paged(const void *d_q, size_t q_seq_stride, size_t q_head_stride, int act_type,
+                       const void *d_k_cache, size_t k_page_stride, size_t k_slot_stride, size_t k_head_stride,
+                       const void *d_v_cache, size_t v_page_stride, size_t v_slot_stride, size_t v_head_stride,
+                       int cache_type, int n_pages, int page_size, const int32_t *d_block_table,
+                       size_t table_stride, int table_width, const int32_t *d_lens, int n_seqs, int n_q_heads,
+                       int n_kv_heads, int head_dim, float scale, int window, void *d_out, float *d_lse,
+                       void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* The routed block's ids and w from router logits [n_tokens][n_experts]
+ * (act_type f32, f16 or bf16; n_experts <= 2048): the n_used <= 32 largest per
+ * token, ties to the lower index, in descending order, and their softmax
+ * weights times scale, over all experts or (renorm) over the chosen ones.
+ * Outputs are dense [n_tokens][n_used]. A row of -inf only gives zero weights;
+ * a NaN ranks last and makes its row's weights NaN; ids are always in range. */
+int sabah_route_topk(const void *d_logits, size_t row_stride, int act_type, int n_tokens, int n_experts, int n_used,
+                     int renorm, float scale, int32_t *d_ids, float *d_w, void *stream);
 
 /* ---- dequantization ---------------------------------------------------------- */
 

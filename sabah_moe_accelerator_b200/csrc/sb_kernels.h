@@ -55,7 +55,12 @@ struct sb_block_args {
 };
 
 // device-side error codes written to *err
-enum { SB_DERR_NONE = 0, SB_DERR_BAD_ID = 1, SB_DERR_TIMEOUT = 2, SB_DERR_MISALIGNED = 3 };
+enum { SB_DERR_NONE = 0, SB_DERR_BAD_ID = 1, SB_DERR_TIMEOUT = 2, SB_DERR_MISALIGNED = 3, SB_DERR_BAD_INDEX = 4 };
+
+// What the entry points outside sb_runtime.cu do first: the runtime is
+// initialised, an error left by an earlier kernel is reported, and NULL means
+// the runtime's compute stream. *err is the device error word.
+bool sb_op_begin(void* stream, cudaStream_t* st, int** err);
 
 // Optional per-kernel timing (SABAH_LLAMA_EVENTS=1 or sabah_rt_kernel_timing):
 // launches are bracketed by CUDA events on their own stream and accumulated

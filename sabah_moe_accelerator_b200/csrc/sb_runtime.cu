@@ -548,6 +548,7 @@ bool device_errors_clear() {
         sb_set_error("%s (device error %d, reported by the first call after the kernel ran)",
                      code == SB_DERR_BAD_ID ? "a kernel found an expert id outside [0, n_experts)"
                      : code == SB_DERR_MISALIGNED ? "an expert base was not 16-byte aligned"
+                     : code == SB_DERR_BAD_INDEX ? "a kernel found a cache page, slot, length or position out of range"
                      : "a kernel gave up waiting for its weight tiles", code);
         return false;
     }
@@ -1144,8 +1145,16 @@ SABAH_API int sabah_moe_block_ids_noalloc(const void* gate_bank, const void* up_
     return sb_block_iq3s_fixed(a, stream ? (cudaStream_t)stream : g_rt.compute);
 }
 
+bool sb_op_begin(void* stream, cudaStream_t* st, int** err) {
+    if (!ensure_init() || !device_errors_clear()) return false;
+    *st = stream ? (cudaStream_t)stream : g_rt.compute;
+    *err = g_rt.err_d;
+    return true;
+}
+
 // Reads and clears the device error word (1 = an out-of-range expert id met
-// by a kernel reading a device-resident bank). Returns the code, 0 if none.
+// by a kernel reading a device-resident bank, 4 = a cache page, slot, length
+// or position out of range). Returns the code, 0 if none.
 SABAH_API int sabah_rt_device_error(void) {
     if (!g_rt.err_h) return 0;
     const int c = *(volatile int*)g_rt.err_h;

@@ -23,6 +23,8 @@ QTYPE = {
     "IQ3_XXS": 18, "IQ4_NL": 20, "IQ3_S": 21, "IQ2_S": 22, "IQ4_XS": 23, "Q2_0": 42,
 }
 QTYPE_NAME = {v: k for k, v in QTYPE.items()}
+# element types of activations and key-value caches (ggml's codes too)
+ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 30
 
 # (elements per block, bytes per block) (reference rt.py:26-31, plus Q6_K)
 QBLOCK = {
@@ -106,6 +108,13 @@ SIGNATURES = {
     "sabah_rt_device_error": ([], c_i),
     "sabah_moe_decode": ([c_i, c_vp, c_vp, c_vp, c_sz, c_sz, c_i, c_vp, c_vp, c_vp, c_vp,
                           c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_vp], c_i),
+    "sabah_qk_norm_rope": ([c_vp, c_sz, c_sz, c_i, c_vp, c_sz, c_sz, c_vp, c_sz, c_sz, c_i, c_i, c_i, c_i,
+                            c_vp, c_vp, c_f, c_vp, c_i, c_i, c_i, c_vp, c_i, c_vp, c_vp, c_vp,
+                            c_vp, c_sz, c_sz, c_sz, c_vp, c_sz, c_sz, c_sz, c_i, c_i, c_i, c_vp, c_vp], c_i),
+    "sabah_attend_paged_workspace": ([c_i, c_i, c_i], c_sz),
+    "sabah_attend_paged": ([c_vp, c_sz, c_sz, c_i, c_vp, c_sz, c_sz, c_sz, c_vp, c_sz, c_sz, c_sz, c_i, c_i, c_i,
+                            c_vp, c_sz, c_i, c_vp, c_i, c_i, c_i, c_i, c_f, c_i, c_vp, c_vp, c_vp, c_sz, c_vp], c_i),
+    "sabah_route_topk": ([c_vp, c_sz, c_i, c_i, c_i, c_i, c_i, c_f, c_vp, c_vp, c_vp], c_i),
     "sabah_rt_kernel_timing": ([c_i], c_i),
     "sabah_rt_kernel_times": ([ctypes.c_char_p, c_sz], c_i),
     "sabah_synth_rows": ([c_vp, c_i, ctypes.c_longlong, c_i, ctypes.c_ulonglong, c_f, c_vp], c_i),
