@@ -6,12 +6,47 @@
 // Key j of sequence b is row j % page_size of page block_table[b][j / page_size].
 // A sequence of length zero gives zeros and lse = -inf. Nothing outside
 // [lo, len) is read: not a key, not a table entry.
+//
+// Bound: DRAM, every key and value row once. A key-value head's query heads
+// (up to 16: the rows of an MMA tile) are taken together, so the rows are read
+// once for all of them; the arithmetic is 16-row mma.sync on 16 keys at a time,
+// a fraction of the tensor rate and well under the time the rows take to
+// arrive. tcgen05's 128-row tiles would be 87-99% padding here.
+//
+// The work is a list of steps of 16 keys over all (sequence, key-value head)
+// rows. Each warp takes an equal, contiguous part of it, whatever the lengths:
+// one long sequence spreads over the whole chip, and many short ones stay whole
+// within a warp. Warps never wait for one another; each streams its own keys
+// and values through its own ring in shared memory (cp.async, rows padded by 16
+// bytes so that ldmatrix meets no bank twice). A row that ends in a part is
+// left as (m, l, unnormalised out) in the workspace, and a second, small launch
+// (a programmatic dependent of the first) joins the pieces of each cut row in
+// a fixed order. Rows of at most kWhole steps are never cut; where the block
+// table cannot hold a longer sequence the second launch is left out.
+//
+// Precision: scores, m, l and out are fp32. The MMA takes 16-bit factors, so
+// fp32 queries and the softmax weights are split into a sum of 16-bit parts
+// (f16: 2 parts, 22 bits; bf16: 3 parts, 24 bits), each multiplied exactly.
+// With 16-bit outputs the weights take two parts, which leaves the output's
+// own rounding as the only one. f16 parts keep their bits only in f16's normal
+// range: a query row is scaled to below 2 by a power of two, and the weights
+// are computed times 2^12. The parts but the last are cut off rather than
+// rounded, so all of a number's parts have its sign, and the first part's
+// products are summed apart from the others': where an infinite key or value
+// makes the others infinite or NaN (0 * inf), add_rest() leaves the first.
+#include <algorithm>
+
 #include "sb_act.cuh"
 #include "sb_kernels.h"
 
 namespace {
 
 constexpr int kMaxDim = 256;
+constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in shared memory
+constexpr int kStep = 16;        // keys per step
+constexpr int kWhole = 8;        // rows of at most this many steps are never cut
+constexpr int kMinSteps = 4;     // and a part is at least this long
+constexpr int kSmemLimit = 227 * 1024;
 
 struct AttendParams {
     const uint8_t* q;
@@ -24,78 +59,611 @@ struct AttendParams {
     int table_width;
     const int32_t* lens;
     int n_seqs, n_q, n_kv, dim, window;
+    int group, tiles;       // query heads per key-value head; 16-row tiles of them
     float scale_log2;       // scale * log2(e)
     uint8_t* out;
     float* lse;
     int* err;
+    int2* cuts;             // per warp: the row cut in its part (-1: none) and its number of pieces
+    float* pieces;          // per warp two: the row it enters in the middle of, the row it leaves early
+    int piece_floats, piece_rows;
 };
 
-// one warp per (sequence, query head), one key at a time
-template <class Act, class Cache>
-__global__ void k_attend(AttendParams p) {
-    const int lane = threadIdx.x, b = blockIdx.x / p.n_q, h = blockIdx.x % p.n_q, kv = h / (p.n_q / p.n_kv);
-    int len = p.lens[b];
-    bool bad = len < 0 || len > (long long)p.table_width * p.page_size;
-    if (bad) len = 0;
-    const int lo = p.window > 0 ? max(0, len - p.window) : 0;
-    constexpr int N = kMaxDim / 32;
-    // sums of kBlock keys are added up among themselves first: one running fp32
-    // sum over 10^5 keys would lose half its digits
-    constexpr int kBlock = 64;
-    float q[N], o[N], ob[N], m = -INFINITY, l = 0.f, lb = 0.f;
-    for (int i = 0; i < N; ++i) {
-        const int d = lane + 32 * i;
-        q[i] = d < p.dim ? sb_to_float(((const Act*)(p.q + b * p.q_seq + h * p.q_head))[d]) : 0.f;
-        o[i] = ob[i] = 0.f;
+// ------------------------------------------------------------ PTX helpers
+__device__ inline uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ inline void copy16(uint32_t dst, const void* src, bool real) {   // zeros unless real
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ inline void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ inline void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ inline void ldsm4(uint32_t* r, uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ inline void ldsm4t(uint32_t* r, uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <class T>
+__device__ inline void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ inline float exp2_fast(float x) {   // 2 ulp; exp2(-inf) = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two values as 16-bit ones, cut off (CUT) or rounded to nearest
+template <class T, bool CUT>
+__device__ inline uint32_t pack2(float a, float b) {
+    uint32_t u;
+    if constexpr (std::is_same<T, __half>::value && CUT)
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+    else if constexpr (std::is_same<T, __half>::value)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+    else if constexpr (CUT)
+        u = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+    return u;
+}
+// first + rest, where rest counts only if it is a number: first is infinite or
+// NaN whenever rest is, and of the same sign (fmaxf takes a NaN's other side)
+__device__ inline float add_rest(float first, float rest) { return first + fmaxf(rest, -3.402823466e38f); }
+template <class T>
+__device__ inline float2 unpack2(uint32_t u) {
+    if constexpr (std::is_same<T, __half>::value)
+        return __half22float2(*(const __half2*)&u);
+    else
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// ------------------------------------------------------------ shapes
+// DP: head size rounded up to a tile width. The ring of one warp has `stages`
+// steps of 16 keys and 16 values.
+template <int DP>
+struct Shape {
+    static constexpr int kRow = DP * 2 + 16;                  // bytes of a padded row
+    static constexpr int kStage = 2 * kStep * kRow;
+    static constexpr int kStages = DP <= 64 ? 6 : DP <= 96 ? 4 : 3;
+    static constexpr int kLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // lanes that copy one row
+    static constexpr int kWarps = 8;                          // at most
+};
+
+// The lengths' scan: steps of sequences before b, for one key-value head.
+struct Seqs {
+    long long* pre;   // [n_seqs + 1]
+    int* len;         // [n_seqs], -1 where out of range
+};
+__device__ inline int window_start(int len, int window) { return window > 0 ? max(0, len - window) : 0; }
+__device__ inline int seq_steps(int len, int window) {
+    return len <= 0 ? 1 : (len + kStep - 1) / kStep - window_start(len, window) / kStep;
+}
+
+// A place in the list of steps; each warp has one that loads and one that computes.
+struct Cursor {
+    int b, h;            // sequence, row of it (key-value head and tile)
+    int j, end, steps;   // step in the row, where this warp leaves it, the row's steps
+    int len, lo;
+    long long row_at;    // the row's first step in the list
+};
+
+// starts the row at c.b, c.h; the warp takes its steps from j on
+__device__ inline void enter_row(Cursor& c, const Seqs& s, const AttendParams& p, int j, long long until) {
+    c.len = s.len[c.b];
+    c.lo = window_start(max(c.len, 0), p.window);
+    c.steps = (int)(s.pre[c.b + 1] - s.pre[c.b]);
+    c.j = j;
+    c.end = c.steps <= kWhole ? c.steps : (int)min((long long)c.steps, until - c.row_at);
+}
+// false at the end of the warp's part
+__device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p, long long until) {
+    c.row_at += c.steps;
+    if (c.row_at >= until) return false;
+    if (++c.h == p.n_kv * p.tiles) {
+        c.h = 0;
+        if (++c.b == p.n_seqs) return false;
     }
-    for (int j = lo; j < len; ++j) {
-        const int page = p.table[b * p.table_stride + j / p.page_size];
-        if (page < 0 || page >= p.n_pages) {
-            bad = true;
-            break;
-        }
-        const Cache* k = (const Cache*)(p.k + page * p.k_page + (j % p.page_size) * p.k_slot + kv * p.k_head);
-        const Cache* v = (const Cache*)(p.v + page * p.v_page + (j % p.page_size) * p.v_slot + kv * p.v_head);
-        float s = 0.f;
-        for (int i = 0; i < N; ++i)
-            if (lane + 32 * i < p.dim) s += q[i] * sb_to_float(k[lane + 32 * i]);
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-        s *= p.scale_log2;
-        const float top = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - top), e = exp2f(s - top);
-        m = top;
-        l *= a;
-        lb = lb * a + e;
-        for (int i = 0; i < N; ++i)
-            if (lane + 32 * i < p.dim) {
-                o[i] *= a;
-                ob[i] = ob[i] * a + e * sb_to_float(v[lane + 32 * i]);
+    enter_row(c, s, p, 0, until);
+    return true;
+}
+
+// ------------------------------------------------------------ the kernel
+// QP: parts of a query value (1: it has the cache's type), PP: of a weight
+template <class Cache, int DP, int QP, int PP>
+__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const AttendParams p) {
+    using S = Shape<DP>;
+    using Act = typename std::conditional<QP == 1, Cache, float>::type;
+    constexpr float kUp = std::is_same<Cache, __half>::value ? 12.f : 0.f;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- the scan of the lengths
+    Seqs seqs{(long long*)smem, (int*)(smem + 8 * (p.n_seqs + 1))};
+    __shared__ long long warp_sum[32];
+    {
+        const int per = (p.n_seqs + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per;
+        long long sum = 0;
+        for (int b = b0; b < min(b0 + per, p.n_seqs); ++b) {
+            int len = p.lens[b];
+            if (len < 0 || len > (long long)p.table_width * p.page_size) {
+                len = -1;
+                if (blockIdx.x == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
             }
-        if ((j - lo) % kBlock == kBlock - 1 || j == len - 1) {
-            l += lb;
-            lb = 0.f;
-            for (int i = 0; i < N; ++i) {
-                o[i] += ob[i];
-                ob[i] = 0.f;
-            }
+            seqs.len[b] = len;
+            sum += seq_steps(len, p.window);
         }
+        long long run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(~0u, run, o);
+            if (lane >= o) run += x;
+        }
+        if (lane == 31) warp_sum[wid] = run;
+        __syncthreads();
+        run -= sum;
+        for (int w = 0; w < wid; ++w) run += warp_sum[w];
+        for (int b = b0; b < min(b0 + per, p.n_seqs); ++b) {
+            seqs.pre[b] = run;
+            run += seq_steps(seqs.len[b], p.window);
+        }
+        if (b0 < p.n_seqs && b0 + per >= p.n_seqs) seqs.pre[p.n_seqs] = run;
+        __syncthreads();
     }
-    if (bad && lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
-    const float nan = __int_as_float(0x7fc00000);
-    for (int i = 0; i < N; ++i)
-        if (lane + 32 * i < p.dim)
-            ((Act*)p.out)[((size_t)b * p.n_q + h) * p.dim + lane + 32 * i] =
-                sb_from_float<Act>(bad ? nan : len == lo ? 0.f : o[i] / l);
-    if (p.lse && lane == 0)
-        p.lse[(size_t)b * p.n_q + h] = bad ? nan : len == lo ? -INFINITY : 0.69314718f * (m + log2f(l));
+
+    // ---- this warp's part of the list; neighbours in it sit on different SMs
+    const int w = wid * gridDim.x + blockIdx.x, n_rows = p.n_kv * p.tiles;
+    const long long total = seqs.pre[p.n_seqs] * n_rows, all_warps = (long long)gridDim.x * n_warps;
+    const long long part = max((total + all_warps - 1) / all_warps, (long long)kMinSteps);
+    const long long from = w * part, until = min(from + part, total);
+    if (lane == 0) p.cuts[w] = make_int2(-1, 0);
+    if (from >= total) return;
+    Cursor cc;
+    {
+        int a = 0, z = p.n_seqs - 1;   // the last sequence that starts at or before `from`
+        while (a < z) {
+            const int mid = (a + z + 1) / 2;
+            if (seqs.pre[mid] * n_rows <= from) a = mid;
+            else z = mid - 1;
+        }
+        cc.b = a;
+        const long long at = from - seqs.pre[a] * n_rows, steps = seqs.pre[a + 1] - seqs.pre[a];
+        cc.h = (int)(at / steps);
+        const int j = (int)(at % steps);
+        cc.row_at = from - j;
+        enter_row(cc, seqs, p, j, until);
+        // a whole row is its first step's warp's
+        if (cc.steps <= kWhole && j > 0 && !next_row(cc, seqs, p, until)) return;
+    }
+
+    // ---- shared memory of this warp: the ring, then the query rows
+    const int rows = min(p.group, 16);
+    const uint32_t q_bytes = (uint32_t)rows * QP * S::kRow;
+    const uint32_t head = (12 * p.n_seqs + 8 + 15) / 16 * 16;
+    uint8_t* mine = smem + head + wid * (S::kStages * S::kStage + q_bytes);
+    const uint32_t ring = smem_addr(mine), qs = ring + S::kStages * S::kStage;
+    if (p.dim < DP) {   // columns past the head size stay zero
+        const int pad = (DP - p.dim) / 8, n = (S::kStages * 2 * kStep + rows * QP) * pad;
+        for (int i = lane; i < n; i += 32)
+            *(uint4*)(mine + i / pad * S::kRow + (p.dim + i % pad * 8) * 2) = make_uint4(0, 0, 0, 0);
+    }
+
+    // ---- the loading side
+    const int copy_lane = lane % S::kLanes, copy_row = lane / S::kLanes;
+    const bool copies = copy_lane * 8 < p.dim;
+    const uint8_t* nowhere = (const uint8_t*)p.pieces;   // an address for copies of no bytes
+    Cursor pc = cc;
+    bool more = true;
+    int page = -1;             // lane < 16: the page of this step's key `lane`, -1 outside the window
+    uint32_t bad_steps = 0;    // bit per ring stage: the step met a page out of range
+    auto fetch_page = [&]() {
+        page = -1;
+        const int key = (max(pc.lo, 0) / kStep + pc.j) * kStep + lane;
+        if (more && lane < kStep && key >= pc.lo && key < pc.len)
+            page = p.table[pc.b * p.table_stride + key / p.page_size];
+        else if (lane < kStep)
+            page = -2;
+    };
+    fetch_page();
+    auto issue = [&](int stage) {
+        if (more) {
+            const int key = (pc.lo / kStep + pc.j) * kStep + lane;
+            const bool bad = lane < kStep && page != -2 && (page < 0 || page >= p.n_pages);
+            const bool any_bad = __any_sync(~0u, bad);
+            if (any_bad && lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
+            bad_steps = (bad_steps & ~(1u << stage)) | (any_bad ? 1u << stage : 0u);
+            const bool real = lane < kStep && page >= 0 && !bad;
+            const int kv = pc.h / p.tiles;
+            const unsigned slot = real ? (unsigned)key % (unsigned)p.page_size : 0;
+            const long long ko = real ? (long long)(page * p.k_page + slot * p.k_slot + kv * p.k_head) : -1;
+            const long long vo = real ? (long long)(page * p.v_page + slot * p.v_slot + kv * p.v_head) : -1;
+            const uint32_t dst = ring + stage * S::kStage + copy_lane * 16;
+#pragma unroll
+            for (int i = 0; i < kStep * S::kLanes / 32; ++i) {
+                const int r = i * (32 / S::kLanes) + copy_row;
+                const long long a = __shfl_sync(~0u, ko, r);
+                if (copies) copy16(dst + r * S::kRow, a < 0 ? nowhere : p.k + a + copy_lane * 16, a >= 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kStep * S::kLanes / 32; ++i) {
+                const int r = i * (32 / S::kLanes) + copy_row;
+                const long long a = __shfl_sync(~0u, vo, r);
+                if (copies) copy16(dst + (kStep + r) * S::kRow, a < 0 ? nowhere : p.v + a + copy_lane * 16, a >= 0);
+            }
+            if (++pc.j == pc.end) more = next_row(pc, seqs, p, until);
+            fetch_page();   // its latency passes while the warp computes
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+
+    // ---- the computing side
+    const int g = lane >> 2, quad = lane & 3;
+    float o[DP / 8][4], m[2], l[2], unscale[2];
+    bool row_bad = false;
+    const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * S::kRow + ((lane >> 3) & 1) * 16;
+    const uint32_t v_lane = kStep * S::kRow + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::kRow + (lane >> 4) * 16;
+    int stage = 0;
+    for (bool live = true; live;) {
+        // queries of this row, split into parts
+        const int first_head = cc.h / p.tiles * p.group + cc.h % p.tiles * 16;
+        const int heads = min(16, p.group - cc.h % p.tiles * 16);
+        const uint32_t q_lane = qs + min((int)(lane & 15), heads - 1) * S::kRow + (lane >> 4) * 16;
+        __syncwarp();
+        unscale[0] = unscale[1] = 1.f;
+        for (int r = 0; r < heads; ++r) {
+            const Act* src = (const Act*)(p.q + cc.b * p.q_seq + (size_t)(first_head + r) * p.q_head);
+            uint8_t* dst = mine + S::kStages * S::kStage + r * S::kRow;
+            if constexpr (QP == 1) {
+#pragma unroll
+                for (int i = 0; i < (DP + 31) / 32; ++i) {
+                    const int d = lane + 32 * i;
+                    if (d < p.dim) ((Act*)dst)[d] = src[d];
+                }
+            } else {
+                float x[(DP + 31) / 32], top = 0.f;
+#pragma unroll
+                for (int i = 0; i < (DP + 31) / 32; ++i) {
+                    const int d = lane + 32 * i;
+                    x[i] = d < p.dim ? src[d] : 0.f;
+                    top = fmaxf(top, fabsf(x[i]));
+                }
+#pragma unroll
+                for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+                // 2^-e with 2^e <= top < 2^(e + 1); zero, infinite and NaN rows as they are
+                int e = (__float_as_int(top) >> 23) - 127;
+                e = top > 0.f && top < INFINITY ? min(max(e, -126), 126) : 0;
+                const float down = __int_as_float((127 - e) << 23);
+                if (r == g) unscale[0] = __int_as_float((127 + e) << 23);
+                if (r == g + 8) unscale[1] = __int_as_float((127 + e) << 23);
+#pragma unroll
+                for (int i = 0; i < (DP + 31) / 32; ++i) {
+                    const int d = lane + 32 * i;
+                    float rest = x[i] * down;
+#pragma unroll
+                    for (int s = 0; s < QP; ++s) {
+                        const uint32_t u = s < QP - 1 ? pack2<Cache, true>(rest, 0.f) : pack2<Cache, false>(rest, 0.f);
+                        rest -= unpack2<Cache>(u).x;
+                        if (d < p.dim) ((uint16_t*)(dst + s * rows * S::kRow))[d] = (uint16_t)u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+        row_bad = cc.len < 0;
+        const int first_j = cc.j;
+        for (; cc.j < cc.end; ++cc.j) {
+            copy_wait<S::kStages - 2>();
+            __syncwarp();   // and every lane has read the stage before, which the next copy fills
+            row_bad |= (bad_steps >> stage) & 1;
+            const uint32_t at = ring + stage * S::kStage;
+            issue(stage == 0 ? S::kStages - 1 : stage - 1);
+
+            // scores of 16 rows x 16 keys, in two chains: of a split query's
+            // first part and of its rest, else of every other 16 dimensions
+            float c[2][2][4];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) (&c[0][0][0])[x] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                uint32_t kf[4];
+                ldsm4(kf, at + k_lane + d * 32);
+#pragma unroll
+                for (int s = 0; s < QP; ++s) {
+                    uint32_t qf[4];
+                    ldsm4(qf, q_lane + s * rows * S::kRow + d * 32);
+                    const int chain = QP == 1 ? d & 1 : s != 0;
+                    mma16816<Cache>(c[chain][0], qf, kf[0], kf[1]);
+                    mma16816<Cache>(c[chain][1], qf, kf[2], kf[3]);
+                }
+            }
+            const int key0 = (cc.lo / kStep + cc.j) * kStep;
+            const bool edge = key0 < cc.lo || key0 + kStep > cc.len;
+            float alpha[2];
+            float pr[2][2][2];   // [row half][key tile][pair]
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float f = p.scale_log2 * unscale[r];
+                float top = m[r];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float a = c[0][t][2 * r + i], b = c[1][t][2 * r + i];
+                        float s = (QP == 1 ? a + b : add_rest(a, b)) * f;
+                        const int key = key0 + 8 * t + 2 * quad + i;
+                        if (edge && (key < cc.lo || key >= cc.len)) s = -INFINITY;
+                        pr[r][t][i] = s;
+                        top = fmaxf(top, s);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                const float base = top == -INFINITY ? 0.f : top;
+                alpha[r] = exp2_fast(m[r] - base);
+                m[r] = top;
+                float sum = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        pr[r][t][i] = exp2_fast(pr[r][t][i] - base + kUp);
+                        sum += pr[r][t][i];
+                    }
+                l[r] = l[r] * alpha[r] + sum;
+            }
+            // weights as the A operand, in parts: each what the ones before leave
+            uint32_t pf[PP][4];
+#pragma unroll
+            for (int s = 0; s < PP; ++s)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float* v = pr[x & 1][x >> 1];
+                    pf[s][x] = s < PP - 1 ? pack2<Cache, true>(v[0], v[1]) : pack2<Cache, false>(v[0], v[1]);
+                    const float2 hi = unpack2<Cache>(pf[s][x]);
+                    v[0] -= hi.x;
+                    v[1] -= hi.y;
+                }
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                uint32_t vf[4];
+                ldsm4t(vf, at + v_lane + d * 32);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816<Cache>(x, pf[0], vf[2 * t], vf[2 * t + 1]);
+#pragma unroll
+                    for (int s = 1; s < PP; ++s) mma16816<Cache>(y, pf[s], vf[2 * t], vf[2 * t + 1]);
+                    // the running sum is an fp32 fma, rounded to nearest
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[2 * d + t][i] = o[2 * d + t][i] * alpha[i >> 1] + add_rest(x[i], y[i]);
+                }
+            }
+            stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        }
+
+        // ---- the end of the row, or of this warp's part of it
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(~0u, l[r], 1);
+            l[r] += __shfl_xor_sync(~0u, l[r], 2);
+            if (row_bad) l[r] = __int_as_float(0x7fc00000);
+        }
+        const bool whole = first_j == 0 && cc.end == cc.steps;
+        float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
+        if (!whole && first_j == 0 && lane == 0)
+            p.cuts[w] = make_int2(cc.b * n_rows + cc.h,
+                                  (int)((cc.row_at + cc.steps - 1) / part - w + 1));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
+            if (row >= heads) continue;
+            if (whole) {
+                const size_t at = (size_t)cc.b * p.n_q + first_head + row;
+                const bool none = cc.len == cc.lo;
+                const float inv = none ? 0.f : 1.f / l[r];
+                Act* dst = (Act*)p.out + at * p.dim;
+#pragma unroll
+                for (int t = 0; t < DP / 8; ++t)
+                    if (t * 8 < p.dim) {
+                        const float a = o[t][2 * r] * inv, b = o[t][2 * r + 1] * inv;
+                        dst[t * 8 + 2 * quad] = sb_from_float<Act>(none ? 0.f : a);
+                        dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(none ? 0.f : b);
+                    }
+                if (p.lse && quad == 0)
+                    p.lse[at] = none ? -INFINITY : 0.69314718055994531f * (m[r] + (log2f(l[r]) - kUp));
+            } else {
+                if (quad == 0) {
+                    piece[row] = m[r];
+                    piece[16 + row] = l[r];
+                }
+#pragma unroll
+                for (int t = 0; t < DP / 8; ++t)
+                    *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(o[t][2 * r], o[t][2 * r + 1]);
+            }
+        }
+        live = next_row(cc, seqs, p, until);
+    }
+}
+
+// ------------------------------------------------------------ the join
+// One (cut row, query head) per CTA at a time: weights of its pieces from their
+// m and l, then the weighted sum of their rows, in the order of the keys.
+constexpr int kJoinThreads = 256, kJoinUnits = 16, kMaxPieces = 148 * 2 * 8;
+
+template <class Act, int DP>
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams p, int n_warps, float up) {
+    constexpr int kCols = DP / 4, kGroups = kJoinThreads / kCols;
+    __shared__ float weight[kMaxPieces];
+    __shared__ float red[kJoinThreads / 32 + 1];
+    __shared__ float4 sums[kGroups][kCols];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int heads_of = p.piece_rows, units = n_warps * heads_of;
+    // which of this CTA's units are cut rows
+    int2 cut = make_int2(-1, 0);
+    const int u = blockIdx.x + lane * gridDim.x;
+    if (lane < kJoinUnits && u < units) {
+        cut = p.cuts[u / heads_of];
+        const int tile = cut.x < 0 ? 0 : cut.x % p.tiles;
+        if (u % heads_of >= min(16, p.group - tile * 16)) cut.x = -1;
+    }
+    unsigned todo = __ballot_sync(~0u, cut.x >= 0);
+    auto block = [&](float v, bool is_max) {
+#pragma unroll
+        for (int s = 16; s; s >>= 1) {
+            const float x = __shfl_xor_sync(~0u, v, s);
+            v = is_max ? fmaxf(v, x) : v + x;
+        }
+        __syncthreads();
+        if (lane == 0) red[wid] = v;
+        __syncthreads();
+        v = red[0];
+        for (int i = 1; i < kJoinThreads / 32; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
+        return v;
+    };
+    for (; todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1;
+        const int row = __shfl_sync(~0u, cut.x, i), n = __shfl_sync(~0u, cut.y, i);
+        const int unit = blockIdx.x + i * gridDim.x, w = unit / heads_of, head = unit % heads_of;
+        auto piece = [&](int k) { return p.pieces + (size_t)(2 * (w + k) + (k == 0)) * p.piece_floats; };
+        float top = -INFINITY;
+        for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, piece(k)[head]);
+        top = block(top, true);
+        const float base = top == -INFINITY ? 0.f : top;
+        float l = 0.f;
+        for (int k = threadIdx.x; k < n; k += kJoinThreads) {
+            const float f = exp2_fast(piece(k)[head] - base);
+            weight[k] = f;
+            l += f * piece(k)[16 + head];
+        }
+        l = block(l, false);
+        const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (grp < kGroups) {
+#pragma unroll 4
+            for (int k = grp; k < n; k += kGroups) {
+                const float4 x = *(const float4*)(piece(k) + 32 + head * DP + col * 4);
+                const float f = weight[k];
+                a.x += f * x.x, a.y += f * x.y, a.z += f * x.z, a.w += f * x.w;
+            }
+            sums[grp][col] = a;
+        }
+        __syncthreads();
+        const int b = row / (p.n_kv * p.tiles), h = row % (p.n_kv * p.tiles);
+        const size_t at = (size_t)b * p.n_q + h / p.tiles * p.group + h % p.tiles * 16 + head;
+        if (grp == 0) {
+            for (int k = 1; k < kGroups; ++k) {
+                const float4 x = sums[k][col];
+                a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+            }
+            const float inv = 1.f / l;
+            Act* dst = (Act*)p.out + at * p.dim + col * 4;
+            if (col * 4 < p.dim) {
+                dst[0] = sb_from_float<Act>(a.x * inv);
+                dst[1] = sb_from_float<Act>(a.y * inv);
+                dst[2] = sb_from_float<Act>(a.z * inv);
+                dst[3] = sb_from_float<Act>(a.w * inv);
+            }
+        }
+        if (p.lse && threadIdx.x == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------ launches
+int sm_count() {
+    static int sms = 0;
+    if (!sms) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (sms < 1) sms = 148;
+        sms = std::min(sms, kMaxPieces / 8);
+    }
+    return sms;
+}
+int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+size_t cuts_bytes() { return ((size_t)sm_count() * 8 * sizeof(int2) + 255) / 256 * 256; }
+int piece_floats(int group, int dim) { return 32 + std::min(group, 16) * tile_width(dim); }
+
+template <class Cache, int DP, int QP, int PP>
+int launch(AttendParams p, cudaStream_t st) {
+    using S = Shape<DP>;
+    using Act = typename std::conditional<QP == 1, Cache, float>::type;
+    const int rows = std::min(p.group, 16);
+    const size_t per_warp = S::kStages * S::kStage + (size_t)rows * QP * S::kRow;
+    const size_t head = (12 * (size_t)p.n_seqs + 8 + 15) / 16 * 16;
+    // static shared memory (the scan's warp sums) is 256 bytes
+    const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 512 - head) / per_warp);
+    const size_t bytes = head + warps * per_warp;
+    static bool opted = false;
+    if (!opted) {
+        if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSmemLimit - 512), "attend shared memory"))
+            return -1;
+        opted = true;
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = sm_count();
+    cfg.blockDim = warps * 32;
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, PP>, (const AttendParams)p), "attend launch")) return -1;
+    const long long longest = std::min((long long)p.table_width * p.page_size,
+                                       p.window > 0 ? p.window + kStep - 1ll : 1ll << 40);
+    if (longest <= kWhole * kStep) return 0;   // no row can be cut
+    const int n_warps = sm_count() * warps;
+    cfg.gridDim = (n_warps * p.piece_rows + kJoinUnits - 1) / kJoinUnits;
+    cfg.blockDim = kJoinThreads;
+    cfg.dynamicSmemBytes = 0;
+    const float up = std::is_same<Cache, __half>::value ? 12.f : 0.f;
+    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act, DP>, (const AttendParams)p, n_warps, up), "attend join launch")
+               ? 0 : -1;
+}
+
+template <class Cache, int QP, int PP>
+int launch_dim(const AttendParams& p, cudaStream_t st) {
+    switch (tile_width(p.dim)) {
+    case 64: return launch<Cache, 64, QP, PP>(p, st);
+    case 96: return launch<Cache, 96, QP, PP>(p, st);
+    case 128: return launch<Cache, 128, QP, PP>(p, st);
+    case 192: return launch<Cache, 192, QP, PP>(p, st);
+    default: return launch<Cache, 256, QP, PP>(p, st);
+    }
 }
 
 }  // namespace
 
 SABAH_API size_t sabah_attend_paged_workspace(int n_q_heads, int n_kv_heads, int head_dim) {
-    (void)n_q_heads;
-    (void)n_kv_heads;
-    (void)head_dim;
-    return 0;
+    if (n_kv_heads <= 0 || n_q_heads <= 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
+    return cuts_bytes() + (size_t)sm_count() * 8 * 2 * piece_floats(n_q_heads / n_kv_heads, head_dim) * sizeof(float);
 }
 
 SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_head_stride, int act_type,
@@ -142,17 +710,33 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     p.lens = d_lens, p.n_seqs = n_seqs, p.n_q = n_q_heads, p.n_kv = n_kv_heads, p.dim = head_dim, p.window = window;
     p.scale_log2 = scale * 1.44269504088896341f;
     p.out = (uint8_t*)d_out, p.lse = d_lse, p.err = err;
-    (void)d_workspace;
-    (void)workspace_bytes;
+    if (!d_workspace || (uintptr_t)d_workspace % 16 ||
+        workspace_bytes < sabah_attend_paged_workspace(n_q_heads, n_kv_heads, head_dim)) {
+        sb_set_error("attend workspace of %zu bytes: %zu, 16-byte aligned, are needed", workspace_bytes,
+                     sabah_attend_paged_workspace(n_q_heads, n_kv_heads, head_dim));
+        return -1;
+    }
+    p.group = n_q_heads / n_kv_heads;
+    p.tiles = (p.group + 15) / 16;
+    p.piece_rows = std::min(p.group, 16);
+    p.piece_floats = piece_floats(p.group, head_dim);
+    p.cuts = (int2*)d_workspace;
+    p.pieces = (float*)((uint8_t*)d_workspace + cuts_bytes());
     const int slot = sb_timing_begin("attend_paged", st);
-    const unsigned grid = (unsigned)n_seqs * (unsigned)n_q_heads;
-    if (act_type == SB_F32)
-        cache_type == SB_F16 ? k_attend<float, __half><<<grid, 32, 0, st>>>(p)
-                             : k_attend<float, __nv_bfloat16><<<grid, 32, 0, st>>>(p);
-    else if (act_type == SB_F16)
-        k_attend<__half, __half><<<grid, 32, 0, st>>>(p);
-    else
-        k_attend<__nv_bfloat16, __nv_bfloat16><<<grid, 32, 0, st>>>(p);
+    int rc = 0;
+    for (int b = 0; b < n_seqs && rc == 0; b += kMaxSeqs) {
+        AttendParams a = p;
+        a.n_seqs = std::min(kMaxSeqs, n_seqs - b);
+        a.q += (size_t)b * q_seq_stride;
+        a.table += (size_t)b * p.table_stride;
+        a.lens += b;
+        a.out += (size_t)b * n_q_heads * head_dim * ab;
+        if (a.lse) a.lse += (size_t)b * n_q_heads;
+        if (act_type == SB_F32)
+            rc = cache_type == SB_F16 ? launch_dim<__half, 2, 2>(a, st) : launch_dim<__nv_bfloat16, 3, 3>(a, st);
+        else
+            rc = cache_type == SB_F16 ? launch_dim<__half, 1, 2>(a, st) : launch_dim<__nv_bfloat16, 1, 2>(a, st);
+    }
     sb_timing_end(slot, st);
-    return sb_cuda_ok(cudaGetLastError(), "attend launch") ? 0 : -1;
+    return rc;
 }
