@@ -51,9 +51,10 @@ constexpr int kSmemLimit = 227 * 1024;
 struct AttendParams {
     const uint8_t* q;
     size_t q_seq, q_head;   // bytes
+    int q_pairs;            // pairs of query values are aligned
     const uint8_t *k, *v;
     size_t k_page, k_slot, k_head, v_page, v_slot, v_head;   // bytes
-    int n_pages, page_size;
+    int n_pages, page_size, page_shift;   // shift: log2(page_size), or -1
     const int32_t* table;
     size_t table_stride;    // elements
     int table_width;
@@ -71,7 +72,10 @@ struct AttendParams {
 
 // ------------------------------------------------------------ PTX helpers
 __device__ inline uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ inline void copy16(uint32_t dst, const void* src, bool real) {   // zeros unless real
+__device__ inline void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ inline void copy16_or_zero(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ inline void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -89,7 +93,7 @@ __device__ inline void ldsm4t(uint32_t* r, uint32_t a) {
 }
 template <class T>
 __device__ inline void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+    if constexpr (std::is_same<T, __half>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -128,8 +132,23 @@ __device__ inline float2 unpack2(uint32_t u) {
         return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
+// the next part of (a, b), which keep what it leaves
+template <class T>
+__device__ inline uint32_t take_part(float& a, float& b, bool last) {
+    const uint32_t u = last ? pack2<T, false>(a, b) : pack2<T, true>(a, b);
+    const float2 f = unpack2<T>(u);
+    a -= f.x;
+    b -= f.y;
+    return u;
+}
+// e with 2^e <= x < 2^(e + 1); 0 for zero, infinity and NaN
+__device__ inline int exponent(float x) {
+    return x > 0.f && x < INFINITY ? min(max((__float_as_int(x) >> 23) - 127, -126), 126) : 0;
+}
+__device__ inline float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+
 // ------------------------------------------------------------ shapes
-// DP: head size rounded up to a tile width. The ring of one warp has `stages`
+// DP: head size rounded up to a tile width. Each warp has a ring of kStages
 // steps of 16 keys and 16 values.
 template <int DP>
 struct Shape {
@@ -140,7 +159,7 @@ struct Shape {
     static constexpr int kWarps = 8;                          // at most
 };
 
-// The lengths' scan: steps of sequences before b, for one key-value head.
+// The scan of the lengths: steps of the sequences before b, for one row of each.
 struct Seqs {
     long long* pre;   // [n_seqs + 1]
     int* len;         // [n_seqs], -1 where out of range
@@ -148,6 +167,10 @@ struct Seqs {
 __device__ inline int window_start(int len, int window) { return window > 0 ? max(0, len - window) : 0; }
 __device__ inline int seq_steps(int len, int window) {
     return len <= 0 ? 1 : (len + kStep - 1) / kStep - window_start(len, window) / kStep;
+}
+// a / b of non-negative numbers; the 64-bit division is a long subroutine
+__device__ inline long long div_fast(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
 // A place in the list of steps; each warp has one that loads and one that computes.
@@ -178,12 +201,143 @@ __device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p,
     return true;
 }
 
+// ------------------------------------------------------------ the loading side
+// One warp's copies into its ring, kStages - 1 steps ahead of its arithmetic.
+// Block table entries are held 32 to a register, one per lane, and the register
+// after the current one is always on its way, as are the first entries of this
+// sequence (the next key-value head starts there again) and of the next.
+template <int DP>
+struct Loader {
+    using S = Shape<DP>;
+    const AttendParams& p;
+    const Seqs& seqs;
+    const long long until;
+    const int lane;
+    const uint32_t ring;
+    Cursor c;
+    bool more = true;
+    uint32_t bad_steps = 0;             // bit per stage: the step met a page out of range
+    int first, cur, next, head, ahead;  // cur: entries first ..; next: the 32 after them
+
+    __device__ Loader(const AttendParams& p_, const Seqs& s_, long long until_, int lane_, uint32_t ring_, const Cursor& c_)
+        : p(p_), seqs(s_), until(until_), lane(lane_), ring(ring_), c(c_) {
+        first = entry_of((c.lo / kStep + c.j) * kStep);
+        cur = entries(c.b, first);
+        next = entries(c.b, first + 32);
+        head = entries(c.b, entry_of(c.lo / kStep * kStep));
+        ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
+    }
+    __device__ int entry_of(int key) const {
+        return p.page_shift >= 0 ? key >> p.page_shift : (int)((unsigned)key / (unsigned)p.page_size);
+    }
+    // table entries e .. e + 31 of sequence b that its window needs, -1 for the others
+    __device__ int entries(int b, int e) const {
+        const int len = seqs.len[b], lo = window_start(max(len, 0), p.window);
+        return len > lo && e + lane >= entry_of(lo) && e + lane <= entry_of(len - 1)
+                   ? __ldg(p.table + b * p.table_stride + e + lane) : -1;
+    }
+    __device__ int first_entries(int b) const {
+        const int lo = window_start(max(seqs.len[b], 0), p.window);
+        return entries(b, entry_of(lo / kStep * kStep));
+    }
+    __device__ int page_of(int e) const {   // e: per lane, first <= e < first + 64
+        const int a = __shfl_sync(~0u, cur, e - first), b = __shfl_sync(~0u, next, e - first);
+        return e - first < 32 ? a : b;
+    }
+    __device__ void advance() {
+        if (++c.j < c.end) return;
+        const int b = c.b;
+        more = next_row(c, seqs, p, until);
+        if (!more) return;
+        if (c.b != b) {
+            head = ahead;
+            ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
+        }
+        first = entry_of(c.lo / kStep * kStep);
+        cur = head;
+        next = entries(c.b, first + 32);
+    }
+    __device__ void issue(int stage) {
+        if (more) {
+            const int key0 = (c.lo / kStep + c.j) * kStep, kv = p.tiles == 1 ? c.h : c.h / p.tiles;
+            const int e0 = entry_of(key0);
+            if (e0 >= first + 32) {
+                first += 32;
+                cur = next;
+                next = entries(c.b, first + 32);
+            }
+            const int copy_lane = lane % S::kLanes, copy_row = lane / S::kLanes;
+            const bool copies = copy_lane * 8 < p.dim;
+            const uint32_t dst = ring + stage * S::kStage + copy_row * S::kRow + copy_lane * 16;
+            constexpr int kAtOnce = 32 / S::kLanes, kTimes = kStep / kAtOnce;
+            const uint8_t* nowhere = (const uint8_t*)p.pieces;   // an address for copies of no bytes
+            bool bad;
+            if (p.page_size % kStep == 0) {   // the step lies in one page
+                const int page = page_of(e0);
+                bad = (page < 0 || page >= p.n_pages) && c.len > c.lo;
+                const bool none = page < 0 || page >= p.n_pages;
+                const long long slot = key0 - e0 * p.page_size + copy_row;
+                const uint8_t* k = p.k + (none ? 0 : page) * p.k_page + slot * p.k_slot + kv * p.k_head + copy_lane * 16;
+                const uint8_t* v = p.v + (none ? 0 : page) * p.v_page + slot * p.v_slot + kv * p.v_head + copy_lane * 16;
+                if (!none && key0 >= c.lo && key0 + kStep <= c.len) {
+                    if (copies) {
+#pragma unroll
+                        for (int i = 0; i < kTimes; ++i, k += kAtOnce * p.k_slot) copy16(dst + i * kAtOnce * S::kRow, k);
+#pragma unroll
+                        for (int i = 0; i < kTimes; ++i, v += kAtOnce * p.v_slot)
+                            copy16(dst + (kStep + i * kAtOnce) * S::kRow, v);
+                    }
+                } else if (copies) {
+#pragma unroll
+                    for (int i = 0; i < kTimes; ++i, k += kAtOnce * p.k_slot, v += kAtOnce * p.v_slot) {
+                        const int key = key0 + i * kAtOnce + copy_row;
+                        const bool real = !none && key >= c.lo && key < c.len;
+                        copy16_or_zero(dst + i * kAtOnce * S::kRow, real ? k : nowhere, real);
+                        copy16_or_zero(dst + (kStep + i * kAtOnce) * S::kRow, real ? v : nowhere, real);
+                    }
+                }
+            } else {   // lane i finds key i's place, the lanes that copy it ask that lane
+                const int key = key0 + (lane & 15), inside = min(max(key, c.lo), max(c.len - 1, c.lo));
+                const int e = entry_of(inside), page = page_of(e);
+                const bool valid = key >= c.lo && key < c.len, out = page < 0 || page >= p.n_pages;
+                bad = __any_sync(~0u, valid && out);
+                const unsigned slot = (unsigned)inside - (unsigned)e * (unsigned)p.page_size;
+                const bool real = valid && !out;
+                const long long ko = real ? (long long)(page * p.k_page + slot * p.k_slot + kv * p.k_head) : -1;
+                const long long vo = real ? (long long)(page * p.v_page + slot * p.v_slot + kv * p.v_head) : -1;
+#pragma unroll
+                for (int i = 0; i < kTimes; ++i) {
+                    const int r = i * kAtOnce + copy_row;
+                    const long long a = __shfl_sync(~0u, ko, r), b = __shfl_sync(~0u, vo, r);
+                    if (!copies) continue;
+                    copy16_or_zero(dst + i * kAtOnce * S::kRow, a < 0 ? nowhere : p.k + a + copy_lane * 16, a >= 0);
+                    copy16_or_zero(dst + (kStep + i * kAtOnce) * S::kRow, a < 0 ? nowhere : p.v + b + copy_lane * 16, a >= 0);
+                }
+            }
+            bad_steps &= ~(1u << stage);
+            if (bad) {
+                bad_steps |= 1u << stage;
+                if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
+            }
+            advance();
+        }
+        copy_commit();
+    }
+};
+
 // ------------------------------------------------------------ the kernel
-// QP: parts of a query value (1: it has the cache's type), PP: of a weight
-template <class Cache, int DP, int QP, int PP>
+// QP: parts of a query value (1: it has the cache's type); the weights take as
+// many, and at least two. HALF: at most 8 query heads per key-value head; the
+// tile's rows 8-15 then hold the second parts of rows 0-7, so one MMA multiplies
+// both parts, and the query fragments stay in registers. With 9-16 heads each
+// part is an MMA of its own and the queries lie in shared memory.
+template <class Cache, int DP, int QP, bool HALF>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const AttendParams p) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
+    constexpr int PP = QP == 1 ? 2 : QP;
+    constexpr int R = HALF ? 1 : 2;          // row halves with heads of their own
+    constexpr int ND = DP / 16;
     constexpr float kUp = std::is_same<Cache, __half>::value ? 12.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
@@ -227,7 +381,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
     // ---- this warp's part of the list; neighbours in it sit on different SMs
     const int w = wid * gridDim.x + blockIdx.x, n_rows = p.n_kv * p.tiles;
     const long long total = seqs.pre[p.n_seqs] * n_rows, all_warps = (long long)gridDim.x * n_warps;
-    const long long part = max((total + all_warps - 1) / all_warps, (long long)kMinSteps);
+    const long long part = max(div_fast(total + all_warps - 1, all_warps), (long long)kMinSteps);
     const long long from = w * part, until = min(from + part, total);
     if (lane == 0) p.cuts[w] = make_int2(-1, 0);
     if (from >= total) return;
@@ -241,222 +395,267 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
         }
         cc.b = a;
         const long long at = from - seqs.pre[a] * n_rows, steps = seqs.pre[a + 1] - seqs.pre[a];
-        cc.h = (int)(at / steps);
-        const int j = (int)(at % steps);
+        cc.h = (int)div_fast(at, steps);
+        const int j = (int)(at - cc.h * steps);
         cc.row_at = from - j;
         enter_row(cc, seqs, p, j, until);
         // a whole row is its first step's warp's
         if (cc.steps <= kWhole && j > 0 && !next_row(cc, seqs, p, until)) return;
     }
 
-    // ---- shared memory of this warp: the ring, then the query rows
-    const int rows = min(p.group, 16);
-    const uint32_t q_bytes = (uint32_t)rows * QP * S::kRow;
+    // ---- shared memory of this warp: the ring, then (not HALF) the query rows
+    const int rows = min(p.group, 16), q_rows = HALF ? 0 : rows * QP;
     const uint32_t head = (12 * p.n_seqs + 8 + 15) / 16 * 16;
-    uint8_t* mine = smem + head + wid * (S::kStages * S::kStage + q_bytes);
-    const uint32_t ring = smem_addr(mine), qs = ring + S::kStages * S::kStage;
+    uint8_t* mine = smem + head + wid * (S::kStages * S::kStage + q_rows * S::kRow);
+    uint8_t* q_mem = mine + S::kStages * S::kStage;
+    const uint32_t ring = smem_addr(mine);
+    Loader<DP> loader(p, seqs, until, lane, ring, cc);
     if (p.dim < DP) {   // columns past the head size stay zero
-        const int pad = (DP - p.dim) / 8, n = (S::kStages * 2 * kStep + rows * QP) * pad;
+        const int pad = (DP - p.dim) / 8, n = (S::kStages * 2 * kStep + q_rows) * pad;
         for (int i = lane; i < n; i += 32)
             *(uint4*)(mine + i / pad * S::kRow + (p.dim + i % pad * 8) * 2) = make_uint4(0, 0, 0, 0);
     }
-
-    // ---- the loading side
-    const int copy_lane = lane % S::kLanes, copy_row = lane / S::kLanes;
-    const bool copies = copy_lane * 8 < p.dim;
-    const uint8_t* nowhere = (const uint8_t*)p.pieces;   // an address for copies of no bytes
-    Cursor pc = cc;
-    bool more = true;
-    int page = -1;             // lane < 16: the page of this step's key `lane`, -1 outside the window
-    uint32_t bad_steps = 0;    // bit per ring stage: the step met a page out of range
-    auto fetch_page = [&]() {
-        page = -1;
-        const int key = (max(pc.lo, 0) / kStep + pc.j) * kStep + lane;
-        if (more && lane < kStep && key >= pc.lo && key < pc.len)
-            page = p.table[pc.b * p.table_stride + key / p.page_size];
-        else if (lane < kStep)
-            page = -2;
-    };
-    fetch_page();
-    auto issue = [&](int stage) {
-        if (more) {
-            const int key = (pc.lo / kStep + pc.j) * kStep + lane;
-            const bool bad = lane < kStep && page != -2 && (page < 0 || page >= p.n_pages);
-            const bool any_bad = __any_sync(~0u, bad);
-            if (any_bad && lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
-            bad_steps = (bad_steps & ~(1u << stage)) | (any_bad ? 1u << stage : 0u);
-            const bool real = lane < kStep && page >= 0 && !bad;
-            const int kv = pc.h / p.tiles;
-            const unsigned slot = real ? (unsigned)key % (unsigned)p.page_size : 0;
-            const long long ko = real ? (long long)(page * p.k_page + slot * p.k_slot + kv * p.k_head) : -1;
-            const long long vo = real ? (long long)(page * p.v_page + slot * p.v_slot + kv * p.v_head) : -1;
-            const uint32_t dst = ring + stage * S::kStage + copy_lane * 16;
 #pragma unroll
-            for (int i = 0; i < kStep * S::kLanes / 32; ++i) {
-                const int r = i * (32 / S::kLanes) + copy_row;
-                const long long a = __shfl_sync(~0u, ko, r);
-                if (copies) copy16(dst + r * S::kRow, a < 0 ? nowhere : p.k + a + copy_lane * 16, a >= 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kStep * S::kLanes / 32; ++i) {
-                const int r = i * (32 / S::kLanes) + copy_row;
-                const long long a = __shfl_sync(~0u, vo, r);
-                if (copies) copy16(dst + (kStep + r) * S::kRow, a < 0 ? nowhere : p.v + a + copy_lane * 16, a >= 0);
-            }
-            if (++pc.j == pc.end) more = next_row(pc, seqs, p, until);
-            fetch_page();   // its latency passes while the warp computes
-        }
-        copy_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+    for (int i = 0; i < S::kStages - 1; ++i) loader.issue(i);
 
     // ---- the computing side
     const int g = lane >> 2, quad = lane & 3;
-    float o[DP / 8][4], m[2], l[2], unscale[2];
-    bool row_bad = false;
+    float o[DP / 8][2 * R], m[R], l[R], unscale[R];
+    uint32_t qf[HALF ? ND : 1][QP == 1 ? 2 : 2 * QP];   // HALF: per 16 dimensions, the parts of both 8s
     const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * S::kRow + ((lane >> 3) & 1) * 16;
     const uint32_t v_lane = kStep * S::kRow + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::kRow + (lane >> 4) * 16;
     int stage = 0;
     for (bool live = true; live;) {
-        // queries of this row, split into parts
-        const int first_head = cc.h / p.tiles * p.group + cc.h % p.tiles * 16;
-        const int heads = min(16, p.group - cc.h % p.tiles * 16);
-        const uint32_t q_lane = qs + min((int)(lane & 15), heads - 1) * S::kRow + (lane >> 4) * 16;
-        __syncwarp();
-        unscale[0] = unscale[1] = 1.f;
-        for (int r = 0; r < heads; ++r) {
-            const Act* src = (const Act*)(p.q + cc.b * p.q_seq + (size_t)(first_head + r) * p.q_head);
-            uint8_t* dst = mine + S::kStages * S::kStage + r * S::kRow;
+        const int tile = p.tiles == 1 ? 0 : cc.h % p.tiles, kv = p.tiles == 1 ? cc.h : cc.h / p.tiles;
+        const int first_head = kv * p.group + tile * 16, heads = min(16, p.group - tile * 16);
+        const uint8_t* q_row0 = p.q + cc.b * p.q_seq + first_head * p.q_head;
+
+        // ---- this row's queries, split into parts
+#pragma unroll
+        for (int r = 0; r < R; ++r) unscale[r] = 1.f;
+        if constexpr (HALF) {
+            const Act* src = (const Act*)(q_row0 + min(g, heads - 1) * p.q_head);
+            struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
+            Act x[ND][4];   // values 16 d + 2 quad + {0, 1, 8, 9}
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = 16 * d + 2 * quad + i * 8;
+                    Pair u{sb_from_float<Act>(0.f), sb_from_float<Act>(0.f)};
+                    if (at < p.dim) {
+                        if (p.q_pairs)
+                            u = *(const Pair*)(src + at);
+                        else
+                            u.a = src[at], u.b = src[at + 1];
+                    }
+                    x[d][2 * i] = u.a, x[d][2 * i + 1] = u.b;
+                }
             if constexpr (QP == 1) {
 #pragma unroll
-                for (int i = 0; i < (DP + 31) / 32; ++i) {
-                    const int d = lane + 32 * i;
-                    if (d < p.dim) ((Act*)dst)[d] = src[d];
-                }
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float a = sb_to_float(x[d][2 * i]), b = sb_to_float(x[d][2 * i + 1]);
+                        qf[d][i] = take_part<Cache>(a, b, true);
+                    }
             } else {
+                float top = 0.f;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[d][i]));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                const int e = exponent(top);
+                unscale[0] = power_of_two(e);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float a = x[d][2 * i] * power_of_two(-e), b = x[d][2 * i + 1] * power_of_two(-e);
+#pragma unroll
+                        for (int s = 0; s < QP; ++s) qf[d][i * QP + s] = take_part<Cache>(a, b, s == QP - 1);
+                    }
+            }
+        } else {
+            __syncwarp();
+            for (int r = 0; r < heads; ++r) {
+                const Act* src = (const Act*)(q_row0 + r * p.q_head);
                 float x[(DP + 31) / 32], top = 0.f;
 #pragma unroll
                 for (int i = 0; i < (DP + 31) / 32; ++i) {
                     const int d = lane + 32 * i;
-                    x[i] = d < p.dim ? src[d] : 0.f;
+                    x[i] = d < p.dim ? sb_to_float(src[d]) : 0.f;
                     top = fmaxf(top, fabsf(x[i]));
                 }
+                int e = 0;
+                if constexpr (QP > 1) {
 #pragma unroll
-                for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-                // 2^-e with 2^e <= top < 2^(e + 1); zero, infinite and NaN rows as they are
-                int e = (__float_as_int(top) >> 23) - 127;
-                e = top > 0.f && top < INFINITY ? min(max(e, -126), 126) : 0;
-                const float down = __int_as_float((127 - e) << 23);
-                if (r == g) unscale[0] = __int_as_float((127 + e) << 23);
-                if (r == g + 8) unscale[1] = __int_as_float((127 + e) << 23);
+                    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+                    e = exponent(top);
+                    if (r == g) unscale[0] = power_of_two(e);
+                    if (r == g + 8) unscale[R - 1] = power_of_two(e);
+                }
 #pragma unroll
                 for (int i = 0; i < (DP + 31) / 32; ++i) {
                     const int d = lane + 32 * i;
-                    float rest = x[i] * down;
+                    float rest = x[i] * power_of_two(-e), zero = 0.f;
 #pragma unroll
                     for (int s = 0; s < QP; ++s) {
-                        const uint32_t u = s < QP - 1 ? pack2<Cache, true>(rest, 0.f) : pack2<Cache, false>(rest, 0.f);
-                        rest -= unpack2<Cache>(u).x;
-                        if (d < p.dim) ((uint16_t*)(dst + s * rows * S::kRow))[d] = (uint16_t)u;
+                        const uint32_t u = take_part<Cache>(rest, zero, s == QP - 1);
+                        if (d < p.dim) ((uint16_t*)(q_mem + (s * rows + r) * S::kRow))[d] = (uint16_t)u;
                     }
                 }
             }
+            __syncwarp();
         }
-        __syncwarp();
+        const uint32_t q_lane = smem_addr(q_mem) + min(lane & 15, heads - 1) * S::kRow + (lane >> 4) * 16;
+
 #pragma unroll
         for (int t = 0; t < DP / 8; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
-        row_bad = cc.len < 0;
+            for (int i = 0; i < 2 * R; ++i) o[t][i] = 0.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+        }
+        bool row_bad = cc.len < 0;
         const int first_j = cc.j;
         for (; cc.j < cc.end; ++cc.j) {
             copy_wait<S::kStages - 2>();
             __syncwarp();   // and every lane has read the stage before, which the next copy fills
-            row_bad |= (bad_steps >> stage) & 1;
+            row_bad |= (loader.bad_steps >> stage) & 1;
             const uint32_t at = ring + stage * S::kStage;
-            issue(stage == 0 ? S::kStages - 1 : stage - 1);
+            loader.issue(stage == 0 ? S::kStages - 1 : stage - 1);
 
-            // scores of 16 rows x 16 keys, in two chains: of a split query's
-            // first part and of its rest, else of every other 16 dimensions
-            float c[2][2][4];
+            // ---- scores of the tile's rows and 16 keys: first the products of
+            // the first parts, and apart from them those of the rest
+            float sc[R][2][2];   // [row half][key tile][pair]
+            if constexpr (HALF) {
+                float c[2][2][4] = {}, e[2][4] = {};
 #pragma unroll
-            for (int x = 0; x < 16; ++x) (&c[0][0][0])[x] = 0.f;
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                uint32_t kf[4];
-                ldsm4(kf, at + k_lane + d * 32);
-#pragma unroll
-                for (int s = 0; s < QP; ++s) {
-                    uint32_t qf[4];
-                    ldsm4(qf, q_lane + s * rows * S::kRow + d * 32);
-                    const int chain = QP == 1 ? d & 1 : s != 0;
-                    mma16816<Cache>(c[chain][0], qf, kf[0], kf[1]);
-                    mma16816<Cache>(c[chain][1], qf, kf[2], kf[3]);
+                for (int d = 0; d < ND; ++d) {
+                    uint32_t kf[4];
+                    ldsm4(kf, at + k_lane + d * 32);
+                    const uint32_t qa[4] = {qf[d][0], qf[d][QP == 1 ? 0 : 1], qf[d][QP == 1 ? 1 : QP], qf[d][QP == 1 ? 1 : QP + 1]};
+                    mma16816<Cache>(c[d & 1][0], qa, kf[0], kf[1]);
+                    mma16816<Cache>(c[d & 1][1], qa, kf[2], kf[3]);
+                    if constexpr (QP == 3) {
+                        const uint32_t q3[4] = {qf[d][2], qf[d][2], qf[d][5], qf[d][5]};
+                        mma16816<Cache>(e[0], q3, kf[0], kf[1]);
+                        mma16816<Cache>(e[1], q3, kf[2], kf[3]);
+                    }
                 }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        sc[0][t][i] = c[0][t][i] + c[1][t][i];
+                        if constexpr (QP > 1)
+                            sc[0][t][i] = add_rest(sc[0][t][i], (c[0][t][2 + i] + c[1][t][2 + i]) + e[t][i]);
+                    }
+            } else {
+                float c[2][2][4] = {};
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    uint32_t kf[4];
+                    ldsm4(kf, at + k_lane + d * 32);
+#pragma unroll
+                    for (int s = 0; s < QP; ++s) {
+                        uint32_t qa[4];
+                        ldsm4(qa, q_lane + s * rows * S::kRow + d * 32);
+                        const int chain = QP == 1 ? d & 1 : s != 0;
+                        mma16816<Cache>(c[chain][0], qa, kf[0], kf[1]);
+                        mma16816<Cache>(c[chain][1], qa, kf[2], kf[3]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a = c[0][t][2 * r + i], b = c[1][t][2 * r + i];
+                            sc[r][t][i] = QP == 1 ? a + b : add_rest(a, b);
+                        }
             }
+
+            // ---- the running softmax
             const int key0 = (cc.lo / kStep + cc.j) * kStep;
             const bool edge = key0 < cc.lo || key0 + kStep > cc.len;
-            float alpha[2];
-            float pr[2][2][2];   // [row half][key tile][pair]
+            float alpha[R];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < R; ++r) {
                 const float f = p.scale_log2 * unscale[r];
                 float top = m[r];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float a = c[0][t][2 * r + i], b = c[1][t][2 * r + i];
-                        float s = (QP == 1 ? a + b : add_rest(a, b)) * f;
+                        sc[r][t][i] *= f;
                         const int key = key0 + 8 * t + 2 * quad + i;
-                        if (edge && (key < cc.lo || key >= cc.len)) s = -INFINITY;
-                        pr[r][t][i] = s;
-                        top = fmaxf(top, s);
+                        if (edge && (key < cc.lo || key >= cc.len)) sc[r][t][i] = -INFINITY;
+                        top = fmaxf(top, sc[r][t][i]);
                     }
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 const float base = top == -INFINITY ? 0.f : top;
                 alpha[r] = exp2_fast(m[r] - base);
                 m[r] = top;
-                float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        pr[r][t][i] = exp2_fast(pr[r][t][i] - base + kUp);
-                        sum += pr[r][t][i];
-                    }
-                l[r] = l[r] * alpha[r] + sum;
+                    for (int i = 0; i < 2; ++i) sc[r][t][i] = exp2_fast(sc[r][t][i] - base + kUp);
+                l[r] = l[r] * alpha[r] + ((sc[r][0][0] + sc[r][0][1]) + (sc[r][1][0] + sc[r][1][1]));
             }
-            // weights as the A operand, in parts: each what the ones before leave
-            uint32_t pf[PP][4];
-#pragma unroll
-            for (int s = 0; s < PP; ++s)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float* v = pr[x & 1][x >> 1];
-                    pf[s][x] = s < PP - 1 ? pack2<Cache, true>(v[0], v[1]) : pack2<Cache, false>(v[0], v[1]);
-                    const float2 hi = unpack2<Cache>(pf[s][x]);
-                    v[0] -= hi.x;
-                    v[1] -= hi.y;
-                }
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                uint32_t vf[4];
-                ldsm4t(vf, at + v_lane + d * 32);
+
+            // ---- weights as the A operand, in parts, times the values; the
+            // running sums are fp32 fmas, rounded to nearest
+            if constexpr (HALF) {
+                uint32_t w1[4], w2[4];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816<Cache>(x, pf[0], vf[2 * t], vf[2 * t + 1]);
+                    w1[2 * t] = take_part<Cache>(sc[0][t][0], sc[0][t][1], false);
+                    w1[2 * t + 1] = take_part<Cache>(sc[0][t][0], sc[0][t][1], PP == 2);
+                    if constexpr (PP == 3) w2[2 * t] = w2[2 * t + 1] = take_part<Cache>(sc[0][t][0], sc[0][t][1], true);
+                }
 #pragma unroll
-                    for (int s = 1; s < PP; ++s) mma16816<Cache>(y, pf[s], vf[2 * t], vf[2 * t + 1]);
-                    // the running sum is an fp32 fma, rounded to nearest
+                for (int d = 0; d < ND; ++d) {
+                    uint32_t vf[4];
+                    ldsm4t(vf, at + v_lane + d * 32);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[2 * d + t][i] = o[2 * d + t][i] * alpha[i >> 1] + add_rest(x[i], y[i]);
+                    for (int t = 0; t < 2; ++t) {
+                        float x[4] = {}, y[4] = {};
+                        mma16816<Cache>(x, w1, vf[2 * t], vf[2 * t + 1]);
+                        if constexpr (PP == 3) mma16816<Cache>(y, w2, vf[2 * t], vf[2 * t + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            o[2 * d + t][i] = o[2 * d + t][i] * alpha[0] + add_rest(x[i], PP == 3 ? x[2 + i] + y[i] : x[2 + i]);
+                    }
+                }
+            } else {
+                uint32_t wf[PP][4];
+#pragma unroll
+                for (int s = 0; s < PP; ++s)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        wf[s][x] = take_part<Cache>(sc[x & (R - 1)][x >> 1][0], sc[x & (R - 1)][x >> 1][1], s == PP - 1);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    uint32_t vf[4];
+                    ldsm4t(vf, at + v_lane + d * 32);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float x[4] = {}, y[4] = {};
+                        mma16816<Cache>(x, wf[0], vf[2 * t], vf[2 * t + 1]);
+#pragma unroll
+                        for (int s = 1; s < PP; ++s) mma16816<Cache>(y, wf[s], vf[2 * t], vf[2 * t + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2 * R; ++i)
+                            o[2 * d + t][i] = o[2 * d + t][i] * alpha[i >> 1] + add_rest(x[i], y[i]);
+                    }
                 }
             }
             stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -464,7 +663,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
 
         // ---- the end of the row, or of this warp's part of it
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < R; ++r) {
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
             if (row_bad) l[r] = __int_as_float(0x7fc00000);
@@ -472,31 +671,26 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
         const bool whole = first_j == 0 && cc.end == cc.steps;
         float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
         if (!whole && first_j == 0 && lane == 0)
-            p.cuts[w] = make_int2(cc.b * n_rows + cc.h,
-                                  (int)((cc.row_at + cc.steps - 1) / part - w + 1));
+            p.cuts[w] = make_int2(cc.b * n_rows + cc.h, (int)(div_fast(cc.row_at + cc.steps - 1, part) - w + 1));
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < R; ++r) {
             const int row = g + 8 * r;
             if (row >= heads) continue;
             if (whole) {
                 const size_t at = (size_t)cc.b * p.n_q + first_head + row;
                 const bool none = cc.len == cc.lo;
-                const float inv = none ? 0.f : 1.f / l[r];
+                const float inv = 1.f / l[r];
                 Act* dst = (Act*)p.out + at * p.dim;
 #pragma unroll
                 for (int t = 0; t < DP / 8; ++t)
                     if (t * 8 < p.dim) {
-                        const float a = o[t][2 * r] * inv, b = o[t][2 * r + 1] * inv;
-                        dst[t * 8 + 2 * quad] = sb_from_float<Act>(none ? 0.f : a);
-                        dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(none ? 0.f : b);
+                        dst[t * 8 + 2 * quad] = sb_from_float<Act>(none ? 0.f : o[t][2 * r] * inv);
+                        dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(none ? 0.f : o[t][2 * r + 1] * inv);
                     }
                 if (p.lse && quad == 0)
                     p.lse[at] = none ? -INFINITY : 0.69314718055994531f * (m[r] + (log2f(l[r]) - kUp));
             } else {
-                if (quad == 0) {
-                    piece[row] = m[r];
-                    piece[16 + row] = l[r];
-                }
+                if (quad == 0) *(float2*)(piece + 2 * row) = make_float2(m[r], l[r]);
 #pragma unroll
                 for (int t = 0; t < DP / 8; ++t)
                     *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(o[t][2 * r], o[t][2 * r + 1]);
@@ -507,88 +701,145 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
 }
 
 // ------------------------------------------------------------ the join
-// One (cut row, query head) per CTA at a time: weights of its pieces from their
-// m and l, then the weighted sum of their rows, in the order of the keys.
-constexpr int kJoinThreads = 256, kJoinUnits = 16, kMaxPieces = 148 * 2 * 8;
+// Pieces of a cut row, in the order of the keys: weights from their m and l,
+// then the weighted sum of their rows. Rows of few pieces are joined by a warp
+// per query head; rows of more by a CTA per query head and 64 columns, so that
+// all of a long row's pieces are read at once.
+constexpr int kJoinThreads = 256, kMaxWarps = 148 * 2 * 8, kFew = 4;
 
 template <class Act, int DP>
 __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams p, int n_warps, float up) {
-    constexpr int kCols = DP / 4, kGroups = kJoinThreads / kCols;
-    __shared__ float weight[kMaxPieces];
-    __shared__ float red[kJoinThreads / 32 + 1];
+    constexpr int kCols = DP % 64 ? 8 : 16, kSlices = DP / 4 / kCols, kGroups = kJoinThreads / kCols;
+    static_assert(kCols * kSlices * 4 == DP && kJoinThreads % kCols == 0, "columns divide the row and the CTA");
+    __shared__ float weight[kMaxWarps];
+    __shared__ short few[kMaxWarps], many[kMaxWarps];
+    __shared__ int count[2][kJoinThreads / 32];
+    __shared__ float red[2][kJoinThreads / 32];
     __shared__ float4 sums[kGroups][kCols];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int heads_of = p.piece_rows, units = n_warps * heads_of;
-    // which of this CTA's units are cut rows
-    int2 cut = make_int2(-1, 0);
-    const int u = blockIdx.x + lane * gridDim.x;
-    if (lane < kJoinUnits && u < units) {
-        cut = p.cuts[u / heads_of];
-        const int tile = cut.x < 0 ? 0 : cut.x % p.tiles;
-        if (u % heads_of >= min(16, p.group - tile * 16)) cut.x = -1;
-    }
-    unsigned todo = __ballot_sync(~0u, cut.x >= 0);
-    auto block = [&](float v, bool is_max) {
-#pragma unroll
-        for (int s = 16; s; s >>= 1) {
-            const float x = __shfl_xor_sync(~0u, v, s);
-            v = is_max ? fmaxf(v, x) : v + x;
+
+    // ---- the cut rows, in the order of the warps that begin them
+    const int per = (n_warps + kJoinThreads - 1) / kJoinThreads, w0 = wid * per * 32;
+    int n_few = 0, n_many = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        int at_few = 0, at_many = 0;
+        if (pass == 1)
+            for (int i = 0; i < kJoinThreads / 32; ++i) {
+                if (i == wid) at_few = n_few, at_many = n_many;
+                n_few += count[0][i];
+                n_many += count[1][i];
+            }
+        int c_few = 0, c_many = 0;
+        for (int i = 0; i < per; ++i) {
+            const int w = w0 + i * 32 + lane;
+            const int n = w < n_warps ? p.cuts[w].y : 0;
+            const unsigned f = __ballot_sync(~0u, n > 0 && n <= kFew), y = __ballot_sync(~0u, n > kFew);
+            const unsigned before = (1u << lane) - 1;
+            if (pass == 1) {
+                if (f >> lane & 1) few[at_few + __popc(f & before)] = (short)w;
+                if (y >> lane & 1) many[at_many + __popc(y & before)] = (short)w;
+                at_few += __popc(f);
+                at_many += __popc(y);
+            }
+            c_few += __popc(f);
+            c_many += __popc(y);
+        }
+        if (pass == 0 && lane == 0) {
+            count[0][wid] = c_few;
+            count[1][wid] = c_many;
         }
         __syncthreads();
-        if (lane == 0) red[wid] = v;
-        __syncthreads();
-        v = red[0];
-        for (int i = 1; i < kJoinThreads / 32; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
-        return v;
+    }
+    const int n_rows = p.n_kv * p.tiles;
+    auto place = [&](int row, int head, bool& real) -> size_t {   // of the output row
+        const int b = row / n_rows, h = row % n_rows, tile = h % p.tiles;
+        real = head < min(16, p.group - tile * 16);
+        return (size_t)b * p.n_q + h / p.tiles * p.group + tile * 16 + head;
     };
-    for (; todo; todo &= todo - 1) {
-        const int i = __ffs(todo) - 1;
-        const int row = __shfl_sync(~0u, cut.x, i), n = __shfl_sync(~0u, cut.y, i);
-        const int unit = blockIdx.x + i * gridDim.x, w = unit / heads_of, head = unit % heads_of;
-        auto piece = [&](int k) { return p.pieces + (size_t)(2 * (w + k) + (k == 0)) * p.piece_floats; };
+    auto piece = [&](int w, int k) { return p.pieces + (size_t)(2 * (w + k) + (k == 0)) * p.piece_floats; };
+
+    // ---- rows of many pieces
+    for (int u = blockIdx.x; u < n_many * p.piece_rows * kSlices; u += gridDim.x) {
+        const int w = many[u / (p.piece_rows * kSlices)], head = u / kSlices % p.piece_rows, slice = u % kSlices;
+        const int2 cut = p.cuts[w];
+        bool real;
+        const size_t at = place(cut.x, head, real);
+        if (!real) continue;
+        const int n = cut.y, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
         float top = -INFINITY;
-        for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, piece(k)[head]);
-        top = block(top, true);
+        for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, piece(w, k)[2 * head]);
+#pragma unroll
+        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+        if (lane == 0) red[0][wid] = top;
+        __syncthreads();
+        for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red[0][i]);
         const float base = top == -INFINITY ? 0.f : top;
         float l = 0.f;
         for (int k = threadIdx.x; k < n; k += kJoinThreads) {
-            const float f = exp2_fast(piece(k)[head] - base);
+            const float2 ml = *(const float2*)(piece(w, k) + 2 * head);
+            const float f = exp2_fast(ml.x - base);
             weight[k] = f;
-            l += f * piece(k)[16 + head];
+            l += f * ml.y;
         }
-        l = block(l, false);
-        const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+#pragma unroll
+        for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
+        if (lane == 0) red[1][wid] = l;
+        __syncthreads();
+        l = 0.f;
+        for (int i = 0; i < kJoinThreads / 32; ++i) l += red[1][i];
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (grp < kGroups) {
-#pragma unroll 4
-            for (int k = grp; k < n; k += kGroups) {
-                const float4 x = *(const float4*)(piece(k) + 32 + head * DP + col * 4);
-                const float f = weight[k];
-                a.x += f * x.x, a.y += f * x.y, a.z += f * x.z, a.w += f * x.w;
-            }
-            sums[grp][col] = a;
+#pragma unroll 8
+        for (int k = grp; k < n; k += kGroups) {
+            const float4 x = *(const float4*)(piece(w, k) + 32 + head * DP + (slice * kCols + col) * 4);
+            const float f = weight[k];
+            a.x += f * x.x, a.y += f * x.y, a.z += f * x.z, a.w += f * x.w;
         }
+        sums[grp][col] = a;
         __syncthreads();
-        const int b = row / (p.n_kv * p.tiles), h = row % (p.n_kv * p.tiles);
-        const size_t at = (size_t)b * p.n_q + h / p.tiles * p.group + h % p.tiles * 16 + head;
-        if (grp == 0) {
-            for (int k = 1; k < kGroups; ++k) {
-                const float4 x = sums[k][col];
-                a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-            }
-            const float inv = 1.f / l;
-            Act* dst = (Act*)p.out + at * p.dim + col * 4;
-            if (col * 4 < p.dim) {
-                dst[0] = sb_from_float<Act>(a.x * inv);
-                dst[1] = sb_from_float<Act>(a.y * inv);
-                dst[2] = sb_from_float<Act>(a.z * inv);
-                dst[3] = sb_from_float<Act>(a.w * inv);
-            }
+        if (threadIdx.x < kCols * 4) {   // one column per thread
+            const float* s = (const float*)sums + threadIdx.x;
+            float sum = 0.f;
+            for (int k = 0; k < kGroups; ++k) sum += s[k * kCols * 4];
+            const int d = slice * kCols * 4 + threadIdx.x;
+            if (d < p.dim) ((Act*)p.out)[at * p.dim + d] = sb_from_float<Act>(sum / l);
         }
-        if (p.lse && threadIdx.x == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
+        if (p.lse && slice == 0 && threadIdx.x == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
         __syncthreads();
+    }
+
+    // ---- rows of few
+    for (int u = blockIdx.x * (kJoinThreads / 32) + wid; u < n_few * p.piece_rows; u += gridDim.x * (kJoinThreads / 32)) {
+        const int w = few[u / p.piece_rows], head = u % p.piece_rows;
+        const int2 cut = p.cuts[w];
+        bool real;
+        const size_t at = place(cut.x, head, real);
+        if (!real) continue;
+        float2 ml[kFew];
+        float x[kFew][DP / 32];
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) {
+            ml[k] = k < cut.y ? *(const float2*)(piece(w, k) + 2 * head) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) x[k][i] = k < cut.y ? piece(w, k)[32 + head * DP + i * 32 + lane] : 0.f;
+        }
+        float top = ml[0].x;
+#pragma unroll
+        for (int k = 1; k < kFew; ++k) top = fmaxf(top, ml[k].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float l = 0.f, a[DP / 32] = {};
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) {
+            const float f = exp2_fast(ml[k].x - base);
+            l += f * ml[k].y;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) a[i] += k < cut.y ? f * x[k][i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+            if (i * 32 + lane < p.dim) ((Act*)p.out)[at * p.dim + i * 32 + lane] = sb_from_float<Act>(a[i] / l);
+        if (p.lse && lane == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
     }
 }
 
@@ -600,7 +851,7 @@ int sm_count() {
         cudaGetDevice(&dev);
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (sms < 1) sms = 148;
-        sms = std::min(sms, kMaxPieces / 8);
+        sms = std::min(sms, kMaxWarps / 8);
     }
     return sms;
 }
@@ -608,19 +859,19 @@ int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 
 size_t cuts_bytes() { return ((size_t)sm_count() * 8 * sizeof(int2) + 255) / 256 * 256; }
 int piece_floats(int group, int dim) { return 32 + std::min(group, 16) * tile_width(dim); }
 
-template <class Cache, int DP, int QP, int PP>
+template <class Cache, int DP, int QP, bool HALF>
 int launch(AttendParams p, cudaStream_t st) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
     const int rows = std::min(p.group, 16);
-    const size_t per_warp = S::kStages * S::kStage + (size_t)rows * QP * S::kRow;
+    const size_t per_warp = S::kStages * S::kStage + (HALF ? 0 : (size_t)rows * QP * S::kRow);
     const size_t head = (12 * (size_t)p.n_seqs + 8 + 15) / 16 * 16;
     // static shared memory (the scan's warp sums) is 256 bytes
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 512 - head) / per_warp);
     const size_t bytes = head + warps * per_warp;
     static bool opted = false;
     if (!opted) {
-        if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              kSmemLimit - 512), "attend shared memory"))
             return -1;
         opted = true;
@@ -635,12 +886,12 @@ int launch(AttendParams p, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, PP>, (const AttendParams)p), "attend launch")) return -1;
+    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, HALF>, (const AttendParams)p), "attend launch")) return -1;
     const long long longest = std::min((long long)p.table_width * p.page_size,
                                        p.window > 0 ? p.window + kStep - 1ll : 1ll << 40);
     if (longest <= kWhole * kStep) return 0;   // no row can be cut
     const int n_warps = sm_count() * warps;
-    cfg.gridDim = (n_warps * p.piece_rows + kJoinUnits - 1) / kJoinUnits;
+    cfg.gridDim = 2 * sm_count();
     cfg.blockDim = kJoinThreads;
     cfg.dynamicSmemBytes = 0;
     const float up = std::is_same<Cache, __half>::value ? 12.f : 0.f;
@@ -648,15 +899,19 @@ int launch(AttendParams p, cudaStream_t st) {
                ? 0 : -1;
 }
 
-template <class Cache, int QP, int PP>
+template <class Cache, int QP, bool HALF>
 int launch_dim(const AttendParams& p, cudaStream_t st) {
     switch (tile_width(p.dim)) {
-    case 64: return launch<Cache, 64, QP, PP>(p, st);
-    case 96: return launch<Cache, 96, QP, PP>(p, st);
-    case 128: return launch<Cache, 128, QP, PP>(p, st);
-    case 192: return launch<Cache, 192, QP, PP>(p, st);
-    default: return launch<Cache, 256, QP, PP>(p, st);
+    case 64: return launch<Cache, 64, QP, HALF>(p, st);
+    case 96: return launch<Cache, 96, QP, HALF>(p, st);
+    case 128: return launch<Cache, 128, QP, HALF>(p, st);
+    case 192: return launch<Cache, 192, QP, HALF>(p, st);
+    default: return launch<Cache, 256, QP, HALF>(p, st);
     }
+}
+template <class Cache, int QP>
+int launch_group(const AttendParams& p, cudaStream_t st) {
+    return p.group <= 8 ? launch_dim<Cache, QP, true>(p, st) : launch_dim<Cache, QP, false>(p, st);
 }
 
 }  // namespace
@@ -702,10 +957,12 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     }
     AttendParams p{};
     p.q = (const uint8_t*)d_q, p.q_seq = q_seq_stride, p.q_head = q_head_stride;
+    p.q_pairs = ((uintptr_t)d_q | q_seq_stride | q_head_stride) % (2 * ab) == 0;
     p.k = (const uint8_t*)d_k_cache, p.v = (const uint8_t*)d_v_cache;
     p.k_page = k_page_stride, p.k_slot = k_slot_stride, p.k_head = k_head_stride;
     p.v_page = v_page_stride, p.v_slot = v_slot_stride, p.v_head = v_head_stride;
     p.n_pages = n_pages, p.page_size = page_size;
+    p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
     p.table = d_block_table, p.table_stride = table_stride / 4, p.table_width = table_width;
     p.lens = d_lens, p.n_seqs = n_seqs, p.n_q = n_q_heads, p.n_kv = n_kv_heads, p.dim = head_dim, p.window = window;
     p.scale_log2 = scale * 1.44269504088896341f;
@@ -733,9 +990,9 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
         a.out += (size_t)b * n_q_heads * head_dim * ab;
         if (a.lse) a.lse += (size_t)b * n_q_heads;
         if (act_type == SB_F32)
-            rc = cache_type == SB_F16 ? launch_dim<__half, 2, 2>(a, st) : launch_dim<__nv_bfloat16, 3, 3>(a, st);
+            rc = cache_type == SB_F16 ? launch_group<__half, 2>(a, st) : launch_group<__nv_bfloat16, 3>(a, st);
         else
-            rc = cache_type == SB_F16 ? launch_dim<__half, 1, 2>(a, st) : launch_dim<__nv_bfloat16, 1, 2>(a, st);
+            rc = cache_type == SB_F16 ? launch_group<__half, 1>(a, st) : launch_group<__nv_bfloat16, 1>(a, st);
     }
     sb_timing_end(slot, st);
     return rc;
