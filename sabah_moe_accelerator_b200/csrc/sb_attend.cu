@@ -46,6 +46,7 @@ constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in 
 constexpr int kStep = 16;        // keys per step
 constexpr int kWhole = 8;        // rows of at most this many steps are never cut
 constexpr int kMinSteps = 4;     // and a part is at least this long
+constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps
 constexpr int kSmemLimit = 227 * 1024;
 
 struct AttendParams {
@@ -159,7 +160,9 @@ struct Shape {
     static constexpr int kWarps = 8;                          // at most
 };
 
-// The scan of the lengths: steps of the sequences before b, for one row of each.
+// The scan of the lengths: cost of the sequences before b, for one row of each.
+// A row takes its steps, then kRowCost idle places in the list, so that parts
+// of many short rows and parts of one long row take as long.
 struct Seqs {
     long long* pre;   // [n_seqs + 1]
     int* len;         // [n_seqs], -1 where out of range
@@ -185,13 +188,13 @@ struct Cursor {
 __device__ inline void enter_row(Cursor& c, const Seqs& s, const AttendParams& p, int j, long long until) {
     c.len = s.len[c.b];
     c.lo = window_start(max(c.len, 0), p.window);
-    c.steps = (int)(s.pre[c.b + 1] - s.pre[c.b]);
+    c.steps = (int)(s.pre[c.b + 1] - s.pre[c.b]) - kRowCost;
     c.j = j;
     c.end = c.steps <= kWhole ? c.steps : (int)min((long long)c.steps, until - c.row_at);
 }
 // false at the end of the warp's part
 __device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p, long long until) {
-    c.row_at += c.steps;
+    c.row_at += c.steps + kRowCost;
     if (c.row_at >= until) return false;
     if (++c.h == p.n_kv * p.tiles) {
         c.h = 0;
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
                 if (blockIdx.x == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
             }
             seqs.len[b] = len;
-            sum += seq_steps(len, p.window);
+            sum += seq_steps(len, p.window) + kRowCost;
         }
         long long run = sum;
 #pragma unroll
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
         for (int w = 0; w < wid; ++w) run += warp_sum[w];
         for (int b = b0; b < min(b0 + per, p.n_seqs); ++b) {
             seqs.pre[b] = run;
-            run += seq_steps(seqs.len[b], p.window);
+            run += seq_steps(seqs.len[b], p.window) + kRowCost;
         }
         if (b0 < p.n_seqs && b0 + per >= p.n_seqs) seqs.pre[p.n_seqs] = run;
         __syncthreads();
@@ -387,20 +390,23 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
     if (from >= total) return;
     Cursor cc;
     {
-        int a = 0, z = p.n_seqs - 1;   // the last sequence that starts at or before `from`
-        while (a < z) {
-            const int mid = (a + z + 1) / 2;
-            if (seqs.pre[mid] * n_rows <= from) a = mid;
-            else z = mid - 1;
+        // the last sequence that starts at or before `from`: 32 probes at a time
+        int a = 0, span = p.n_seqs;   // it is in [a, a + span)
+        while (span > 1) {
+            const int hop = (span + 31) / 32, at = a + lane * hop;
+            const unsigned hit = __ballot_sync(~0u, at < a + span && seqs.pre[min(at, p.n_seqs)] * n_rows <= from);
+            const int last = 31 - __clz(hit);
+            span = min(hop, a + span - (a + last * hop));
+            a += last * hop;
         }
         cc.b = a;
-        const long long at = from - seqs.pre[a] * n_rows, steps = seqs.pre[a + 1] - seqs.pre[a];
-        cc.h = (int)div_fast(at, steps);
-        const int j = (int)(at - cc.h * steps);
+        const long long at = from - seqs.pre[a] * n_rows, cost = seqs.pre[a + 1] - seqs.pre[a];
+        cc.h = (int)div_fast(at, cost);
+        const int j = (int)(at - cc.h * cost);
         cc.row_at = from - j;
         enter_row(cc, seqs, p, j, until);
         // a whole row is its first step's warp's
-        if (cc.steps <= kWhole && j > 0 && !next_row(cc, seqs, p, until)) return;
+        if ((j >= cc.steps || (cc.steps <= kWhole && j > 0)) && !next_row(cc, seqs, p, until)) return;
     }
 
     // ---- shared memory of this warp: the ring, then (not HALF) the query rows
@@ -409,6 +415,34 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
     uint8_t* mine = smem + head + wid * (S::kStages * S::kStage + q_rows * S::kRow);
     uint8_t* q_mem = mine + S::kStages * S::kStage;
     const uint32_t ring = smem_addr(mine);
+    const int g = lane >> 2, quad = lane & 3;
+    Act qx[HALF ? ND : 1][4];   // the row's query values 16 d + 2 quad + {0, 1, 8, 9}, as they are
+    auto fetch_queries = [&](const Cursor& c) {
+        if constexpr (HALF) {
+            const int first = c.h * p.group, heads = p.group;
+            const Act* src = (const Act*)(p.q + c.b * p.q_seq + (first + min(g, heads - 1)) * p.q_head);
+            if (p.q_pairs) {
+                struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = 16 * d + 2 * quad + i * 8;
+                        const Pair u = *(const Pair*)(src + (at < p.dim ? at : 0));
+                        qx[d][2 * i] = u.a, qx[d][2 * i + 1] = u.b;
+                    }
+            } else {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 16 * d + 2 * quad + (i & 1) + (i >> 1) * 8;
+                        qx[d][i] = src[at < p.dim ? at : 0];
+                    }
+            }
+        }
+    };
+    fetch_queries(cc);
     Loader<DP> loader(p, seqs, until, lane, ring, cc);
     if (p.dim < DP) {   // columns past the head size stay zero
         const int pad = (DP - p.dim) / 8, n = (S::kStages * 2 * kStep + q_rows) * pad;
@@ -419,7 +453,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
     for (int i = 0; i < S::kStages - 1; ++i) loader.issue(i);
 
     // ---- the computing side
-    const int g = lane >> 2, quad = lane & 3;
     float o[DP / 8][2 * R], m[R], l[R], unscale[R];
     uint32_t qf[HALF ? ND : 1][QP == 1 ? 2 : 2 * QP];   // HALF: per 16 dimensions, the parts of both 8s
     const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * S::kRow + ((lane >> 3) & 1) * 16;
@@ -434,29 +467,16 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
 #pragma unroll
         for (int r = 0; r < R; ++r) unscale[r] = 1.f;
         if constexpr (HALF) {
-            const Act* src = (const Act*)(q_row0 + min(g, heads - 1) * p.q_head);
-            struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
-            Act x[ND][4];   // values 16 d + 2 quad + {0, 1, 8, 9}
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int at = 16 * d + 2 * quad + i * 8;
-                    Pair u{sb_from_float<Act>(0.f), sb_from_float<Act>(0.f)};
-                    if (at < p.dim) {
-                        if (p.q_pairs)
-                            u = *(const Pair*)(src + at);
-                        else
-                            u.a = src[at], u.b = src[at + 1];
-                    }
-                    x[d][2 * i] = u.a, x[d][2 * i + 1] = u.b;
-                }
+            // values past the head size are zero
+            auto value = [&](int d, int i) {
+                return 16 * d + 2 * quad + (i >> 1) * 8 < p.dim ? sb_to_float(qx[d][i]) : 0.f;
+            };
             if constexpr (QP == 1) {
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float a = sb_to_float(x[d][2 * i]), b = sb_to_float(x[d][2 * i + 1]);
+                        float a = value(d, 2 * i), b = value(d, 2 * i + 1);
                         qf[d][i] = take_part<Cache>(a, b, true);
                     }
             } else {
@@ -464,7 +484,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[d][i]));
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(value(d, i)));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 const int e = exponent(top);
@@ -473,7 +493,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float a = x[d][2 * i] * power_of_two(-e), b = x[d][2 * i + 1] * power_of_two(-e);
+                        float a = value(d, 2 * i) * power_of_two(-e), b = value(d, 2 * i + 1) * power_of_two(-e);
 #pragma unroll
                         for (int s = 0; s < QP; ++s) qf[d][i * QP + s] = take_part<Cache>(a, b, s == QP - 1);
                     }
@@ -661,24 +681,28 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
             stage = stage + 1 == S::kStages ? 0 : stage + 1;
         }
 
-        // ---- the end of the row, or of this warp's part of it
+        // ---- the end of the row, or of this warp's part of it; the next row's
+        // queries are on their way meanwhile, where there are registers for them
+        const Cursor done = cc;
+        live = next_row(cc, seqs, p, until);
+        if (DP <= 128 && live) fetch_queries(cc);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
             if (row_bad) l[r] = __int_as_float(0x7fc00000);
         }
-        const bool whole = first_j == 0 && cc.end == cc.steps;
+        const bool whole = first_j == 0 && done.end == done.steps;
         float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
         if (!whole && first_j == 0 && lane == 0)
-            p.cuts[w] = make_int2(cc.b * n_rows + cc.h, (int)(div_fast(cc.row_at + cc.steps - 1, part) - w + 1));
+            p.cuts[w] = make_int2(done.b * n_rows + done.h, (int)(div_fast(done.row_at + done.steps - 1, part) - w + 1));
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int row = g + 8 * r;
             if (row >= heads) continue;
             if (whole) {
-                const size_t at = (size_t)cc.b * p.n_q + first_head + row;
-                const bool none = cc.len == cc.lo;
+                const size_t at = (size_t)done.b * p.n_q + first_head + row;
+                const bool none = done.len == done.lo;
                 const float inv = 1.f / l[r];
                 Act* dst = (Act*)p.out + at * p.dim;
 #pragma unroll
@@ -696,150 +720,132 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
                     *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(o[t][2 * r], o[t][2 * r + 1]);
             }
         }
-        live = next_row(cc, seqs, p, until);
+        if (DP > 128 && live) fetch_queries(cc);
     }
 }
 
 // ------------------------------------------------------------ the join
 // Pieces of a cut row, in the order of the keys: weights from their m and l,
-// then the weighted sum of their rows. Rows of few pieces are joined by a warp
-// per query head; rows of more by a CTA per query head and 64 columns, so that
-// all of a long row's pieces are read at once.
-constexpr int kJoinThreads = 256, kMaxWarps = 148 * 2 * 8, kFew = 4;
+// then the weighted sum of their rows. A unit is a query head of a cut row and
+// 32 of its columns, one per lane. Latency is all there is to it, so a unit is
+// joined by one warp where its row has at most 32 pieces and by the eight warps
+// of a CTA where it has more, with the pieces' loads in flight together.
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kMaxWarps = 148 * 2 * 8, kFew = 32;
 
 template <class Act, int DP>
 __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams p, int n_warps, float up) {
-    constexpr int kCols = DP % 64 ? 8 : 16, kSlices = DP / 4 / kCols, kGroups = kJoinThreads / kCols;
-    static_assert(kCols * kSlices * 4 == DP && kJoinThreads % kCols == 0, "columns divide the row and the CTA");
-    __shared__ float weight[kMaxWarps];
-    __shared__ short few[kMaxWarps], many[kMaxWarps];
-    __shared__ int count[2][kJoinThreads / 32];
-    __shared__ float red[2][kJoinThreads / 32];
-    __shared__ float4 sums[kGroups][kCols];
+    constexpr int kSlices = DP / 32, kPer = kMaxWarps / kJoinThreads + 1;
+    __shared__ short few[kMaxWarps], many[kMaxWarps];   // the warps that begin a cut row
+    __shared__ int counts[2][kPer * kJoinWarps];
+    __shared__ float red[2][kJoinWarps], sums[kJoinWarps][32];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ---- the cut rows, in the order of the warps that begin them
-    const int per = (n_warps + kJoinThreads - 1) / kJoinThreads, w0 = wid * per * 32;
     int n_few = 0, n_many = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        int at_few = 0, at_many = 0;
-        if (pass == 1)
-            for (int i = 0; i < kJoinThreads / 32; ++i) {
-                if (i == wid) at_few = n_few, at_many = n_many;
-                n_few += count[0][i];
-                n_many += count[1][i];
-            }
-        int c_few = 0, c_many = 0;
+    {
+        const int per = (n_warps + kJoinThreads - 1) / kJoinThreads, chunks = per * kJoinWarps;
         for (int i = 0; i < per; ++i) {
-            const int w = w0 + i * 32 + lane;
-            const int n = w < n_warps ? p.cuts[w].y : 0;
+            const int w = i * kJoinThreads + threadIdx.x, n = w < n_warps ? p.cuts[w].y : 0;
+            const unsigned f = __ballot_sync(~0u, n > 0 && n <= kFew), y = __ballot_sync(~0u, n > kFew);
+            if (lane == 0) counts[0][i * kJoinWarps + wid] = __popc(f), counts[1][i * kJoinWarps + wid] = __popc(y);
+        }
+        __syncthreads();
+        for (int i = 0; i < per; ++i) {
+            int at_few = 0, at_many = 0;   // in the chunks before this warp's
+            n_few = n_many = 0;
+            for (int c = lane; c < chunks; c += 32) {
+                n_few += counts[0][c], n_many += counts[1][c];
+                if (c < i * kJoinWarps + wid) at_few += counts[0][c], at_many += counts[1][c];
+            }
+            n_few = __reduce_add_sync(~0u, n_few), n_many = __reduce_add_sync(~0u, n_many);
+            at_few = __reduce_add_sync(~0u, at_few), at_many = __reduce_add_sync(~0u, at_many);
+            if (n_few + n_many == 0) return;
+            const int w = i * kJoinThreads + threadIdx.x, n = w < n_warps ? p.cuts[w].y : 0;
             const unsigned f = __ballot_sync(~0u, n > 0 && n <= kFew), y = __ballot_sync(~0u, n > kFew);
             const unsigned before = (1u << lane) - 1;
-            if (pass == 1) {
-                if (f >> lane & 1) few[at_few + __popc(f & before)] = (short)w;
-                if (y >> lane & 1) many[at_many + __popc(y & before)] = (short)w;
-                at_few += __popc(f);
-                at_many += __popc(y);
-            }
-            c_few += __popc(f);
-            c_many += __popc(y);
-        }
-        if (pass == 0 && lane == 0) {
-            count[0][wid] = c_few;
-            count[1][wid] = c_many;
+            if (f >> lane & 1) few[at_few + __popc(f & before)] = (short)w;
+            if (y >> lane & 1) many[at_many + __popc(y & before)] = (short)w;
         }
         __syncthreads();
     }
-    const int n_rows = p.n_kv * p.tiles;
+    const int n_rows = p.n_kv * p.tiles, units = p.piece_rows * kSlices;
     auto place = [&](int row, int head, bool& real) -> size_t {   // of the output row
         const int b = row / n_rows, h = row % n_rows, tile = h % p.tiles;
         real = head < min(16, p.group - tile * 16);
         return (size_t)b * p.n_q + h / p.tiles * p.group + tile * 16 + head;
     };
     auto piece = [&](int w, int k) { return p.pieces + (size_t)(2 * (w + k) + (k == 0)) * p.piece_floats; };
+    auto finish = [&](size_t at, int col, float a, float top, float l) {
+        if (col < p.dim) ((Act*)p.out)[at * p.dim + col] = sb_from_float<Act>(a / l);
+        if (p.lse && col == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
+    };
 
-    // ---- rows of many pieces
-    for (int u = blockIdx.x; u < n_many * p.piece_rows * kSlices; u += gridDim.x) {
-        const int w = many[u / (p.piece_rows * kSlices)], head = u / kSlices % p.piece_rows, slice = u % kSlices;
+    // ---- rows of more than kFew pieces
+    for (int u = blockIdx.x; u < n_many * units; u += gridDim.x) {
+        const int w = many[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
         const int2 cut = p.cuts[w];
+        const int n = cut.y;
         bool real;
         const size_t at = place(cut.x, head, real);
         if (!real) continue;
-        const int n = cut.y, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-        float top = -INFINITY;
-        for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, piece(w, k)[2 * head]);
+        // this warp's pieces: wid, wid + 8, ..; 32 at a time, one per lane
+        float top = -INFINITY, l = 0.f, a = 0.f;
+        for (int k0 = wid; k0 < n; k0 += kJoinThreads) {
+            const int k = k0 + lane * kJoinWarps;
+            const float2 ml = k < n ? *(const float2*)(piece(w, k) + 2 * head) : make_float2(-INFINITY, 0.f);
+            float t = fmaxf(top, ml.x);
 #pragma unroll
-        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-        if (lane == 0) red[0][wid] = top;
-        __syncthreads();
-        for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red[0][i]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float l = 0.f;
-        for (int k = threadIdx.x; k < n; k += kJoinThreads) {
-            const float2 ml = *(const float2*)(piece(w, k) + 2 * head);
-            const float f = exp2_fast(ml.x - base);
-            weight[k] = f;
-            l += f * ml.y;
+            for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, s));
+            const float base = t == -INFINITY ? 0.f : t, old = exp2_fast(top - base), f = exp2_fast(ml.x - base);
+            top = t;
+            l = l * old + f * ml.y;   // of this lane's pieces
+            a *= old;
+            const int here = min(32, (n - k0 + kJoinWarps - 1) / kJoinWarps);
+#pragma unroll 16
+            for (int i = 0; i < here; ++i)
+                a += __shfl_sync(~0u, f, i) * piece(w, k0 + i * kJoinWarps)[32 + head * DP + col];
         }
 #pragma unroll
         for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
-        if (lane == 0) red[1][wid] = l;
+        if (lane == 0) red[0][wid] = top, red[1][wid] = l;
+        sums[wid][lane] = a;
         __syncthreads();
-        l = 0.f;
-        for (int i = 0; i < kJoinThreads / 32; ++i) l += red[1][i];
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int k = grp; k < n; k += kGroups) {
-            const float4 x = *(const float4*)(piece(w, k) + 32 + head * DP + (slice * kCols + col) * 4);
-            const float f = weight[k];
-            a.x += f * x.x, a.y += f * x.y, a.z += f * x.z, a.w += f * x.w;
+        if (wid == 0) {
+            top = red[0][0];
+            for (int i = 1; i < kJoinWarps; ++i) top = fmaxf(top, red[0][i]);
+            const float base = top == -INFINITY ? 0.f : top;
+            a = l = 0.f;
+            for (int i = 0; i < kJoinWarps; ++i) {
+                const float f = exp2_fast(red[0][i] - base);
+                l += f * red[1][i];
+                a += f * sums[i][lane];
+            }
+            finish(at, col, a, top, l);
         }
-        sums[grp][col] = a;
-        __syncthreads();
-        if (threadIdx.x < kCols * 4) {   // one column per thread
-            const float* s = (const float*)sums + threadIdx.x;
-            float sum = 0.f;
-            for (int k = 0; k < kGroups; ++k) sum += s[k * kCols * 4];
-            const int d = slice * kCols * 4 + threadIdx.x;
-            if (d < p.dim) ((Act*)p.out)[at * p.dim + d] = sb_from_float<Act>(sum / l);
-        }
-        if (p.lse && slice == 0 && threadIdx.x == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
         __syncthreads();
     }
 
-    // ---- rows of few
-    for (int u = blockIdx.x * (kJoinThreads / 32) + wid; u < n_few * p.piece_rows; u += gridDim.x * (kJoinThreads / 32)) {
-        const int w = few[u / p.piece_rows], head = u % p.piece_rows;
+    // ---- the others
+    for (int u = blockIdx.x * kJoinWarps + wid; u < n_few * units; u += gridDim.x * kJoinWarps) {
+        const int w = few[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
         const int2 cut = p.cuts[w];
+        const int n = cut.y;
         bool real;
         const size_t at = place(cut.x, head, real);
         if (!real) continue;
-        float2 ml[kFew];
-        float x[kFew][DP / 32];
+        const float2 ml = lane < n ? *(const float2*)(piece(w, lane) + 2 * head) : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
 #pragma unroll
-        for (int k = 0; k < kFew; ++k) {
-            ml[k] = k < cut.y ? *(const float2*)(piece(w, k) + 2 * head) : make_float2(-INFINITY, 0.f);
+        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+        const float f = exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
+        float l = lane < n ? f * ml.y : 0.f, a = 0.f;
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) x[k][i] = k < cut.y ? piece(w, k)[32 + head * DP + i * 32 + lane] : 0.f;
-        }
-        float top = ml[0].x;
-#pragma unroll
-        for (int k = 1; k < kFew; ++k) top = fmaxf(top, ml[k].x);
-        const float base = top == -INFINITY ? 0.f : top;
-        float l = 0.f, a[DP / 32] = {};
-#pragma unroll
-        for (int k = 0; k < kFew; ++k) {
-            const float f = exp2_fast(ml[k].x - base);
-            l += f * ml[k].y;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) a[i] += k < cut.y ? f * x[k][i] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-            if (i * 32 + lane < p.dim) ((Act*)p.out)[at * p.dim + i * 32 + lane] = sb_from_float<Act>(a[i] / l);
-        if (p.lse && lane == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
+        for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
+#pragma unroll 16
+        for (int k = 0; k < n; ++k) a += __shfl_sync(~0u, f, k) * piece(w, k)[32 + head * DP + col];
+        finish(at, col, a, top, l);
     }
 }
 
