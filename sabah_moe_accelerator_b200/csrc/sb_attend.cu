@@ -5,36 +5,46 @@
 //
 // Key j of sequence b is row j % page_size of page block_table[b][j / page_size].
 // A sequence of length zero gives zeros and lse = -inf. Nothing outside
-// [lo, len) is read: not a key, not a table entry.
+// [lo, len) counts, and no table entry outside it is read.
 //
 // Bound: DRAM, every key and value row once. A key-value head's query heads
 // (up to 16: the rows of an MMA tile) are taken together, so the rows are read
-// once for all of them; the arithmetic is 16-row mma.sync on 16 keys at a time,
+// once for all of them; the arithmetic is 16-row mma.sync on 32 keys at a time,
 // a fraction of the tensor rate and well under the time the rows take to
 // arrive. tcgen05's 128-row tiles would be 87-99% padding here.
 //
-// The work is a list of steps of 16 keys over all (sequence, key-value head)
-// rows. Each warp takes an equal, contiguous part of it, whatever the lengths:
-// one long sequence spreads over the whole chip, and many short ones stay whole
-// within a warp. Warps never wait for one another; each streams its own keys
-// and values through its own ring in shared memory (cp.async, rows padded by 16
-// bytes so that ldmatrix meets no bank twice). A row that ends in a part is
-// left as (m, l, unnormalised out) in the workspace, and a second, small launch
-// (a programmatic dependent of the first) joins the pieces of each cut row in
-// a fixed order. Rows of at most kWhole steps are never cut; where the block
-// table cannot hold a longer sequence the second launch is left out.
+// The work is a list of steps of 32 keys over all (sequence, key-value head)
+// rows, cut into equal parts whatever the lengths: one long sequence spreads
+// over the whole chip, and many short ones stay whole within a warp. Each warp
+// has one part of its own; where parts are long they cover 13/16 of the list,
+// and the rest is small parts that warps take as they finish, because SMs do
+// not all get the same share of the bandwidth. Warps never wait for one
+// another; each streams its own keys and values through its own ring in shared
+// memory, filled by TMA: boxes of as many rows as divide both a page and 16, 64
+// columns wide in the 128-byte swizzle that lets ldmatrix meet no bank twice.
+// Rows of a box past the window's ends are masked (keys) or zeroed (values),
+// so that nothing they hold counts. A row of the list that ends in a
+// part is left as (m, l, unnormalised out) in the workspace, and a second,
+// small launch (a programmatic dependent of the first) joins the pieces of each
+// cut row in the order of its keys, so results do not depend on who took which
+// part. Rows of at most kWhole steps are never cut; where the block table
+// cannot hold a longer sequence the second launch is left out.
 //
 // Precision: scores, m, l and out are fp32. The MMA takes 16-bit factors, so
 // fp32 queries and the softmax weights are split into a sum of 16-bit parts
 // (f16: 2 parts, 22 bits; bf16: 3 parts, 24 bits), each multiplied exactly.
-// With 16-bit outputs the weights take two parts, which leaves the output's
-// own rounding as the only one. f16 parts keep their bits only in f16's normal
+// With 16-bit outputs the weights take two parts, which leaves the output's own
+// rounding as the only one. f16 parts keep their bits only in f16's normal
 // range: a query row is scaled to below 2 by a power of two, and the weights
-// are computed times 2^12. The parts but the last are cut off rather than
-// rounded, so all of a number's parts have its sign, and the first part's
-// products are summed apart from the others': where an infinite key or value
-// makes the others infinite or NaN (0 * inf), add_rest() leaves the first.
+// are computed times 2^11. The reference m of a running sum moves only when a
+// score exceeds it by 2^4, which leaves most steps without a rescaling. The
+// MMA's accumulation cuts off instead of rounding (measured: 1 + 1.75 * 2^-24
+// gives 1), half a unit per step and always toward zero, so its sums are added
+// to rounded fp32 sums every kFold steps.
+#include <cuda.h>
+
 #include <algorithm>
+#include <atomic>
 
 #include "sb_act.cuh"
 #include "sb_kernels.h"
@@ -43,11 +53,21 @@ namespace {
 
 constexpr int kMaxDim = 256;
 constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in shared memory
-constexpr int kStep = 16;        // keys per step
-constexpr int kWhole = 8;        // rows of at most this many steps are never cut
-constexpr int kMinSteps = 4;     // and a part is at least this long
-constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps
+constexpr int kStep = 32;        // keys per step
+constexpr int kWhole = 4;        // rows of at most this many steps are never cut
+constexpr int kMinSteps = 2;     // and a part is at least this long
+constexpr int kRowCost = 1;      // what a row costs besides its steps, in steps
+constexpr int kShare = 16;       // steps per warp from which the last 3/16 are shared out
+constexpr int kMaxWarps = 148 * 2 * 8, kMaxParts = 3 * kMaxWarps;
 constexpr int kSmemLimit = 227 * 1024;
+constexpr float kLazy = 4.f;     // how far, in powers of two, a score may exceed the reference
+
+// The head of the workspace; the arrays of the parts follow.
+struct Header {
+    unsigned long long ready;    // the call's number, once `next` is zero
+    int next;                    // the next shared part
+    int n_parts;
+};
 
 struct AttendParams {
     const uint8_t* q;
@@ -56,6 +76,7 @@ struct AttendParams {
     const uint8_t *k, *v;
     size_t k_page, k_slot, k_head, v_page, v_slot, v_head;   // bytes
     int n_pages, page_size, page_shift;   // shift: log2(page_size), or -1
+    int box;                // rows of a TMA box: a power of two to 16 that divides the page
     const int32_t* table;
     size_t table_stride;    // elements
     int table_width;
@@ -66,23 +87,38 @@ struct AttendParams {
     uint8_t* out;
     float* lse;
     int* err;
-    int2* cuts;             // per warp: the row cut in its part (-1: none) and its number of pieces
-    float* pieces;          // per warp two: the row it enters in the middle of, the row it leaves early
+    int share;              // parts may be shared out
+    unsigned long long call;
+    Header* head;
+    uint16_t* cut_pieces;   // per part: the pieces of the row cut in it (0: none)
+    int* cut_row;           // and which row
+    float* pieces;          // per part two: the row it enters in the middle of, the row it leaves early
+    float* sums;            // per warp one: its rounded sums, where registers have no room for them
     int piece_floats, piece_rows;
 };
 
 // ------------------------------------------------------------ PTX helpers
 __device__ inline uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ inline void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ inline void bar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
-__device__ inline void copy16_or_zero(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+__device__ inline void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ inline void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ inline void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// bounded: false after about 2 s
+__device__ inline bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < 1 << 17; ++i) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ inline void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int slot, int head, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(slot), "r"(head), "r"(page)
+                 : "memory");
 }
 __device__ inline void ldsm4(uint32_t* r, uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -95,51 +131,31 @@ __device__ inline void ldsm4t(uint32_t* r, uint32_t a) {
 template <class T>
 __device__ inline void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ inline float exp2_fast(float x) {   // 2 ulp; exp2(-inf) = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two values as 16-bit ones, cut off (CUT) or rounded to nearest
-template <class T, bool CUT>
-__device__ inline uint32_t pack2(float a, float b) {
+// the next 16-bit part of (a, b), which keep what it leaves
+template <class T>
+__device__ inline uint32_t take_part(float& a, float& b) {
     uint32_t u;
-    if constexpr (std::is_same<T, __half>::value && CUT)
-        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
-    else if constexpr (std::is_same<T, __half>::value)
+    if constexpr (std::is_same<T, __half>::value) {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
-    else if constexpr (CUT)
-        u = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    else
+        const float2 f = __half22float2(*(const __half2*)&u);
+        a -= f.x, b -= f.y;
+    } else {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
-    return u;
-}
-// first + rest, where rest counts only if it is a number: first is infinite or
-// NaN whenever rest is, and of the same sign (fmaxf takes a NaN's other side)
-__device__ inline float add_rest(float first, float rest) { return first + fmaxf(rest, -3.402823466e38f); }
-template <class T>
-__device__ inline float2 unpack2(uint32_t u) {
-    if constexpr (std::is_same<T, __half>::value)
-        return __half22float2(*(const __half2*)&u);
-    else
-        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-
-// the next part of (a, b), which keep what it leaves
-template <class T>
-__device__ inline uint32_t take_part(float& a, float& b, bool last) {
-    const uint32_t u = last ? pack2<T, false>(a, b) : pack2<T, true>(a, b);
-    const float2 f = unpack2<T>(u);
-    a -= f.x;
-    b -= f.y;
+        a -= __uint_as_float(u << 16), b -= __uint_as_float(u & 0xffff0000u);
+    }
     return u;
 }
 // e with 2^e <= x < 2^(e + 1); 0 for zero, infinity and NaN
@@ -147,19 +163,21 @@ __device__ inline int exponent(float x) {
     return x > 0.f && x < INFINITY ? min(max((__float_as_int(x) >> 23) - 127, -126), 126) : 0;
 }
 __device__ inline float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+__device__ inline bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // ------------------------------------------------------------ shapes
-// DP: head size rounded up to a tile width. Each warp has a ring of kStages
-// steps of 16 keys and 16 values.
+// DP: head size rounded up to a tile width. A slot of a ring is the keys or the
+// values of a step, as kTiles tiles of 32 rows x 64 columns (128 swizzled bytes).
 template <int DP>
 struct Shape {
-    static constexpr int kRow = DP * 2 + 16;                  // bytes of a padded row
-    static constexpr int kStage = 2 * kStep * kRow;
-    static constexpr int kStages = DP <= 64 ? 6 : DP <= 96 ? 4 : 3;
-    static constexpr int kLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // lanes that copy one row
-    static constexpr int kWarps = 8;                          // at most
+    static constexpr int kTiles = (DP + 63) / 64;
+    static constexpr int kTileBytes = kStep * 128, kSlot = kTiles * kTileBytes;
+    static constexpr int kSlots = DP <= 64 ? 6 : 3;
+    static constexpr int kWarps = DP <= 128 ? 8 : DP <= 192 ? 5 : 4;
 };
+constexpr float up_of(bool f16) { return f16 ? 11.f : 0.f; }
 
+// ------------------------------------------------------------ the list of steps
 // The scan of the lengths: cost of the sequences before b, for one row of each.
 // A row takes its steps, then kRowCost idle places in the list, so that parts
 // of many short rows and parts of one long row take as long.
@@ -175,60 +193,113 @@ __device__ inline int seq_steps(int len, int window) {
 __device__ inline long long div_fast(long long a, long long b) {
     return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
-
-// A place in the list of steps; each warp has one that loads and one that computes.
-struct Cursor {
-    int b, h;            // sequence, row of it (key-value head and tile)
-    int j, end, steps;   // step in the row, where this warp leaves it, the row's steps
-    int len, lo;
-    long long row_at;    // the row's first step in the list
+// The parts: n_own of `own` places, one per warp, then shared ones of `small`.
+struct Parts {
+    long long cost, own, own_end, small;
+    int n_own, n;
+    __device__ Parts(long long cost_, int warps, bool share) : cost(cost_) {
+        own = max(div_fast(cost + warps - 1, warps), (long long)kMinSteps);
+        if (share && own >= kShare) {
+            own = own * 13 / 16;
+            n_own = warps;
+            own_end = own * warps;
+            const long long rest = cost - own_end;
+            small = max(div_fast(rest + 2 * warps - 1, 2 * warps), (long long)kMinSteps);
+            n = n_own + (int)div_fast(rest + small - 1, small);
+        } else {
+            n = n_own = (int)div_fast(cost + own - 1, own);
+            own_end = cost;
+            small = 1;
+        }
+    }
+    __device__ long long begin(int i) const { return i < n_own ? i * own : own_end + (i - n_own) * small; }
+    __device__ long long end(int i) const { return i < n_own ? min((i + 1) * own, own_end) : min(own_end + (i + 1 - n_own) * small, cost); }
+    __device__ int of(long long at) const {
+        return at < own_end ? (int)div_fast(at, own) : n_own + (int)div_fast(at - own_end, small);
+    }
 };
 
-// starts the row at c.b, c.h; the warp takes its steps from j on
-__device__ inline void enter_row(Cursor& c, const Seqs& s, const AttendParams& p, int j, long long until) {
+// A place in the list; each warp has one that loads and one that computes.
+struct Cursor {
+    int b, h;            // sequence, row of it (key-value head and tile)
+    int j, end, steps;   // step in the row, where the part leaves it, the row's steps
+    int len, lo;
+    int part;
+    long long row_at, until;   // the row's first place in the list, the part's end
+};
+// starts the row at c.b, c.h, from its step j on
+__device__ inline void enter_row(Cursor& c, const Seqs& s, const AttendParams& p, int j) {
     c.len = s.len[c.b];
     c.lo = window_start(max(c.len, 0), p.window);
     c.steps = (int)(s.pre[c.b + 1] - s.pre[c.b]) - kRowCost;
     c.j = j;
-    c.end = c.steps <= kWhole ? c.steps : (int)min((long long)c.steps, until - c.row_at);
+    c.end = c.steps <= kWhole ? c.steps : (int)min((long long)c.steps, c.until - c.row_at);
 }
-// false at the end of the warp's part
-__device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p, long long until) {
+// false at the end of the part
+__device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p) {
     c.row_at += c.steps + kRowCost;
-    if (c.row_at >= until) return false;
+    if (c.row_at >= c.until) return false;
     if (++c.h == p.n_kv * p.tiles) {
         c.h = 0;
         if (++c.b == p.n_seqs) return false;
     }
-    enter_row(c, s, p, 0, until);
+    enter_row(c, s, p, 0);
     return true;
+}
+// the first step of a part; b = -1 where the part has none of its own
+__device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, long long from, long long until, int part, int lane) {
+    const int n_rows = p.n_kv * p.tiles;
+    Cursor c;
+    c.part = part;
+    c.until = until;
+    int a = 0, span = p.n_seqs;   // the last sequence that starts at or before `from` is in [a, a + span)
+    while (span > 1) {            // 32 probes at a time
+        const int hop = (span + 31) / 32, at = a + lane * hop;
+        const unsigned hit = __ballot_sync(~0u, at < a + span && s.pre[min(at, p.n_seqs)] * n_rows <= from);
+        const int last = 31 - __clz(hit);
+        span = min(hop, span - last * hop);
+        a += last * hop;
+    }
+    c.b = a;
+    const long long at = from - s.pre[a] * n_rows, cost = s.pre[a + 1] - s.pre[a];
+    c.h = (int)div_fast(at, cost);
+    const int j = (int)(at - c.h * cost);
+    c.row_at = from - j;
+    enter_row(c, s, p, j);
+    // a whole row is its first step's part's; past a row's steps are its idle places
+    if (!(j < c.steps && (c.steps > kWhole || j == 0)) && !next_row(c, s, p)) c.b = -1;
+    return c;
 }
 
 // ------------------------------------------------------------ the loading side
-// One warp's copies into its ring, kStages - 1 steps ahead of its arithmetic.
-// Block table entries are held 32 to a register, one per lane, and the register
-// after the current one is always on its way, as are the first entries of this
-// sequence (the next key-value head starts there again) and of the next.
+// One warp's loads into its ring: every slot is filled again as soon as it has
+// been read. Block table entries are held 32 to a register, one per lane, and
+// the register after the current one is always on its way, as are the first
+// entries of this sequence (the next key-value head starts there again) and of
+// the next. Row starts go to the computing side through a small queue.
+constexpr int kQueue = 8;   // row starts between the two: at most one per two slots, and one
+
 template <int DP>
 struct Loader {
     using S = Shape<DP>;
     const AttendParams& p;
+    const CUtensorMap *kmap, *vmap;
     const Seqs& seqs;
-    const long long until;
+    const Parts& parts;
     const int lane;
-    const uint32_t ring;
+    const uint32_t ring, bars;
+    int4* queue;
     Cursor c;
-    bool more = true;
-    uint32_t bad_steps = 0;             // bit per stage: the step met a page out of range
-    int first, cur, next, head, ahead;  // cur: entries first ..; next: the 32 after them
+    bool more = true, asked = false, values = false;   // values: the next slot is the step's values
+    int claimed = 0, pushed = 0;
+    uint32_t bad = 0, dirty = 0;        // bits per slot: the step met a page out of range; zeros were stored to it
+    int first, cur, next, start, ahead; // cur: table entries first ..; next: the 32 after them
+    int page = -1, row = 0;             // lane i: where box i of the step lies; page -1: it is not loaded
 
-    __device__ Loader(const AttendParams& p_, const Seqs& s_, long long until_, int lane_, uint32_t ring_, const Cursor& c_)
-        : p(p_), seqs(s_), until(until_), lane(lane_), ring(ring_), c(c_) {
-        first = entry_of((c.lo / kStep + c.j) * kStep);
-        cur = entries(c.b, first);
-        next = entries(c.b, first + 32);
-        head = entries(c.b, entry_of(c.lo / kStep * kStep));
-        ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
+    __device__ Loader(const AttendParams& p_, const CUtensorMap* km, const CUtensorMap* vm, const Seqs& s_, const Parts& parts_,
+                      int lane_, uint32_t ring_, uint32_t bars_, int4* queue_, const Cursor& c_)
+        : p(p_), kmap(km), vmap(vm), seqs(s_), parts(parts_), lane(lane_), ring(ring_), bars(bars_), queue(queue_), c(c_) {
+        begin_part();
     }
     __device__ int entry_of(int key) const {
         return p.page_shift >= 0 ? key >> p.page_shift : (int)((unsigned)key / (unsigned)p.page_size);
@@ -243,90 +314,153 @@ struct Loader {
         const int lo = window_start(max(seqs.len[b], 0), p.window);
         return entries(b, entry_of(lo / kStep * kStep));
     }
-    __device__ int page_of(int e) const {   // e: per lane, first <= e < first + 64
-        const int a = __shfl_sync(~0u, cur, e - first), b = __shfl_sync(~0u, next, e - first);
-        return e - first < 32 ? a : b;
+    __device__ void push() {
+        queue[pushed++ % kQueue] = make_int4(c.b, c.h, c.j, c.part);   // every lane writes, and reads its own
+    }
+    __device__ void begin_part() {
+        first = entry_of((c.lo / kStep + c.j) * kStep);
+        cur = entries(c.b, first);
+        next = entries(c.b, first + 32);
+        start = first_entries(c.b);
+        ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
+        push();
+    }
+    // A shared part's number is asked for some steps before it is needed. The
+    // count starts at zero once a warp of the first CTA has said so; a warp
+    // that does not see that yet leaves the parts to others, to that CTA's
+    // warps at least, which have seen it before they start (and have parts of
+    // their own: one of at least kShare * 13 / 16 places holds a row's start).
+    __device__ void ask() {
+        asked = true;
+        claimed = kMaxParts;
+        if (lane == 0) {
+            unsigned long long r;
+            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(r) : "l"(&p.head->ready) : "memory");
+            if (r == p.call) claimed = atomicAdd(&p.head->next, 1);
+        }
     }
     __device__ void advance() {
-        if (++c.j < c.end) return;
+        ++c.j;
+        if (parts.n > parts.n_own && !asked && c.until - c.row_at - c.j <= 2) ask();
+        if (c.j < c.end) return;
         const int b = c.b;
-        more = next_row(c, seqs, p, until);
-        if (!more) return;
-        if (c.b != b) {
-            head = ahead;
-            ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
-        }
-        first = entry_of(c.lo / kStep * kStep);
-        cur = head;
-        next = entries(c.b, first + 32);
-    }
-    __device__ void issue(int stage) {
+        more = next_row(c, seqs, p);
         if (more) {
-            const int key0 = (c.lo / kStep + c.j) * kStep, kv = p.tiles == 1 ? c.h : c.h / p.tiles;
-            const int e0 = entry_of(key0);
-            if (e0 >= first + 32) {
+            if (c.b != b) {
+                start = ahead;
+                ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
+            }
+            first = entry_of(c.lo / kStep * kStep);
+            cur = start;
+            next = entries(c.b, first + 32);
+            push();
+            return;
+        }
+        while (parts.n > parts.n_own) {
+            if (!asked) ask();
+            asked = false;
+            const int i = __shfl_sync(~0u, claimed, 0);
+            if (i >= parts.n - parts.n_own) break;
+            const int part = parts.n_own + i;
+            if (lane == 0) p.cut_pieces[part] = 0;
+            const Cursor at = enter_part(seqs, p, parts.begin(part), parts.end(part), part, lane);
+            if (at.b >= 0) {
+                c = at;
+                more = true;
+                begin_part();
+                break;
+            }
+        }
+    }
+    // fills a slot with the next keys or values
+    __device__ void issue(int slot) {
+        if (!more) return;
+        if (!values) {
+            const int key0 = (c.lo / kStep + c.j) * kStep, key = key0 + lane * p.box;
+            if (entry_of(key0) >= first + 32) {
                 first += 32;
                 cur = next;
                 next = entries(c.b, first + 32);
             }
-            const int copy_lane = lane % S::kLanes, copy_row = lane / S::kLanes;
-            const bool copies = copy_lane * 8 < p.dim;
-            const uint32_t dst = ring + stage * S::kStage + copy_row * S::kRow + copy_lane * 16;
-            constexpr int kAtOnce = 32 / S::kLanes, kTimes = kStep / kAtOnce;
-            const uint8_t* nowhere = (const uint8_t*)p.pieces;   // an address for copies of no bytes
-            bool bad;
-            if (p.page_size % kStep == 0) {   // the step lies in one page
-                const int page = page_of(e0);
-                bad = (page < 0 || page >= p.n_pages) && c.len > c.lo;
-                const bool none = page < 0 || page >= p.n_pages;
-                const long long slot = key0 - e0 * p.page_size + copy_row;
-                const uint8_t* k = p.k + (none ? 0 : page) * p.k_page + slot * p.k_slot + kv * p.k_head + copy_lane * 16;
-                const uint8_t* v = p.v + (none ? 0 : page) * p.v_page + slot * p.v_slot + kv * p.v_head + copy_lane * 16;
-                if (!none && key0 >= c.lo && key0 + kStep <= c.len) {
-                    if (copies) {
-#pragma unroll
-                        for (int i = 0; i < kTimes; ++i, k += kAtOnce * p.k_slot) copy16(dst + i * kAtOnce * S::kRow, k);
-#pragma unroll
-                        for (int i = 0; i < kTimes; ++i, v += kAtOnce * p.v_slot)
-                            copy16(dst + (kStep + i * kAtOnce) * S::kRow, v);
-                    }
-                } else if (copies) {
-#pragma unroll
-                    for (int i = 0; i < kTimes; ++i, k += kAtOnce * p.k_slot, v += kAtOnce * p.v_slot) {
-                        const int key = key0 + i * kAtOnce + copy_row;
-                        const bool real = !none && key >= c.lo && key < c.len;
-                        copy16_or_zero(dst + i * kAtOnce * S::kRow, real ? k : nowhere, real);
-                        copy16_or_zero(dst + (kStep + i * kAtOnce) * S::kRow, real ? v : nowhere, real);
-                    }
-                }
-            } else {   // lane i finds key i's place, the lanes that copy it ask that lane
-                const int key = key0 + (lane & 15), inside = min(max(key, c.lo), max(c.len - 1, c.lo));
-                const int e = entry_of(inside), page = page_of(e);
-                const bool valid = key >= c.lo && key < c.len, out = page < 0 || page >= p.n_pages;
-                bad = __any_sync(~0u, valid && out);
-                const unsigned slot = (unsigned)inside - (unsigned)e * (unsigned)p.page_size;
-                const bool real = valid && !out;
-                const long long ko = real ? (long long)(page * p.k_page + slot * p.k_slot + kv * p.k_head) : -1;
-                const long long vo = real ? (long long)(page * p.v_page + slot * p.v_slot + kv * p.v_head) : -1;
-#pragma unroll
-                for (int i = 0; i < kTimes; ++i) {
-                    const int r = i * kAtOnce + copy_row;
-                    const long long a = __shfl_sync(~0u, ko, r), b = __shfl_sync(~0u, vo, r);
-                    if (!copies) continue;
-                    copy16_or_zero(dst + i * kAtOnce * S::kRow, a < 0 ? nowhere : p.k + a + copy_lane * 16, a >= 0);
-                    copy16_or_zero(dst + (kStep + i * kAtOnce) * S::kRow, a < 0 ? nowhere : p.v + b + copy_lane * 16, a >= 0);
-                }
-            }
-            bad_steps &= ~(1u << stage);
-            if (bad) {
-                bad_steps |= 1u << stage;
+            const int e = entry_of(key), at = e - first;   // a step has at most 32 entries: at < 64
+            const int x = __shfl_sync(~0u, cur, at), y = __shfl_sync(~0u, next, at);
+            page = at < 32 ? x : y;
+            row = key - e * p.page_size;
+            const bool in = lane * p.box < kStep && key < c.len && key + p.box > c.lo;
+            const bool out = in && (page < 0 || page >= p.n_pages);
+            if (!in || out) page = -1;
+            bad &= ~(1u << slot);
+            if (__any_sync(~0u, out)) {
+                bad |= 1u << slot;
                 if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
             }
-            advance();
         }
-        copy_commit();
+        if (dirty >> slot & 1) {   // order the zeros before the TMA's writes
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            dirty &= ~(1u << slot);
+        }
+        const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kSlot + lane * p.box * 128;
+        const unsigned boxes = __popc(__ballot_sync(~0u, page >= 0));
+        if (lane == 0) bar_expect(bar, boxes * p.box * (128 * S::kTiles));
+        if (page >= 0) {
+            const CUtensorMap* map = values ? vmap : kmap;
+            const int kv = p.tiles == 1 ? c.h : c.h / p.tiles;
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) tile_load(dst + t * S::kTileBytes, map, bar, 64 * t, row, kv, page);
+        }
+        if (values) advance();
+        values = !values;
     }
 };
+
+// ------------------------------------------------------------ infinities
+// Products of parts make NaN of what is an infinity in the formula (0 * inf,
+// inf - inf between parts). Where a row's result is not finite, its columns that
+// are not are computed again here, key by key in fp32, for this warp's keys
+// [from, to); all of them where the softmax's own sum is not finite.
+template <class Cache, class Act>
+__device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int head, int from, int to, float m, float l,
+                                      float up, bool whole, float* ml, float* piece, int lane) {
+    constexpr int N = kMaxDim / 32;
+    const Act* q = (const Act*)(p.q + b * p.q_seq + head * p.q_head);
+    float o[N] = {}, top = -INFINITY, sum = 0.f;
+    for (int j = from; j < to; ++j) {
+        const int page = p.table[b * p.table_stride + j / p.page_size];
+        if (page < 0 || page >= p.n_pages) return;   // NaN, as it is
+        const Cache* k = (const Cache*)(p.k + page * p.k_page + (j % p.page_size) * p.k_slot + kv * p.k_head);
+        const Cache* v = (const Cache*)(p.v + page * p.v_page + (j % p.page_size) * p.v_slot + kv * p.v_head);
+        float s = 0.f;
+        for (int i = 0; i < N; ++i)
+            if (lane + 32 * i < p.dim) s += sb_to_float(q[lane + 32 * i]) * sb_to_float(k[lane + 32 * i]);
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
+        s *= p.scale_log2;
+        const float t = fmaxf(top, s), a = top == -INFINITY ? 0.f : exp2f(top - t), e = exp2f(s - t);
+        top = t;
+        sum = sum * a + e;
+        for (int i = 0; i < N; ++i)
+            if (lane + 32 * i < p.dim) o[i] = (a == 0.f ? 0.f : o[i] * a) + e * sb_to_float(v[lane + 32 * i]);
+    }
+    const bool all = !is_finite(l);
+    const size_t at = (size_t)b * p.n_q + head;
+    Act* out = (Act*)p.out + at * p.dim;
+    const float scale = all ? exp2f(up) : exp2f(top - m + up);
+    for (int i = 0; i < N; ++i) {
+        const int d = lane + 32 * i;
+        if (d >= p.dim) break;
+        if (whole) {
+            if (all || !is_finite(sb_to_float(out[d]))) out[d] = sb_from_float<Act>(o[i] / sum);
+        } else if (all || !is_finite(piece[d])) {
+            piece[d] = o[i] * scale;
+        }
+    }
+    if (all && lane == 0) {
+        if (!whole)
+            ml[0] = top, ml[1] = sum * scale;
+        else if (p.lse)
+            p.lse[at] = 0.69314718055994531f * (top + log2f(sum));
+    }
+}
 
 // ------------------------------------------------------------ the kernel
 // QP: parts of a query value (1: it has the cache's type); the weights take as
@@ -335,21 +469,44 @@ struct Loader {
 // both parts, and the query fragments stay in registers. With 9-16 heads each
 // part is an MMA of its own and the queries lie in shared memory.
 template <class Cache, int DP, int QP, bool HALF>
-__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const AttendParams p) {
+__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
+    k_attend(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
+             const __grid_constant__ CUtensorMap vmap) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
     constexpr int PP = QP == 1 ? 2 : QP;
     constexpr int R = HALF ? 1 : 2;          // row halves with heads of their own
     constexpr int ND = DP / 16;
-    constexpr float kUp = std::is_same<Cache, __half>::value ? 12.f : 0.f;
-    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr float kUp = up_of(std::is_same<Cache, __half>::value);
+    // rounded sums stay in registers up to 128 columns
+    constexpr bool kKeep = DP <= 128;
+    constexpr int kFold = QP == 1 ? 32 : 8;
+    constexpr int kQRow = DP * 2 + 16;
+    extern __shared__ __align__(1024) uint8_t smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    const int rows = min(p.group, 16), q_rows = HALF ? 0 : rows * QP;
+    uint8_t* q_mem = smem + n_warps * S::kSlots * S::kSlot + wid * q_rows * kQRow;
+    uint8_t* tail = smem + n_warps * (S::kSlots * S::kSlot + q_rows * kQRow);
+    int4* queue = (int4*)tail + wid * kQueue;
+    tail += n_warps * kQueue * sizeof(int4);
+    const uint32_t bars = smem_addr(tail) + wid * S::kSlots * 8;
+    tail += n_warps * S::kSlots * 8;
+    Seqs seqs{(long long*)tail, (int*)(tail + 8 * (p.n_seqs + 1))};
 
+    if (lane < S::kSlots) bar_init(bars + lane * 8, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.head->next = 0;
+        asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(&p.head->ready), "l"(p.call) : "memory");
+    }
 
     // ---- the scan of the lengths
-    Seqs seqs{(long long*)smem, (int*)(smem + 8 * (p.n_seqs + 1))};
     __shared__ long long warp_sum[32];
     {
         const int per = (p.n_seqs + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per;
@@ -381,46 +538,21 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
         __syncthreads();
     }
 
-    // ---- this warp's part of the list; neighbours in it sit on different SMs
+    // ---- this warp's own part; neighbours in the list sit on different SMs
     const int w = wid * gridDim.x + blockIdx.x, n_rows = p.n_kv * p.tiles;
-    const long long total = seqs.pre[p.n_seqs] * n_rows, all_warps = (long long)gridDim.x * n_warps;
-    const long long part = max(div_fast(total + all_warps - 1, all_warps), (long long)kMinSteps);
-    const long long from = w * part, until = min(from + part, total);
-    if (lane == 0) p.cuts[w] = make_int2(-1, 0);
-    if (from >= total) return;
-    Cursor cc;
-    {
-        // the last sequence that starts at or before `from`: 32 probes at a time
-        int a = 0, span = p.n_seqs;   // it is in [a, a + span)
-        while (span > 1) {
-            const int hop = (span + 31) / 32, at = a + lane * hop;
-            const unsigned hit = __ballot_sync(~0u, at < a + span && seqs.pre[min(at, p.n_seqs)] * n_rows <= from);
-            const int last = 31 - __clz(hit);
-            span = min(hop, a + span - (a + last * hop));
-            a += last * hop;
-        }
-        cc.b = a;
-        const long long at = from - seqs.pre[a] * n_rows, cost = seqs.pre[a + 1] - seqs.pre[a];
-        cc.h = (int)div_fast(at, cost);
-        const int j = (int)(at - cc.h * cost);
-        cc.row_at = from - j;
-        enter_row(cc, seqs, p, j, until);
-        // a whole row is its first step's warp's
-        if ((j >= cc.steps || (cc.steps <= kWhole && j > 0)) && !next_row(cc, seqs, p, until)) return;
-    }
+    const Parts parts(seqs.pre[p.n_seqs] * n_rows, gridDim.x * n_warps, p.share);
+    if (w == 0 && lane == 0) p.head->n_parts = parts.n;
+    if (w >= parts.n_own) return;
+    if (lane == 0) p.cut_pieces[w] = 0;
+    Cursor cc = enter_part(seqs, p, parts.begin(w), parts.end(w), w, lane);
+    if (cc.b < 0) return;
 
-    // ---- shared memory of this warp: the ring, then (not HALF) the query rows
-    const int rows = min(p.group, 16), q_rows = HALF ? 0 : rows * QP;
-    const uint32_t head = (12 * p.n_seqs + 8 + 15) / 16 * 16;
-    uint8_t* mine = smem + head + wid * (S::kStages * S::kStage + q_rows * S::kRow);
-    uint8_t* q_mem = mine + S::kStages * S::kStage;
-    const uint32_t ring = smem_addr(mine);
+    // ---- queries on their way, then keys and values
     const int g = lane >> 2, quad = lane & 3;
     Act qx[HALF ? ND : 1][4];   // the row's query values 16 d + 2 quad + {0, 1, 8, 9}, as they are
     auto fetch_queries = [&](const Cursor& c) {
         if constexpr (HALF) {
-            const int first = c.h * p.group, heads = p.group;
-            const Act* src = (const Act*)(p.q + c.b * p.q_seq + (first + min(g, heads - 1)) * p.q_head);
+            const Act* src = (const Act*)(p.q + c.b * p.q_seq + (c.h * p.group + min(g, p.group - 1)) * p.q_head);
             if (p.q_pairs) {
                 struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
 #pragma unroll
@@ -443,25 +575,26 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
         }
     };
     fetch_queries(cc);
-    Loader<DP> loader(p, seqs, until, lane, ring, cc);
-    if (p.dim < DP) {   // columns past the head size stay zero
-        const int pad = (DP - p.dim) / 8, n = (S::kStages * 2 * kStep + q_rows) * pad;
-        for (int i = lane; i < n; i += 32)
-            *(uint4*)(mine + i / pad * S::kRow + (p.dim + i % pad * 8) * 2) = make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) loader.issue(i);
+    uint8_t* ring_mem = smem + wid * S::kSlots * S::kSlot;
+    const uint32_t ring = smem_addr(ring_mem);
+    Loader<DP> loader(p, &kmap, &vmap, seqs, parts, lane, ring, bars, queue, cc);
+#pragma unroll 1
+    for (int i = 0; i < S::kSlots; ++i) loader.issue(i);
 
     // ---- the computing side
-    float o[DP / 8][2 * R], m[R], l[R], unscale[R];
-    uint32_t qf[HALF ? ND : 1][QP == 1 ? 2 : 2 * QP];   // HALF: per 16 dimensions, the parts of both 8s
-    const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * S::kRow + ((lane >> 3) & 1) * 16;
-    const uint32_t v_lane = kStep * S::kRow + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::kRow + (lane >> 4) * 16;
-    int stage = 0;
+    float acc[DP / 8][4];                          // the MMA's sums; HALF: rows 8-15 are the second parts'
+    float o[kKeep ? DP / 8 : 1][2 * R], m[R], l[R], l_sum[R], unscale[R];
+    uint32_t qf[HALF ? ND : 1][2 * QP];            // HALF: per 16 dimensions, the parts of both 8s
+    const int k_row = (lane >> 4) * 8 + (lane & 7), v_row = ((lane >> 3) & 1) * 8 + (lane & 7);
+    const uint32_t k_lane = k_row * 128 + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
+    const uint32_t v_lane = v_row * 128 + (((lane >> 4) ^ (v_row & 7)) << 4);
+    float* sums = p.sums + (size_t)w * p.piece_floats;
+    uint32_t wf[2][HALF ? PP - 1 : PP][4];         // the weights as the A operand, per 16 keys and part
+    int slot = 0, popped = 1;
+    uint32_t parity = 0;
     for (bool live = true; live;) {
         const int tile = p.tiles == 1 ? 0 : cc.h % p.tiles, kv = p.tiles == 1 ? cc.h : cc.h / p.tiles;
         const int first_head = kv * p.group + tile * 16, heads = min(16, p.group - tile * 16);
-        const uint8_t* q_row0 = p.q + cc.b * p.q_seq + first_head * p.q_head;
 
         // ---- this row's queries, split into parts
 #pragma unroll
@@ -471,15 +604,8 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
             auto value = [&](int d, int i) {
                 return 16 * d + 2 * quad + (i >> 1) * 8 < p.dim ? sb_to_float(qx[d][i]) : 0.f;
             };
-            if constexpr (QP == 1) {
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float a = value(d, 2 * i), b = value(d, 2 * i + 1);
-                        qf[d][i] = take_part<Cache>(a, b, true);
-                    }
-            } else {
+            int e = 0;
+            if constexpr (QP > 1) {
                 float top = 0.f;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
@@ -487,21 +613,21 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(value(d, i)));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const int e = exponent(top);
+                e = exponent(top);
                 unscale[0] = power_of_two(e);
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float a = value(d, 2 * i) * power_of_two(-e), b = value(d, 2 * i + 1) * power_of_two(-e);
-#pragma unroll
-                        for (int s = 0; s < QP; ++s) qf[d][i * QP + s] = take_part<Cache>(a, b, s == QP - 1);
-                    }
             }
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float a = value(d, 2 * i) * power_of_two(-e), b = value(d, 2 * i + 1) * power_of_two(-e);
+#pragma unroll
+                    for (int s = 0; s < QP; ++s) qf[d][i * QP + s] = take_part<Cache>(a, b);
+                }
         } else {
             __syncwarp();
             for (int r = 0; r < heads; ++r) {
-                const Act* src = (const Act*)(q_row0 + r * p.q_head);
+                const Act* src = (const Act*)(p.q + cc.b * p.q_seq + (first_head + r) * p.q_head);
                 float x[(DP + 31) / 32], top = 0.f;
 #pragma unroll
                 for (int i = 0; i < (DP + 31) / 32; ++i) {
@@ -523,204 +649,293 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
                     float rest = x[i] * power_of_two(-e), zero = 0.f;
 #pragma unroll
                     for (int s = 0; s < QP; ++s) {
-                        const uint32_t u = take_part<Cache>(rest, zero, s == QP - 1);
-                        if (d < p.dim) ((uint16_t*)(q_mem + (s * rows + r) * S::kRow))[d] = (uint16_t)u;
+                        const uint32_t u = take_part<Cache>(rest, zero);
+                        if (d < DP) ((uint16_t*)(q_mem + (s * rows + r) * kQRow))[d] = (uint16_t)u;
                     }
                 }
             }
             __syncwarp();
         }
-        const uint32_t q_lane = smem_addr(q_mem) + min(lane & 15, heads - 1) * S::kRow + (lane >> 4) * 16;
+        const uint32_t q_lane = smem_addr(q_mem) + min(lane & 15, heads - 1) * kQRow + (lane >> 4) * 16;
 
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t)
+        for (int t = 0; t < DP / 8; ++t) {
 #pragma unroll
-            for (int i = 0; i < 2 * R; ++i) o[t][i] = 0.f;
+            for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+            if constexpr (kKeep)
+#pragma unroll
+                for (int i = 0; i < 2 * R; ++i) o[t][i] = 0.f;
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             m[r] = -INFINITY;
-            l[r] = 0.f;
+            l[r] = l_sum[r] = 0.f;
         }
         bool row_bad = cc.len < 0;
         const int first_j = cc.j;
-        for (; cc.j < cc.end; ++cc.j) {
-            copy_wait<S::kStages - 2>();
-            __syncwarp();   // and every lane has read the stage before, which the next copy fills
-            row_bad |= (loader.bad_steps >> stage) & 1;
-            const uint32_t at = ring + stage * S::kStage;
-            loader.issue(stage == 0 ? S::kStages - 1 : stage - 1);
-
-            // ---- scores of the tile's rows and 16 keys: first the products of
-            // the first parts, and apart from them those of the rest
-            float sc[R][2][2];   // [row half][key tile][pair]
-            if constexpr (HALF) {
-                float c[2][2][4] = {}, e[2][4] = {};
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    uint32_t kf[4];
-                    ldsm4(kf, at + k_lane + d * 32);
-                    const uint32_t qa[4] = {qf[d][0], qf[d][QP == 1 ? 0 : 1], qf[d][QP == 1 ? 1 : QP], qf[d][QP == 1 ? 1 : QP + 1]};
-                    mma16816<Cache>(c[d & 1][0], qa, kf[0], kf[1]);
-                    mma16816<Cache>(c[d & 1][1], qa, kf[2], kf[3]);
-                    if constexpr (QP == 3) {
-                        const uint32_t q3[4] = {qf[d][2], qf[d][2], qf[d][5], qf[d][5]};
-                        mma16816<Cache>(e[0], q3, kf[0], kf[1]);
-                        mma16816<Cache>(e[1], q3, kf[2], kf[3]);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        sc[0][t][i] = c[0][t][i] + c[1][t][i];
-                        if constexpr (QP > 1)
-                            sc[0][t][i] = add_rest(sc[0][t][i], (c[0][t][2 + i] + c[1][t][2 + i]) + e[t][i]);
-                    }
-            } else {
-                float c[2][2][4] = {};
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    uint32_t kf[4];
-                    ldsm4(kf, at + k_lane + d * 32);
-#pragma unroll
-                    for (int s = 0; s < QP; ++s) {
-                        uint32_t qa[4];
-                        ldsm4(qa, q_lane + s * rows * S::kRow + d * 32);
-                        const int chain = QP == 1 ? d & 1 : s != 0;
-                        mma16816<Cache>(c[chain][0], qa, kf[0], kf[1]);
-                        mma16816<Cache>(c[chain][1], qa, kf[2], kf[3]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float a = c[0][t][2 * r + i], b = c[1][t][2 * r + i];
-                            sc[r][t][i] = QP == 1 ? a + b : add_rest(a, b);
-                        }
+        int fold = kFold, folds = 0;
+        // keys on even counts, then values; one copy of the code that waits and loads
+#pragma unroll 1
+        for (int n = 2 * (cc.end - cc.j); n > 0; --n) {
+            if (!bar_wait(bars + slot * 8, parity)) {   // give up, once the later loads had their time too
+                if (lane == 0) atomicExch(p.err, SB_DERR_TIMEOUT);
+                for (int i = 1; i < S::kSlots; ++i)
+                    bar_wait(bars + (slot + i) % S::kSlots * 8, parity ^ (slot + i >= S::kSlots));
+                return;
             }
-
-            // ---- the running softmax
+            const uint32_t at = ring + slot * S::kSlot;
             const int key0 = (cc.lo / kStep + cc.j) * kStep;
             const bool edge = key0 < cc.lo || key0 + kStep > cc.len;
-            float alpha[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float f = p.scale_log2 * unscale[r];
-                float top = m[r];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        sc[r][t][i] *= f;
-                        const int key = key0 + 8 * t + 2 * quad + i;
-                        if (edge && (key < cc.lo || key >= cc.len)) sc[r][t][i] = -INFINITY;
-                        top = fmaxf(top, sc[r][t][i]);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const float base = top == -INFINITY ? 0.f : top;
-                alpha[r] = exp2_fast(m[r] - base);
-                m[r] = top;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) sc[r][t][i] = exp2_fast(sc[r][t][i] - base + kUp);
-                l[r] = l[r] * alpha[r] + ((sc[r][0][0] + sc[r][0][1]) + (sc[r][1][0] + sc[r][1][1]));
-            }
-
-            // ---- weights as the A operand, in parts, times the values; the
-            // running sums are fp32 fmas, rounded to nearest
-            if constexpr (HALF) {
-                uint32_t w1[4], w2[4];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    w1[2 * t] = take_part<Cache>(sc[0][t][0], sc[0][t][1], false);
-                    w1[2 * t + 1] = take_part<Cache>(sc[0][t][0], sc[0][t][1], PP == 2);
-                    if constexpr (PP == 3) w2[2 * t] = w2[2 * t + 1] = take_part<Cache>(sc[0][t][0], sc[0][t][1], true);
-                }
+            if (!(n & 1)) {
+                row_bad |= (loader.bad >> slot) & 1;
+                // ---- scores of the tile's rows and 32 keys
+                float c[4][4] = {};
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    uint32_t vf[4];
-                    ldsm4t(vf, at + v_lane + d * 32);
+                    uint32_t kf[2][4];
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        float x[4] = {}, y[4] = {};
-                        mma16816<Cache>(x, w1, vf[2 * t], vf[2 * t + 1]);
-                        if constexpr (PP == 3) mma16816<Cache>(y, w2, vf[2 * t], vf[2 * t + 1]);
+                    for (int u = 0; u < 2; ++u)
+                        ldsm4(kf[u], ((at + k_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + u * 2048);
+                    if constexpr (HALF) {
+                        const uint32_t qa[4] = {qf[d][0], QP == 1 ? 0 : qf[d][1], qf[d][QP], QP == 1 ? 0 : qf[d][QP + 1]};
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            o[2 * d + t][i] = o[2 * d + t][i] * alpha[0] + add_rest(x[i], PP == 3 ? x[2 + i] + y[i] : x[2 + i]);
+                        for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], qa, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
+                        if constexpr (QP == 3) {
+                            const uint32_t q3[4] = {0, qf[d][2], 0, qf[d][5]};
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], q3, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < QP; ++s) {
+                            uint32_t qa[4];
+                            ldsm4(qa, q_lane + s * rows * kQRow + d * 32);
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], qa, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
+                        }
+                    }
+                }
+
+                // ---- the running softmax
+                float sc[R][4][2];   // [row half][key tile][pair]
+                bool move = false;
+                float top[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float f = p.scale_log2 * unscale[r];
+                    top[r] = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float s = c[t][2 * r + i];
+                            if (HALF && QP > 1) s += c[t][2 + i];
+                            s *= f;
+                            const int key = key0 + 8 * t + 2 * quad + i;
+                            if (edge && (key < cc.lo || key >= cc.len)) s = -INFINITY;
+                            sc[r][t][i] = s;
+                            top[r] = fmaxf(top[r], s);
+                        }
+                    move |= top[r] > m[r] + kLazy;
+                }
+                if (__any_sync(~0u, move)) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 1));
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 2));
+                        top[r] = fmaxf(top[r], m[r]);
+                        const float a = top[r] == -INFINITY ? 1.f : exp2_fast(m[r] - top[r]);
+                        m[r] = top[r];
+                        l[r] *= a, l_sum[r] *= a;
+#pragma unroll
+                        for (int t = 0; t < DP / 8; ++t) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                acc[t][2 * r + i] *= a;
+                                if (HALF) acc[t][2 + i] *= a;
+                                if constexpr (kKeep) o[t][2 * r + i] *= a;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kUp;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) sc[r][t][i] = exp2_fast(sc[r][t][i] - base);
+                        sum += sc[r][t][0] + sc[r][t][1];
+                    }
+                    l[r] += sum;
+                }
+                // in parts: each what the ones before leave
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if constexpr (HALF) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            float* v = sc[0][2 * u + t];
+                            wf[u][0][2 * t] = take_part<Cache>(v[0], v[1]);
+                            wf[u][0][2 * t + 1] = take_part<Cache>(v[0], v[1]);
+                            if constexpr (PP == 3) wf[u][PP - 2][2 * t] = 0, wf[u][PP - 2][2 * t + 1] = take_part<Cache>(v[0], v[1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < PP; ++s)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                float* v = sc[x & (R - 1)][2 * u + (x >> 1)];
+                                wf[u][s][x] = take_part<Cache>(v[0], v[1]);
+                            }
                     }
                 }
             } else {
-                uint32_t wf[PP][4];
-#pragma unroll
-                for (int s = 0; s < PP; ++s)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        wf[s][x] = take_part<Cache>(sc[x & (R - 1)][x >> 1][0], sc[x & (R - 1)][x >> 1][1], s == PP - 1);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    uint32_t vf[4];
-                    ldsm4t(vf, at + v_lane + d * 32);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        float x[4] = {}, y[4] = {};
-                        mma16816<Cache>(x, wf[0], vf[2 * t], vf[2 * t + 1]);
-#pragma unroll
-                        for (int s = 1; s < PP; ++s) mma16816<Cache>(y, wf[s], vf[2 * t], vf[2 * t + 1]);
-#pragma unroll
-                        for (int i = 0; i < 2 * R; ++i)
-                            o[2 * d + t][i] = o[2 * d + t][i] * alpha[i >> 1] + add_rest(x[i], y[i]);
+                if (edge) {   // zeros for the values outside the window
+                    uint8_t* mem = ring_mem + slot * S::kSlot;
+                    for (int i = lane; i < S::kSlot / 16; i += 32) {
+                        const int key = key0 + (i >> 3) % kStep;
+                        if (key < cc.lo || key >= cc.len) *(uint4*)(mem + i * 16) = make_uint4(0, 0, 0, 0);
                     }
+                    loader.dirty |= 1u << slot;
+                    __syncwarp();
                 }
+                // ---- weights times values
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        uint32_t vf[4];
+                        ldsm4t(vf, ((at + v_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + u * 2048);
+#pragma unroll
+                        for (int s = 0; s < (HALF ? PP - 1 : PP); ++s) {
+                            mma16816<Cache>(acc[2 * d], wf[u][s], vf[0], vf[1]);
+                            mma16816<Cache>(acc[2 * d + 1], wf[u][s], vf[2], vf[3]);
+                        }
+                    }
+
+                // ---- the MMA's sums to the rounded ones
+                if (--fold == 0) {
+                    fold = kFold;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        l_sum[r] += l[r];
+                        l[r] = 0.f;
+                        if constexpr (kKeep) {
+#pragma unroll
+                            for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    o[t][2 * r + i] += HALF ? acc[t][i] + acc[t][2 + i] : acc[t][2 * r + i];
+                                    acc[t][2 * r + i] = 0.f;
+                                    if (HALF) acc[t][2 + i] = 0.f;
+                                }
+                        } else {   // in memory, each lane its own; with the reference they were added at
+                            const int row = g + 8 * r;
+                            if (row >= heads) continue;
+                            const float a = folds ? exp2_fast(sums[row * 4 + quad] - m[r]) : 0.f;
+#pragma unroll
+                            for (int t = 0; t < DP / 8; ++t) {
+                                float2* at2 = (float2*)(sums + 64 + row * DP + t * 8 + 2 * quad);
+                                float2 x = folds ? *at2 : make_float2(0.f, 0.f);
+                                x.x = x.x * a + (HALF ? acc[t][0] + acc[t][2] : acc[t][2 * r]);
+                                x.y = x.y * a + (HALF ? acc[t][1] + acc[t][3] : acc[t][2 * r + 1]);
+                                *at2 = x;
+                            }
+                            sums[row * 4 + quad] = m[r];
+                        }
+                    }
+                    if constexpr (!kKeep)
+#pragma unroll
+                        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+                    ++folds;
+                }
+                ++cc.j;
             }
-            stage = stage + 1 == S::kStages ? 0 : stage + 1;
+            __syncwarp();   // every lane has read the slot
+            loader.issue(slot);
+            if (++slot == S::kSlots) slot = 0, parity ^= 1;
         }
 
-        // ---- the end of the row, or of this warp's part of it; the next row's
-        // queries are on their way meanwhile, where there are registers for them
+        // ---- the end of the row, or of this part of it; the next row's queries
+        // are on their way meanwhile, where there are registers for them
         const Cursor done = cc;
-        live = next_row(cc, seqs, p, until);
-        if (DP <= 128 && live) fetch_queries(cc);
+        live = loader.pushed > popped;
+        if (live) {
+            const int4 s = queue[popped++ % kQueue];
+            cc.b = s.x, cc.h = s.y, cc.part = s.w;
+            cc.until = parts.end(s.w);
+            cc.row_at = seqs.pre[s.x] * n_rows + s.y * (seqs.pre[s.x + 1] - seqs.pre[s.x]);
+            enter_row(cc, seqs, p, s.z);
+            if (kKeep) fetch_queries(cc);
+        }
+        const bool whole = first_j == 0 && done.end == done.steps, none = done.len == done.lo;
+        float* piece = p.pieces + (size_t)(2 * done.part + (first_j == 0)) * p.piece_floats;
+        if (!whole && first_j == 0 && lane == 0) {
+            p.cut_row[done.part] = done.b * n_rows + done.h;
+            p.cut_pieces[done.part] = (uint16_t)(parts.of(done.row_at + done.steps - 1) - done.part + 1);
+        }
+        unsigned odd[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+            l[r] += l_sum[r];
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
             if (row_bad) l[r] = __int_as_float(0x7fc00000);
-        }
-        const bool whole = first_j == 0 && done.end == done.steps;
-        float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
-        if (!whole && first_j == 0 && lane == 0)
-            p.cuts[w] = make_int2(done.b * n_rows + done.h, (int)(div_fast(done.row_at + done.steps - 1, part) - w + 1));
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
             const int row = g + 8 * r;
-            if (row >= heads) continue;
-            if (whole) {
+            bool fine = is_finite(l[r]);
+            if (row < heads) {
                 const size_t at = (size_t)done.b * p.n_q + first_head + row;
-                const bool none = done.len == done.lo;
-                const float inv = 1.f / l[r];
+                const float inv = none ? 0.f : 1.f / l[r];
+                const float a = !kKeep && folds ? exp2_fast(sums[row * 4 + quad] - m[r]) : 0.f;
                 Act* dst = (Act*)p.out + at * p.dim;
 #pragma unroll
-                for (int t = 0; t < DP / 8; ++t)
-                    if (t * 8 < p.dim) {
-                        dst[t * 8 + 2 * quad] = sb_from_float<Act>(none ? 0.f : o[t][2 * r] * inv);
-                        dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(none ? 0.f : o[t][2 * r + 1] * inv);
-                    }
-                if (p.lse && quad == 0)
-                    p.lse[at] = none ? -INFINITY : 0.69314718055994531f * (m[r] + (log2f(l[r]) - kUp));
-            } else {
-                if (quad == 0) *(float2*)(piece + 2 * row) = make_float2(m[r], l[r]);
+                for (int t = 0; t < DP / 8; ++t) {
+                    float x[2];
 #pragma unroll
-                for (int t = 0; t < DP / 8; ++t)
-                    *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(o[t][2 * r], o[t][2 * r + 1]);
+                    for (int i = 0; i < 2; ++i) {
+                        x[i] = HALF ? acc[t][i] + acc[t][2 + i] : acc[t][2 * r + i];
+                        if constexpr (kKeep) x[i] += o[t][2 * r + i];
+                    }
+                    if (!kKeep && folds) {
+                        const float2 y = *(const float2*)(sums + 64 + row * DP + t * 8 + 2 * quad);
+                        x[0] += y.x * a, x[1] += y.y * a;
+                    }
+                    fine &= is_finite(x[0]) && is_finite(x[1]);
+                    if (whole) {
+                        if (t * 8 < p.dim) {
+                            dst[t * 8 + 2 * quad] = sb_from_float<Act>(x[0] * inv);
+                            dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(x[1] * inv);
+                        }
+                    } else {
+                        *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(x[0], x[1]);
+                    }
+                }
+                if (quad == 0) {
+                    if (!whole)
+                        *(float2*)(piece + 2 * row) = make_float2(m[r], l[r]);
+                    else if (p.lse)
+                        p.lse[at] = none ? -INFINITY : 0.69314718055994531f * (m[r] + (log2f(l[r]) - kUp));
+                }
             }
+            odd[r] = __ballot_sync(~0u, row < heads && !fine && !row_bad);
         }
-        if (DP > 128 && live) fetch_queries(cc);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            while (odd[r]) {
+                const int src = __ffs(odd[r]) - 1, row = src / 4 + 8 * r;
+                odd[r] &= ~(0xfu << (src & ~3));
+                const float mr = __shfl_sync(~0u, m[r], src), lr = __shfl_sync(~0u, l[r], src);
+                __syncwarp();
+                const int base = done.lo / kStep;
+                redo_row<Cache, Act>(p, done.b, kv, first_head + row, max(done.lo, (base + first_j) * kStep),
+                                     min(done.len, (base + done.end) * kStep), mr, lr, kUp, whole, piece + 2 * row,
+                                     piece + 32 + row * DP, lane);
+            }
+        if (!kKeep && live) fetch_queries(cc);
     }
 }
 
@@ -730,46 +945,56 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) k_attend(const Atte
 // 32 of its columns, one per lane. Latency is all there is to it, so a unit is
 // joined by one warp where its row has at most 32 pieces and by the eight warps
 // of a CTA where it has more, with the pieces' loads in flight together.
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kMaxWarps = 148 * 2 * 8, kFew = 32;
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kFew = 32;
+constexpr int kBatch = 16;   // pieces whose loads are in flight together
 
 template <class Act, int DP>
-__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams p, int n_warps, float up) {
-    constexpr int kSlices = DP / 32, kPer = kMaxWarps / kJoinThreads + 1;
-    __shared__ short few[kMaxWarps], many[kMaxWarps];   // the warps that begin a cut row
-    __shared__ int counts[2][kPer * kJoinWarps];
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, float up) {
+    constexpr int kSlices = DP / 32;
+    __shared__ uint16_t few[kMaxParts], many[kMaxParts];   // the parts that begin a cut row
+    __shared__ int counts[2][kJoinWarps];
     __shared__ float red[2][kJoinWarps], sums[kJoinWarps][32];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.head->ready = 0;   // for a next call of the same number (a graph's)
 
-    // ---- the cut rows, in the order of the warps that begin them
+    // ---- the cut rows, in the order of the parts that begin them
     int n_few = 0, n_many = 0;
-    {
-        const int per = (n_warps + kJoinThreads - 1) / kJoinThreads, chunks = per * kJoinWarps;
-        for (int i = 0; i < per; ++i) {
-            const int w = i * kJoinThreads + threadIdx.x, n = w < n_warps ? p.cuts[w].y : 0;
-            const unsigned f = __ballot_sync(~0u, n > 0 && n <= kFew), y = __ballot_sync(~0u, n > kFew);
-            if (lane == 0) counts[0][i * kJoinWarps + wid] = __popc(f), counts[1][i * kJoinWarps + wid] = __popc(y);
+    const int n_parts = p.head->n_parts;
+    for (int base = 0; base < n_parts; base += kJoinThreads * 8) {   // 8 parts per thread
+        const int at = base + threadIdx.x * 8;
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (at < n_parts) raw = *(const uint4*)(p.cut_pieces + at);   // the array is padded to 8
+        uint16_t n[8];
+        memcpy(n, &raw, 16);
+        int f = 0, y = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (at + i >= n_parts) n[i] = 0;
+            f += n[i] > 0 && n[i] <= kFew, y += n[i] > kFew;
+        }
+        int before = f | y << 16;   // of both, in the lanes before and this one
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int x = __shfl_up_sync(~0u, before, s);
+            if (lane >= s) before += x;
         }
         __syncthreads();
-        for (int i = 0; i < per; ++i) {
-            int at_few = 0, at_many = 0;   // in the chunks before this warp's
-            n_few = n_many = 0;
-            for (int c = lane; c < chunks; c += 32) {
-                n_few += counts[0][c], n_many += counts[1][c];
-                if (c < i * kJoinWarps + wid) at_few += counts[0][c], at_many += counts[1][c];
-            }
-            n_few = __reduce_add_sync(~0u, n_few), n_many = __reduce_add_sync(~0u, n_many);
-            at_few = __reduce_add_sync(~0u, at_few), at_many = __reduce_add_sync(~0u, at_many);
-            if (n_few + n_many == 0) return;
-            const int w = i * kJoinThreads + threadIdx.x, n = w < n_warps ? p.cuts[w].y : 0;
-            const unsigned f = __ballot_sync(~0u, n > 0 && n <= kFew), y = __ballot_sync(~0u, n > kFew);
-            const unsigned before = (1u << lane) - 1;
-            if (f >> lane & 1) few[at_few + __popc(f & before)] = (short)w;
-            if (y >> lane & 1) many[at_many + __popc(y & before)] = (short)w;
-        }
+        if (lane == 31) counts[0][wid] = before & 0xffff, counts[1][wid] = before >> 16;
         __syncthreads();
+        int at_few = n_few + (before & 0xffff) - f, at_many = n_many + (before >> 16) - y;
+        for (int i = 0; i < kJoinWarps; ++i) {
+            if (i < wid) at_few += counts[0][i], at_many += counts[1][i];
+            n_few += counts[0][i], n_many += counts[1][i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (n[i] > 0 && n[i] <= kFew) few[at_few++] = (uint16_t)(at + i);
+            if (n[i] > kFew) many[at_many++] = (uint16_t)(at + i);
+        }
     }
+    __syncthreads();
     const int n_rows = p.n_kv * p.tiles, units = p.piece_rows * kSlices;
     auto place = [&](int row, int head, bool& real) -> size_t {   // of the output row
         const int b = row / n_rows, h = row % n_rows, tile = h % p.tiles;
@@ -785,10 +1010,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams
     // ---- rows of more than kFew pieces
     for (int u = blockIdx.x; u < n_many * units; u += gridDim.x) {
         const int w = many[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
-        const int2 cut = p.cuts[w];
-        const int n = cut.y;
+        const int row = p.cut_row[w], n = p.cut_pieces[w];
         bool real;
-        const size_t at = place(cut.x, head, real);
+        const size_t at = place(row, head, real);
         if (!real) continue;
         // this warp's pieces: wid, wid + 8, ..; 32 at a time, one per lane
         float top = -INFINITY, l = 0.f, a = 0.f;
@@ -802,10 +1026,18 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams
             top = t;
             l = l * old + f * ml.y;   // of this lane's pieces
             a *= old;
+            const float* src = piece(w, 1) - p.piece_floats * 2 + 32 + head * DP + col;   // piece k of the others
             const int here = min(32, (n - k0 + kJoinWarps - 1) / kJoinWarps);
-#pragma unroll 16
-            for (int i = 0; i < here; ++i)
-                a += __shfl_sync(~0u, f, i) * piece(w, k0 + i * kJoinWarps)[32 + head * DP + col];
+            for (int i0 = 0; i0 < here; i0 += kBatch) {
+                float x[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int k = k0 + (i0 + i) * kJoinWarps;
+                    x[i] = k < n ? src[(size_t)k * 2 * p.piece_floats + (k == 0 ? p.piece_floats : 0)] : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) a += __shfl_sync(~0u, f, i0 + i) * x[i];
+            }
         }
 #pragma unroll
         for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
@@ -830,10 +1062,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams
     // ---- the others
     for (int u = blockIdx.x * kJoinWarps + wid; u < n_few * units; u += gridDim.x * kJoinWarps) {
         const int w = few[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
-        const int2 cut = p.cuts[w];
-        const int n = cut.y;
+        const int row = p.cut_row[w], n = p.cut_pieces[w];
         bool real;
-        const size_t at = place(cut.x, head, real);
+        const size_t at = place(row, head, real);
         if (!real) continue;
         const float2 ml = lane < n ? *(const float2*)(piece(w, lane) + 2 * head) : make_float2(-INFINITY, 0.f);
         float top = ml.x;
@@ -843,8 +1074,13 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendParams
         float l = lane < n ? f * ml.y : 0.f, a = 0.f;
 #pragma unroll
         for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
-#pragma unroll 16
-        for (int k = 0; k < n; ++k) a += __shfl_sync(~0u, f, k) * piece(w, k)[32 + head * DP + col];
+        for (int k0 = 0; k0 < n; k0 += kBatch) {
+            float x[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) x[i] = k0 + i < n ? piece(w, k0 + i)[32 + head * DP + col] : 0.f;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) a += __shfl_sync(~0u, f, k0 + i) * x[i];
+        }
         finish(at, col, a, top, l);
     }
 }
@@ -862,46 +1098,105 @@ int sm_count() {
     return sms;
 }
 int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
-size_t cuts_bytes() { return ((size_t)sm_count() * 8 * sizeof(int2) + 255) / 256 * 256; }
-int piece_floats(int group, int dim) { return 32 + std::min(group, 16) * tile_width(dim); }
+int most_warps(int dim) { return dim <= 128 ? 8 : dim <= 192 ? 5 : 4; }   // Shape<>::kWarps
+int piece_floats(int group, int dim) { return 64 + std::min(group, 16) * tile_width(dim); }
+// The workspace: the header, the parts' cut rows, their pieces, the warps' sums.
+struct Layout {
+    size_t cut_pieces, cut_row, pieces, sums, bytes;
+    Layout(int group, int dim) {
+        const size_t warps = (size_t)sm_count() * most_warps(dim), parts = (3 * warps + 7) / 8 * 8;
+        const size_t piece = piece_floats(group, dim) * sizeof(float);
+        cut_pieces = 256;
+        cut_row = cut_pieces + parts * sizeof(uint16_t);
+        pieces = (cut_row + parts * sizeof(int) + 255) / 256 * 256;
+        sums = pieces + 2 * parts * piece;
+        bytes = sums + warps * piece;
+    }
+};
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = nullptr;
+    static bool looked = false;
+    if (!looked) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiled)f;
+        cudaGetLastError();
+        looked = true;
+    }
+    return fn;
+}
+// [pages][heads][slots][dim] with a box of p.box slots x 64 columns
+bool cache_map(CUtensorMap* map, const void* base, int type, const AttendParams& p, size_t page, size_t slot, size_t head) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+    // the stride of a dimension of one is never used, whatever the caller's
+    const cuuint64_t strides[3] = {p.page_size == 1 ? 16 : slot, p.n_kv == 1 ? 16 : head, p.n_pages == 1 ? 16 : page};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.box, 1, 1}, ones[4] = {1, 1, 1, 1};
+    return encode(map, type == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                  const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 template <class Cache, int DP, int QP, bool HALF>
 int launch(AttendParams p, cudaStream_t st) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
-    const int rows = std::min(p.group, 16);
-    const size_t per_warp = S::kStages * S::kStage + (HALF ? 0 : (size_t)rows * QP * S::kRow);
-    const size_t head = (12 * (size_t)p.n_seqs + 8 + 15) / 16 * 16;
+    constexpr bool kF16 = std::is_same<Cache, __half>::value;
+    const int q_rows = HALF ? 0 : std::min(p.group, 16) * QP;
+    const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16) + kQueue * sizeof(int4);
+    const size_t seqs = 12 * (size_t)p.n_seqs + 8;
     // static shared memory (the scan's warp sums) is 256 bytes
-    const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 512 - head) / per_warp);
-    const size_t bytes = head + warps * per_warp;
+    const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
     static bool opted = false;
     if (!opted) {
         if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kSmemLimit - 512), "attend shared memory"))
+                                             kSmemLimit - 1024), "attend shared memory"))
             return -1;
         opted = true;
     }
+    const int type = kF16 ? SB_F16 : SB_BF16;
+    p.box = 16;
+    while (p.page_size % p.box) p.box /= 2;
+    CUtensorMap kmap{}, vmap{};
+    if (p.n_pages > 0 && (!cache_map(&kmap, p.k, type, p, p.k_page, p.k_slot, p.k_head) ||
+                          !cache_map(&vmap, p.v, type, p, p.v_page, p.v_slot, p.v_head))) {
+        sb_set_error("attend: no tensor map for a cache of %d pages of %d, strides %zu / %zu / %zu and %zu / %zu / %zu bytes",
+                     p.n_pages, p.page_size, p.k_page, p.k_slot, p.k_head, p.v_page, p.v_slot, p.v_head);
+        return -1;
+    }
+    // steps of the longest row that fits; none is cut where that is short
+    const long long longest = std::min((long long)p.table_width * p.page_size,
+                                       p.window > 0 ? p.window + kStep - 1ll : 1ll << 40);
+    const bool cuts = longest > kWhole * kStep;
+    static std::atomic<unsigned long long> calls{0x5361626168000001ull};
+    p.share = cuts;
+    p.call = calls.fetch_add(1);
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = sm_count();
     cfg.blockDim = warps * 32;
-    cfg.dynamicSmemBytes = bytes;
+    cfg.dynamicSmemBytes = warps * per_warp + seqs;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, HALF>, (const AttendParams)p), "attend launch")) return -1;
-    const long long longest = std::min((long long)p.table_width * p.page_size,
-                                       p.window > 0 ? p.window + kStep - 1ll : 1ll << 40);
-    if (longest <= kWhole * kStep) return 0;   // no row can be cut
-    const int n_warps = sm_count() * warps;
+    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, HALF>, (const AttendParams)p, (const CUtensorMap)kmap,
+                                       (const CUtensorMap)vmap), "attend launch"))
+        return -1;
+    if (!cuts) return 0;
     cfg.gridDim = 2 * sm_count();
     cfg.blockDim = kJoinThreads;
     cfg.dynamicSmemBytes = 0;
-    const float up = std::is_same<Cache, __half>::value ? 12.f : 0.f;
-    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act, DP>, (const AttendParams)p, n_warps, up), "attend join launch")
+    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act, DP>, (const AttendParams)p, up_of(kF16)), "attend join launch")
                ? 0 : -1;
 }
 
@@ -924,7 +1219,7 @@ int launch_group(const AttendParams& p, cudaStream_t st) {
 
 SABAH_API size_t sabah_attend_paged_workspace(int n_q_heads, int n_kv_heads, int head_dim) {
     if (n_kv_heads <= 0 || n_q_heads <= 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
-    return cuts_bytes() + (size_t)sm_count() * 8 * 2 * piece_floats(n_q_heads / n_kv_heads, head_dim) * sizeof(float);
+    return Layout(n_q_heads / n_kv_heads, head_dim).bytes;
 }
 
 SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_head_stride, int act_type,
@@ -983,8 +1278,13 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     p.tiles = (p.group + 15) / 16;
     p.piece_rows = std::min(p.group, 16);
     p.piece_floats = piece_floats(p.group, head_dim);
-    p.cuts = (int2*)d_workspace;
-    p.pieces = (float*)((uint8_t*)d_workspace + cuts_bytes());
+    const Layout lay(p.group, head_dim);
+    uint8_t* ws = (uint8_t*)d_workspace;
+    p.head = (Header*)ws;
+    p.cut_pieces = (uint16_t*)(ws + lay.cut_pieces);
+    p.cut_row = (int*)(ws + lay.cut_row);
+    p.pieces = (float*)(ws + lay.pieces);
+    p.sums = (float*)(ws + lay.sums);
     const int slot = sb_timing_begin("attend_paged", st);
     int rc = 0;
     for (int b = 0; b < n_seqs && rc == 0; b += kMaxSeqs) {
