@@ -8,10 +8,11 @@
 // [lo, len) counts, and no table entry outside it is read.
 //
 // Bound: DRAM, every key and value row once. A key-value head's query heads
-// (up to 16: the rows of an MMA tile) are taken together, so the rows are read
-// once for all of them; the arithmetic is 16-row mma.sync on 32 keys at a time,
-// a fraction of the tensor rate and well under the time the rows take to
-// arrive. tcgen05's 128-row tiles would be 87-99% padding here.
+// (up to 16) are taken together, so the rows are read once for all of them. The
+// arithmetic is mma.sync with keys (then value columns) as the 16 rows of the
+// tile and 8 query heads as its columns, a fraction of the tensor rate and under
+// the time the rows take to arrive: with the heads as rows half the tile or more
+// would be padding, and tcgen05's 128 rows would be 87-99% of it.
 //
 // The work is a list of steps of 32 keys over all (sequence, key-value head)
 // rows, cut into equal parts whatever the lengths: one long sequence spreads
@@ -94,7 +95,7 @@ struct AttendParams {
     int* cut_row;           // and which row
     float* pieces;          // per part two: the row it enters in the middle of, the row it leaves early
     float* sums;            // per warp one: its rounded sums, where registers have no room for them
-    int piece_floats, piece_rows;
+    int piece_floats, piece_rows, max_parts;
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -105,12 +106,13 @@ __device__ inline void bar_init(uint32_t bar, int count) {
 __device__ inline void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// bounded: false after about 2 s
+// Bounded: false after 2^24 tries, a second or more. No suspend-time hint: a
+// warp that sleeps on the barrier wakes microseconds late.
 __device__ inline bool bar_wait(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < 1 << 17; ++i) {
+    for (int i = 0; i < 1 << 24; ++i) {
         uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000) : "memory");
+        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
     }
     return false;
@@ -182,40 +184,35 @@ constexpr float up_of(bool f16) { return f16 ? 11.f : 0.f; }
 // A row takes its steps, then kRowCost idle places in the list, so that parts
 // of many short rows and parts of one long row take as long.
 struct Seqs {
-    long long* pre;   // [n_seqs + 1]
+    int* pre;         // [n_seqs + 1]
     int* len;         // [n_seqs], -1 where out of range
 };
 __device__ inline int window_start(int len, int window) { return window > 0 ? max(0, len - window) : 0; }
 __device__ inline int seq_steps(int len, int window) {
     return len <= 0 ? 1 : (len + kStep - 1) / kStep - window_start(len, window) / kStep;
 }
-// a / b of non-negative numbers; the 64-bit division is a long subroutine
-__device__ inline long long div_fast(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
-}
 // The parts: n_own of `own` places, one per warp, then shared ones of `small`.
 struct Parts {
-    long long cost, own, own_end, small;
-    int n_own, n;
-    __device__ Parts(long long cost_, int warps, bool share) : cost(cost_) {
-        own = max(div_fast(cost + warps - 1, warps), (long long)kMinSteps);
+    int cost, own, own_end, small, n_own, n;
+    __device__ Parts(int cost_, int warps, bool share) : cost(cost_) {
+        own = max((int)((unsigned)(cost + warps - 1) / (unsigned)warps), kMinSteps);
         if (share && own >= kShare) {
             own = own * 13 / 16;
             n_own = warps;
             own_end = own * warps;
-            const long long rest = cost - own_end;
-            small = max(div_fast(rest + 2 * warps - 1, 2 * warps), (long long)kMinSteps);
-            n = n_own + (int)div_fast(rest + small - 1, small);
+            const unsigned rest = cost - own_end;
+            small = max((int)((rest + 2 * warps - 1) / (2 * warps)), kMinSteps);
+            n = n_own + (int)((rest + small - 1) / small);
         } else {
-            n = n_own = (int)div_fast(cost + own - 1, own);
+            n = n_own = (int)((unsigned)(cost + own - 1) / (unsigned)own);
             own_end = cost;
             small = 1;
         }
     }
-    __device__ long long begin(int i) const { return i < n_own ? i * own : own_end + (i - n_own) * small; }
-    __device__ long long end(int i) const { return i < n_own ? min((i + 1) * own, own_end) : min(own_end + (i + 1 - n_own) * small, cost); }
-    __device__ int of(long long at) const {
-        return at < own_end ? (int)div_fast(at, own) : n_own + (int)div_fast(at - own_end, small);
+    __device__ int begin(int i) const { return i < n_own ? i * own : own_end + (i - n_own) * small; }
+    __device__ int end(int i) const { return i < n_own ? min((i + 1) * own, own_end) : min(own_end + (i + 1 - n_own) * small, cost); }
+    __device__ int of(int at) const {
+        return at < own_end ? (int)((unsigned)at / (unsigned)own) : n_own + (int)((unsigned)(at - own_end) / (unsigned)small);
     }
 };
 
@@ -225,15 +222,15 @@ struct Cursor {
     int j, end, steps;   // step in the row, where the part leaves it, the row's steps
     int len, lo;
     int part;
-    long long row_at, until;   // the row's first place in the list, the part's end
+    int row_at, until;   // the row's first place in the list, the part's end
 };
 // starts the row at c.b, c.h, from its step j on
 __device__ inline void enter_row(Cursor& c, const Seqs& s, const AttendParams& p, int j) {
     c.len = s.len[c.b];
     c.lo = window_start(max(c.len, 0), p.window);
-    c.steps = (int)(s.pre[c.b + 1] - s.pre[c.b]) - kRowCost;
+    c.steps = s.pre[c.b + 1] - s.pre[c.b] - kRowCost;
     c.j = j;
-    c.end = c.steps <= kWhole ? c.steps : (int)min((long long)c.steps, c.until - c.row_at);
+    c.end = c.steps <= kWhole ? c.steps : min(c.steps, c.until - c.row_at);
 }
 // false at the end of the part
 __device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p) {
@@ -247,7 +244,7 @@ __device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p)
     return true;
 }
 // the first step of a part; b = -1 where the part has none of its own
-__device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, long long from, long long until, int part, int lane) {
+__device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, int from, int until, int part, int lane) {
     const int n_rows = p.n_kv * p.tiles;
     Cursor c;
     c.part = part;
@@ -261,8 +258,8 @@ __device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, l
         a += last * hop;
     }
     c.b = a;
-    const long long at = from - s.pre[a] * n_rows, cost = s.pre[a + 1] - s.pre[a];
-    c.h = (int)div_fast(at, cost);
+    const unsigned at = from - s.pre[a] * n_rows, cost = s.pre[a + 1] - s.pre[a];
+    c.h = (int)(at / cost);
     const int j = (int)(at - c.h * cost);
     c.row_at = from - j;
     enter_row(c, s, p, j);
@@ -414,6 +411,16 @@ struct Loader {
     }
 };
 
+// ------------------------------------------------------------ pieces
+// m and l of each head, then the running sums as the lanes hold them: for 8
+// heads and 16 columns a float4 per lane, of (column, head) = (lane / 4, 2 (lane
+// % 4)), the next head, and both at column + 8.
+constexpr int kPieceHead = 32;
+__host__ __device__ inline int frag_at(int head, int col, int dp) {
+    const int lane = col % 8 * 4 + head % 8 / 2;
+    return ((head / 8 * (dp / 16) + col / 16) * 32 + lane) * 4 + col % 16 / 8 * 2 + head % 2;
+}
+
 // ------------------------------------------------------------ infinities
 // Products of parts make NaN of what is an infinity in the formula (0 * inf,
 // inf - inf between parts). Where a row's result is not finite, its columns that
@@ -421,7 +428,7 @@ struct Loader {
 // [from, to); all of them where the softmax's own sum is not finite.
 template <class Cache, class Act>
 __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int head, int from, int to, float m, float l,
-                                      float up, bool whole, float* ml, float* piece, int lane) {
+                                      float up, bool whole, float* piece, int row, int dp, int lane) {
     constexpr int N = kMaxDim / 32;
     const Act* q = (const Act*)(p.q + b * p.q_seq + head * p.q_head);
     float o[N] = {}, top = -INFINITY, sum = 0.f;
@@ -450,13 +457,14 @@ __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int 
         if (d >= p.dim) break;
         if (whole) {
             if (all || !is_finite(sb_to_float(out[d]))) out[d] = sb_from_float<Act>(o[i] / sum);
-        } else if (all || !is_finite(piece[d])) {
-            piece[d] = o[i] * scale;
+        } else {
+            float* x = piece + kPieceHead + frag_at(row, d, dp);
+            if (all || !is_finite(*x)) *x = o[i] * scale;
         }
     }
     if (all && lane == 0) {
         if (!whole)
-            ml[0] = top, ml[1] = sum * scale;
+            piece[2 * row] = top, piece[2 * row + 1] = sum * scale;
         else if (p.lse)
             p.lse[at] = 0.69314718055994531f * (top + log2f(sum));
     }
@@ -464,34 +472,31 @@ __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int 
 
 // ------------------------------------------------------------ the kernel
 // QP: parts of a query value (1: it has the cache's type); the weights take as
-// many, and at least two. HALF: at most 8 query heads per key-value head; the
-// tile's rows 8-15 then hold the second parts of rows 0-7, so one MMA multiplies
-// both parts, and the query fragments stay in registers. With 9-16 heads each
-// part is an MMA of its own and the queries lie in shared memory.
-template <class Cache, int DP, int QP, bool HALF>
+// many, and at least two. NT: tiles of 8 query heads. With one, the query
+// fragments stay in registers; with two they are read from shared memory.
+template <class Cache, int DP, int QP, int NT>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     k_attend(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
              const __grid_constant__ CUtensorMap vmap) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
     constexpr int PP = QP == 1 ? 2 : QP;
-    constexpr int R = HALF ? 1 : 2;          // row halves with heads of their own
     constexpr int ND = DP / 16;
     constexpr float kUp = up_of(std::is_same<Cache, __half>::value);
-    // rounded sums stay in registers up to 128 columns
-    constexpr bool kKeep = DP <= 128;
+    // rounded sums stay in registers where there is room for them
+    constexpr bool kKeep = ND * (8 * NT + (NT == 1 ? 2 * QP : 0)) <= 160;
     constexpr int kFold = QP == 1 ? 32 : 8;
     constexpr int kQRow = DP * 2 + 16;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-    const int rows = min(p.group, 16), q_rows = HALF ? 0 : rows * QP;
+    const int rows = min(p.group, 16), q_rows = NT == 1 ? 0 : rows * QP;
     uint8_t* q_mem = smem + n_warps * S::kSlots * S::kSlot + wid * q_rows * kQRow;
     uint8_t* tail = smem + n_warps * (S::kSlots * S::kSlot + q_rows * kQRow);
     int4* queue = (int4*)tail + wid * kQueue;
     tail += n_warps * kQueue * sizeof(int4);
     const uint32_t bars = smem_addr(tail) + wid * S::kSlots * 8;
     tail += n_warps * S::kSlots * 8;
-    Seqs seqs{(long long*)tail, (int*)(tail + 8 * (p.n_seqs + 1))};
+    Seqs seqs{(int*)tail, (int*)tail + p.n_seqs + 1};
 
     if (lane < S::kSlots) bar_init(bars + lane * 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -507,10 +512,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     }
 
     // ---- the scan of the lengths
-    __shared__ long long warp_sum[32];
+    __shared__ int warp_sum[32];
     {
         const int per = (p.n_seqs + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per;
-        long long sum = 0;
+        int sum = 0;
         for (int b = b0; b < min(b0 + per, p.n_seqs); ++b) {
             int len = p.lens[b];
             if (len < 0 || len > (long long)p.table_width * p.page_size) {
@@ -520,10 +525,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             seqs.len[b] = len;
             sum += seq_steps(len, p.window) + kRowCost;
         }
-        long long run = sum;
+        int run = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(~0u, run, o);
+            const int x = __shfl_up_sync(~0u, run, o);
             if (lane >= o) run += x;
         }
         if (lane == 31) warp_sum[wid] = run;
@@ -549,9 +554,9 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 
     // ---- queries on their way, then keys and values
     const int g = lane >> 2, quad = lane & 3;
-    Act qx[HALF ? ND : 1][4];   // the row's query values 16 d + 2 quad + {0, 1, 8, 9}, as they are
+    Act qx[NT == 1 ? ND : 1][4];   // the row's query values 16 d + 2 quad + {0, 1, 8, 9}, as they are
     auto fetch_queries = [&](const Cursor& c) {
-        if constexpr (HALF) {
+        if constexpr (NT == 1) {
             const Act* src = (const Act*)(p.q + c.b * p.q_seq + (c.h * p.group + min(g, p.group - 1)) * p.q_head);
             if (p.q_pairs) {
                 struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
@@ -581,15 +586,17 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll 1
     for (int i = 0; i < S::kSlots; ++i) loader.issue(i);
 
-    // ---- the computing side
-    float acc[DP / 8][4];                          // the MMA's sums; HALF: rows 8-15 are the second parts'
-    float o[kKeep ? DP / 8 : 1][2 * R], m[R], l[R], l_sum[R], unscale[R];
-    uint32_t qf[HALF ? ND : 1][2 * QP];            // HALF: per 16 dimensions, the parts of both 8s
-    const int k_row = (lane >> 4) * 8 + (lane & 7), v_row = ((lane >> 3) & 1) * 8 + (lane & 7);
-    const uint32_t k_lane = k_row * 128 + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
-    const uint32_t v_lane = v_row * 128 + (((lane >> 4) ^ (v_row & 7)) << 4);
+    // ---- the computing side. A lane's columns are heads 8 u + 2 quad and the
+    // next; of a 16-row tile it holds rows g and g + 8.
+    float acc[NT][ND][4];                          // the MMA's sums: 16 columns of the values x 8 heads
+    float o[kKeep ? NT : 1][kKeep ? ND : 1][4];    // the rounded ones
+    float m[2 * NT], l[2 * NT], l_sum[2 * NT], unscale[2 * NT], m_fold[2 * NT];
+    uint32_t qf[NT == 1 ? ND : 1][2 * QP];         // per 16 dimensions the parts of both 8s, as the B operand
+    uint32_t wf[2][NT][PP][2];                     // the weights as the B operand, per 16 keys and part
+    const int k_row = ((lane >> 3) & 1) * 8 + (lane & 7), v_row = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t k_lane = k_row * 128 + (((lane >> 4) ^ (k_row & 7)) << 4);
+    const uint32_t v_lane = v_row * 128 + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
     float* sums = p.sums + (size_t)w * p.piece_floats;
-    uint32_t wf[2][HALF ? PP - 1 : PP][4];         // the weights as the A operand, per 16 keys and part
     int slot = 0, popped = 1;
     uint32_t parity = 0;
     for (bool live = true; live;) {
@@ -598,13 +605,13 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 
         // ---- this row's queries, split into parts
 #pragma unroll
-        for (int r = 0; r < R; ++r) unscale[r] = 1.f;
-        if constexpr (HALF) {
+        for (int c = 0; c < 2 * NT; ++c) unscale[c] = p.scale_log2;
+        if constexpr (NT == 1) {   // of head g
             // values past the head size are zero
             auto value = [&](int d, int i) {
                 return 16 * d + 2 * quad + (i >> 1) * 8 < p.dim ? sb_to_float(qx[d][i]) : 0.f;
             };
-            int e = 0;
+            float down = 1.f;
             if constexpr (QP > 1) {
                 float top = 0.f;
 #pragma unroll
@@ -613,14 +620,16 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(value(d, i)));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                e = exponent(top);
-                unscale[0] = power_of_two(e);
+                const int e = exponent(top);
+                down = power_of_two(-e);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) unscale[c] *= power_of_two(__shfl_sync(~0u, e, 4 * (2 * quad + c)));
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float a = value(d, 2 * i) * power_of_two(-e), b = value(d, 2 * i + 1) * power_of_two(-e);
+                    float a = value(d, 2 * i) * down, b = value(d, 2 * i + 1) * down;
 #pragma unroll
                     for (int s = 0; s < QP; ++s) qf[d][i * QP + s] = take_part<Cache>(a, b);
                 }
@@ -640,8 +649,9 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll
                     for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
                     e = exponent(top);
-                    if (r == g) unscale[0] = power_of_two(e);
-                    if (r == g + 8) unscale[R - 1] = power_of_two(e);
+#pragma unroll
+                    for (int c = 0; c < 2 * NT; ++c)
+                        if (r == c / 2 * 8 + 2 * quad + c % 2) unscale[c] *= power_of_two(e);
                 }
 #pragma unroll
                 for (int i = 0; i < (DP + 31) / 32; ++i) {
@@ -656,20 +666,21 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             }
             __syncwarp();
         }
-        const uint32_t q_lane = smem_addr(q_mem) + min(lane & 15, heads - 1) * kQRow + (lane >> 4) * 16;
+        const uint32_t q_lane = smem_addr(q_mem) + min((lane >> 4) * 8 + (lane & 7), heads - 1) * kQRow + ((lane >> 3) & 1) * 16;
 
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t) {
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-            if constexpr (kKeep)
+            for (int t = 0; t < ND; ++t)
 #pragma unroll
-                for (int i = 0; i < 2 * R; ++i) o[t][i] = 0.f;
-        }
+                for (int i = 0; i < 4; ++i) {
+                    acc[u][t][i] = 0.f;
+                    if constexpr (kKeep) o[u][t][i] = 0.f;
+                }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            m[r] = -INFINITY;
-            l[r] = l_sum[r] = 0.f;
+        for (int c = 0; c < 2 * NT; ++c) {
+            m[c] = -INFINITY;
+            l[c] = l_sum[c] = 0.f;
         }
         bool row_bad = cc.len < 0;
         const int first_j = cc.j;
@@ -688,108 +699,81 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             const bool edge = key0 < cc.lo || key0 + kStep > cc.len;
             if (!(n & 1)) {
                 row_bad |= (loader.bad >> slot) & 1;
-                // ---- scores of the tile's rows and 32 keys
-                float c[4][4] = {};
+                // ---- scores of 32 keys and the tile's heads
+                float c[2][NT][4] = {};
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     uint32_t kf[2][4];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        ldsm4(kf[u], ((at + k_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + u * 2048);
-                    if constexpr (HALF) {
-                        const uint32_t qa[4] = {qf[d][0], QP == 1 ? 0 : qf[d][1], qf[d][QP], QP == 1 ? 0 : qf[d][QP + 1]};
+                    for (int h = 0; h < 2; ++h)
+                        ldsm4(kf[h], ((at + k_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + h * 2048);
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], qa, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
-                        if constexpr (QP == 3) {
-                            const uint32_t q3[4] = {0, qf[d][2], 0, qf[d][5]};
+                    for (int s = 0; s < QP; ++s) {
+                        uint32_t qb[4];
+                        if constexpr (NT == 1)
+                            qb[0] = qf[d][s], qb[1] = qf[d][QP + s];
+                        else
+                            ldsm4(qb, q_lane + s * rows * kQRow + d * 32);
 #pragma unroll
-                            for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], q3, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
-                        }
-                    } else {
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int s = 0; s < QP; ++s) {
-                            uint32_t qa[4];
-                            ldsm4(qa, q_lane + s * rows * kQRow + d * 32);
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) mma16816<Cache>(c[t], qa, kf[t >> 1][2 * (t & 1)], kf[t >> 1][2 * (t & 1) + 1]);
-                        }
+                            for (int u = 0; u < NT; ++u) mma16816<Cache>(c[h][u], kf[h], qb[2 * u], qb[2 * u + 1]);
                     }
                 }
 
                 // ---- the running softmax
-                float sc[R][4][2];   // [row half][key tile][pair]
                 bool move = false;
-                float top[R];
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float f = p.scale_log2 * unscale[r];
-                    top[r] = -INFINITY;
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
+                    for (int u = 0; u < NT; ++u)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float s = c[t][2 * r + i];
-                            if (HALF && QP > 1) s += c[t][2 + i];
-                            s *= f;
-                            const int key = key0 + 8 * t + 2 * quad + i;
-                            if (edge && (key < cc.lo || key >= cc.len)) s = -INFINITY;
-                            sc[r][t][i] = s;
-                            top[r] = fmaxf(top[r], s);
+                        for (int i = 0; i < 4; ++i) {
+                            float& s = c[h][u][i];
+                            s *= unscale[2 * u + i % 2];
+                            if (edge) {
+                                const int key = key0 + 16 * h + g + i / 2 * 8;
+                                if (key < cc.lo || key >= cc.len) s = -INFINITY;
+                            }
+                            move |= s > m[2 * u + i % 2] + kLazy;
                         }
-                    move |= top[r] > m[r] + kLazy;
-                }
                 if (__any_sync(~0u, move)) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 1));
-                        top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 2));
-                        top[r] = fmaxf(top[r], m[r]);
-                        const float a = top[r] == -INFINITY ? 1.f : exp2_fast(m[r] - top[r]);
-                        m[r] = top[r];
-                        l[r] *= a, l_sum[r] *= a;
+                    for (int x = 0; x < 2 * NT; ++x) {
+                        const int u = x / 2, i = x % 2;
+                        float top = fmaxf(fmaxf(c[0][u][i], c[0][u][i + 2]), fmaxf(c[1][u][i], c[1][u][i + 2]));
 #pragma unroll
-                        for (int t = 0; t < DP / 8; ++t) {
+                        for (int s = 4; s <= 16; s <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+                        top = fmaxf(top, m[x]);
+                        const float a = top == -INFINITY ? 1.f : exp2_fast(m[x] - top);
+                        m[x] = top;
+                        if (cc.j == first_j) continue;   // nothing to rescale yet
+                        l[x] *= a, l_sum[x] *= a;
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                acc[t][2 * r + i] *= a;
-                                if (HALF) acc[t][2 + i] *= a;
-                                if constexpr (kKeep) o[t][2 * r + i] *= a;
-                            }
+                        for (int t = 0; t < ND; ++t) {
+                            acc[u][t][i] *= a, acc[u][t][i + 2] *= a;
+                            if constexpr (kKeep) o[u][t][i] *= a, o[u][t][i + 2] *= a;
                         }
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kUp;
-                    float sum = 0.f;
+                for (int u = 0; u < NT; ++u) {
+                    float base[2], sum[2] = {};
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
+                    for (int i = 0; i < 2; ++i) base[i] = (m[2 * u + i] == -INFINITY ? 0.f : m[2 * u + i]) - kUp;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) sc[r][t][i] = exp2_fast(sc[r][t][i] - base);
-                        sum += sc[r][t][0] + sc[r][t][1];
-                    }
-                    l[r] += sum;
-                }
-                // in parts: each what the ones before leave
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if constexpr (HALF) {
+                        for (int i = 0; i < 2; ++i) {   // rows g, then g + 8
+                            float a = exp2_fast(c[h][u][2 * i] - base[0]), b = exp2_fast(c[h][u][2 * i + 1] - base[1]);
+                            sum[0] += a, sum[1] += b;
+                            // in parts, each what the ones before leave; transposed to the B operand
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            float* v = sc[0][2 * u + t];
-                            wf[u][0][2 * t] = take_part<Cache>(v[0], v[1]);
-                            wf[u][0][2 * t + 1] = take_part<Cache>(v[0], v[1]);
-                            if constexpr (PP == 3) wf[u][PP - 2][2 * t] = 0, wf[u][PP - 2][2 * t + 1] = take_part<Cache>(v[0], v[1]);
+                            for (int s = 0; s < PP; ++s)
+                                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                                             : "=r"(wf[h][u][s][i]) : "r"(take_part<Cache>(a, b)));
                         }
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < PP; ++s)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                float* v = sc[x & (R - 1)][2 * u + (x >> 1)];
-                                wf[u][s][x] = take_part<Cache>(v[0], v[1]);
-                            }
-                    }
+                    l[2 * u] += sum[0], l[2 * u + 1] += sum[1];
                 }
             } else {
                 if (edge) {   // zeros for the values outside the window
@@ -801,56 +785,49 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                     loader.dirty |= 1u << slot;
                     __syncwarp();
                 }
-                // ---- weights times values
+                // ---- values, transposed, times weights
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
+                    for (int t = 0; t < ND; ++t) {
                         uint32_t vf[4];
-                        ldsm4t(vf, ((at + v_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + u * 2048);
+                        ldsm4t(vf, ((at + v_lane) ^ ((t & 3) << 5)) + (t >> 2) * S::kTileBytes + h * 2048);
 #pragma unroll
-                        for (int s = 0; s < (HALF ? PP - 1 : PP); ++s) {
-                            mma16816<Cache>(acc[2 * d], wf[u][s], vf[0], vf[1]);
-                            mma16816<Cache>(acc[2 * d + 1], wf[u][s], vf[2], vf[3]);
-                        }
+                        for (int u = 0; u < NT; ++u)
+#pragma unroll
+                            for (int s = 0; s < PP; ++s) mma16816<Cache>(acc[u][t], vf, wf[h][u][s][0], wf[h][u][s][1]);
                     }
 
                 // ---- the MMA's sums to the rounded ones
                 if (--fold == 0) {
                     fold = kFold;
+                    float a[2 * NT];
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        l_sum[r] += l[r];
-                        l[r] = 0.f;
-                        if constexpr (kKeep) {
-#pragma unroll
-                            for (int t = 0; t < DP / 8; ++t)
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    o[t][2 * r + i] += HALF ? acc[t][i] + acc[t][2 + i] : acc[t][2 * r + i];
-                                    acc[t][2 * r + i] = 0.f;
-                                    if (HALF) acc[t][2 + i] = 0.f;
-                                }
-                        } else {   // in memory, each lane its own; with the reference they were added at
-                            const int row = g + 8 * r;
-                            if (row >= heads) continue;
-                            const float a = folds ? exp2_fast(sums[row * 4 + quad] - m[r]) : 0.f;
-#pragma unroll
-                            for (int t = 0; t < DP / 8; ++t) {
-                                float2* at2 = (float2*)(sums + 64 + row * DP + t * 8 + 2 * quad);
-                                float2 x = folds ? *at2 : make_float2(0.f, 0.f);
-                                x.x = x.x * a + (HALF ? acc[t][0] + acc[t][2] : acc[t][2 * r]);
-                                x.y = x.y * a + (HALF ? acc[t][1] + acc[t][3] : acc[t][2 * r + 1]);
-                                *at2 = x;
-                            }
-                            sums[row * 4 + quad] = m[r];
+                    for (int x = 0; x < 2 * NT; ++x) {
+                        l_sum[x] += l[x];
+                        l[x] = 0.f;
+                        if constexpr (!kKeep) {   // in memory, with the reference that they were added at
+                            a[x] = folds ? exp2_fast(m_fold[x] - m[x]) : 0.f;
+                            m_fold[x] = m[x];
                         }
                     }
-                    if constexpr (!kKeep)
 #pragma unroll
-                        for (int t = 0; t < DP / 8; ++t)
+                    for (int u = 0; u < NT; ++u)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+                        for (int t = 0; t < ND; ++t) {
+                            if constexpr (kKeep) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[u][t][i] += acc[u][t][i];
+                            } else {
+                                float4* mem = (float4*)sums + (u * ND + t) * 32 + lane;
+                                float4 y = folds ? *mem : make_float4(0.f, 0.f, 0.f, 0.f);
+                                y.x = y.x * a[2 * u] + acc[u][t][0], y.y = y.y * a[2 * u + 1] + acc[u][t][1];
+                                y.z = y.z * a[2 * u] + acc[u][t][2], y.w = y.w * a[2 * u + 1] + acc[u][t][3];
+                                *mem = y;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[u][t][i] = 0.f;
+                        }
                     ++folds;
                 }
                 ++cc.j;
@@ -870,7 +847,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             cc.until = parts.end(s.w);
             cc.row_at = seqs.pre[s.x] * n_rows + s.y * (seqs.pre[s.x + 1] - seqs.pre[s.x]);
             enter_row(cc, seqs, p, s.z);
-            if (kKeep) fetch_queries(cc);
+            if (DP <= 128) fetch_queries(cc);
         }
         const bool whole = first_j == 0 && done.end == done.steps, none = done.len == done.lo;
         float* piece = p.pieces + (size_t)(2 * done.part + (first_j == 0)) * p.piece_floats;
@@ -878,210 +855,222 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             p.cut_row[done.part] = done.b * n_rows + done.h;
             p.cut_pieces[done.part] = (uint16_t)(parts.of(done.row_at + done.steps - 1) - done.part + 1);
         }
-        unsigned odd[R];
+        unsigned odd[2 * NT];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            l[r] += l_sum[r];
-            l[r] += __shfl_xor_sync(~0u, l[r], 1);
-            l[r] += __shfl_xor_sync(~0u, l[r], 2);
-            if (row_bad) l[r] = __int_as_float(0x7fc00000);
-            const int row = g + 8 * r;
-            bool fine = is_finite(l[r]);
-            if (row < heads) {
-                const size_t at = (size_t)done.b * p.n_q + first_head + row;
-                const float inv = none ? 0.f : 1.f / l[r];
-                const float a = !kKeep && folds ? exp2_fast(sums[row * 4 + quad] - m[r]) : 0.f;
-                Act* dst = (Act*)p.out + at * p.dim;
+        for (int u = 0; u < NT; ++u) {
+            float a[2], inv[2], check[2];
 #pragma unroll
-                for (int t = 0; t < DP / 8; ++t) {
-                    float x[2];
+            for (int i = 0; i < 2; ++i) {
+                const int x = 2 * u + i, head = 8 * u + 2 * quad + i;
+                l[x] += l_sum[x];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[i] = HALF ? acc[t][i] + acc[t][2 + i] : acc[t][2 * r + i];
-                        if constexpr (kKeep) x[i] += o[t][2 * r + i];
-                    }
-                    if (!kKeep && folds) {
-                        const float2 y = *(const float2*)(sums + 64 + row * DP + t * 8 + 2 * quad);
-                        x[0] += y.x * a, x[1] += y.y * a;
-                    }
-                    fine &= is_finite(x[0]) && is_finite(x[1]);
-                    if (whole) {
-                        if (t * 8 < p.dim) {
-                            dst[t * 8 + 2 * quad] = sb_from_float<Act>(x[0] * inv);
-                            dst[t * 8 + 2 * quad + 1] = sb_from_float<Act>(x[1] * inv);
-                        }
-                    } else {
-                        *(float2*)(piece + 32 + row * DP + t * 8 + 2 * quad) = make_float2(x[0], x[1]);
-                    }
-                }
-                if (quad == 0) {
+                for (int s = 4; s <= 16; s <<= 1) l[x] += __shfl_xor_sync(~0u, l[x], s);
+                if (row_bad) l[x] = __int_as_float(0x7fc00000);
+                a[i] = !kKeep && folds ? exp2_fast(m_fold[x] - m[x]) : 0.f;
+                inv[i] = !whole ? 1.f : none ? 0.f : 1.f / l[x];
+                check[i] = l[x] * 0.f;   // a NaN once anything infinite or NaN went in
+                if (g == 0 && head < heads) {
                     if (!whole)
-                        *(float2*)(piece + 2 * row) = make_float2(m[r], l[r]);
+                        *(float2*)(piece + 2 * head) = make_float2(m[x], l[x]);
                     else if (p.lse)
-                        p.lse[at] = none ? -INFINITY : 0.69314718055994531f * (m[r] + (log2f(l[r]) - kUp));
+                        p.lse[(size_t)done.b * p.n_q + first_head + head] =
+                            none ? -INFINITY : 0.69314718055994531f * (m[x] + (log2f(l[x]) - kUp));
                 }
             }
-            odd[r] = __ballot_sync(~0u, row < heads && !fine && !row_bad);
+            // where this lane stores: 16-bit results as pairs of columns of head g,
+            // others as it holds them
+            Act* out = (Act*)p.out + ((size_t)done.b * p.n_q + first_head + 8 * u) * p.dim;
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+                float4 x = make_float4(acc[u][t][0], acc[u][t][1], acc[u][t][2], acc[u][t][3]);
+                if constexpr (kKeep) {
+                    x.x += o[u][t][0], x.y += o[u][t][1], x.z += o[u][t][2], x.w += o[u][t][3];
+                } else if (folds) {
+                    const float4 y = ((const float4*)sums)[(u * ND + t) * 32 + lane];
+                    x.x += y.x * a[0], x.y += y.y * a[1], x.z += y.z * a[0], x.w += y.w * a[1];
+                }
+                check[0] += x.x * 0.f, check[1] += x.y * 0.f, check[0] += x.z * 0.f, check[1] += x.w * 0.f;
+                if (!whole) {
+                    if (8 * u + 2 * quad < heads) ((float4*)(piece + kPieceHead))[(u * ND + t) * 32 + lane] = x;
+                    continue;
+                }
+                x.x *= inv[0], x.y *= inv[1], x.z *= inv[0], x.w *= inv[1];
+                if (none) x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if constexpr (QP == 1) {
+                    uint32_t lo = take_part<Cache>(x.x, x.y), hi = take_part<Cache>(x.z, x.w);
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(lo));
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(hi));
+                    uint32_t* dst = (uint32_t*)(out + (size_t)g * p.dim + t * 16 + 2 * quad);
+                    if (8 * u + g < heads && t * 16 < p.dim) dst[0] = lo;
+                    if (8 * u + g < heads && t * 16 + 8 < p.dim) dst[4] = hi;
+                } else {
+                    float* dst = (float*)out + (size_t)2 * quad * p.dim + t * 16 + g;
+                    const bool even = 8 * u + 2 * quad < heads, next = 8 * u + 2 * quad + 1 < heads;
+                    if (t * 16 < p.dim) {
+                        if (even) dst[0] = x.x;
+                        if (next) dst[p.dim] = x.y;
+                    }
+                    if (t * 16 + 8 < p.dim) {
+                        if (even) dst[8] = x.z;
+                        if (next) dst[p.dim + 8] = x.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                odd[2 * u + i] = __ballot_sync(~0u, 8 * u + 2 * quad + i < heads && check[i] != 0.f && !row_bad && !none);
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            while (odd[r]) {
-                const int src = __ffs(odd[r]) - 1, row = src / 4 + 8 * r;
-                odd[r] &= ~(0xfu << (src & ~3));
-                const float mr = __shfl_sync(~0u, m[r], src), lr = __shfl_sync(~0u, l[r], src);
+        for (int x = 0; x < 2 * NT; ++x)
+            while (odd[x]) {
+                const int src = __ffs(odd[x]) - 1, row = x / 2 * 8 + src % 4 * 2 + x % 2;
+                odd[x] &= ~(0x11111111u << src % 4);
+                const float mr = __shfl_sync(~0u, m[x], src), lr = __shfl_sync(~0u, l[x], src);
                 __syncwarp();
                 const int base = done.lo / kStep;
                 redo_row<Cache, Act>(p, done.b, kv, first_head + row, max(done.lo, (base + first_j) * kStep),
-                                     min(done.len, (base + done.end) * kStep), mr, lr, kUp, whole, piece + 2 * row,
-                                     piece + 32 + row * DP, lane);
+                                     min(done.len, (base + done.end) * kStep), mr, lr, kUp, whole, piece, row, DP, lane);
             }
-        if (!kKeep && live) fetch_queries(cc);
+        if (DP > 128 && live) fetch_queries(cc);
     }
 }
 
 // ------------------------------------------------------------ the join
 // Pieces of a cut row, in the order of the keys: weights from their m and l,
-// then the weighted sum of their rows. A unit is a query head of a cut row and
-// 32 of its columns, one per lane. Latency is all there is to it, so a unit is
-// joined by one warp where its row has at most 32 pieces and by the eight warps
-// of a CTA where it has more, with the pieces' loads in flight together.
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kFew = 32;
-constexpr int kBatch = 16;   // pieces whose loads are in flight together
+// then the weighted sum. A unit is 8 query heads of a cut row and 16 of its
+// columns, as a lane holds them in a piece. Latency is all there is to it, so a
+// unit is joined by one warp where its row has few pieces and by the 32 warps of
+// a CTA where it has more, with kBatch pieces' loads in flight together.
+constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32, kFew = 16, kBatch = 4;
 
-template <class Act, int DP>
-__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, float up) {
-    constexpr int kSlices = DP / 32;
-    __shared__ uint16_t few[kMaxParts], many[kMaxParts];   // the parts that begin a cut row
+// The weighted sum of pieces first, first + every, .. below n, in this lane's
+// (column, head) places, with its heads' reference and sum.
+struct Joined {
+    float top[2], l[2];
+    float4 x;
+};
+__device__ inline void join_add(Joined& j, const float4 ml, const float4 x) {   // ml: (m, l) of both heads
+    const float m[2] = {ml.x, ml.z}, l[2] = {ml.y, ml.w};
+    float old[2], f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float t = fmaxf(j.top[i], m[i]), base = t == -INFINITY ? 0.f : t;
+        old[i] = exp2_fast(j.top[i] - base), f[i] = exp2_fast(m[i] - base);
+        j.top[i] = t;
+        j.l[i] = j.l[i] * old[i] + l[i] * f[i];
+    }
+    j.x.x = j.x.x * old[0] + x.x * f[0], j.x.y = j.x.y * old[1] + x.y * f[1];
+    j.x.z = j.x.z * old[0] + x.z * f[0], j.x.w = j.x.w * old[1] + x.w * f[1];
+}
+__device__ inline Joined join_pieces(const float* base, int piece_floats, int part, int n, int first, int every, int heads_at,
+                                     int unit_at, bool real) {
+    Joined j{{-INFINITY, -INFINITY}, {0.f, 0.f}, make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int k0 = first; k0 < n; k0 += every * kBatch) {
+        float4 ml[kBatch], x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = k0 + i * every;
+            ml[i] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n && real) {
+                const float* src = base + (size_t)(2 * (part + k) + (k == 0)) * piece_floats;
+                ml[i] = *(const float4*)(src + heads_at);
+                x[i] = *(const float4*)(src + unit_at);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (k0 + i * every < n) join_add(j, ml[i], x[i]);
+    }
+    return j;
+}
+
+template <class Act>
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, int dp, float up) {
+    __shared__ uint16_t list[kMaxParts];   // the parts that begin a cut row: few pieces from the front, many from the end
     __shared__ int counts[2][kJoinWarps];
-    __shared__ float red[2][kJoinWarps], sums[kJoinWarps][32];
+    __shared__ Joined sums[kJoinWarps][32];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0) p.head->ready = 0;   // for a next call of the same number (a graph's)
 
-    // ---- the cut rows, in the order of the parts that begin them
-    int n_few = 0, n_many = 0;
+    // ---- the cut rows, in the order of the parts that begin them: 8 parts per thread
+    static_assert(kMaxParts <= kJoinThreads * 8, "one pass");
+    const int first = threadIdx.x * 8;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (first < p.max_parts) raw = *(const uint4*)(p.cut_pieces + first);   // the array is padded to 8
     const int n_parts = p.head->n_parts;
-    for (int base = 0; base < n_parts; base += kJoinThreads * 8) {   // 8 parts per thread
-        const int at = base + threadIdx.x * 8;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (at < n_parts) raw = *(const uint4*)(p.cut_pieces + at);   // the array is padded to 8
-        uint16_t n[8];
-        memcpy(n, &raw, 16);
-        int f = 0, y = 0;
+    uint16_t n[8];
+    memcpy(n, &raw, 16);
+    int f = 0, y = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (at + i >= n_parts) n[i] = 0;
-            f += n[i] > 0 && n[i] <= kFew, y += n[i] > kFew;
-        }
-        int before = f | y << 16;   // of both, in the lanes before and this one
+    for (int i = 0; i < 8; ++i) {
+        if (first + i >= n_parts) n[i] = 0;
+        f += n[i] > 0 && n[i] <= kFew, y += n[i] > kFew;
+    }
+    int before = f | y << 16;   // of both, in the lanes before and this one
 #pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int x = __shfl_up_sync(~0u, before, s);
-            if (lane >= s) before += x;
-        }
-        __syncthreads();
-        if (lane == 31) counts[0][wid] = before & 0xffff, counts[1][wid] = before >> 16;
-        __syncthreads();
-        int at_few = n_few + (before & 0xffff) - f, at_many = n_many + (before >> 16) - y;
-        for (int i = 0; i < kJoinWarps; ++i) {
-            if (i < wid) at_few += counts[0][i], at_many += counts[1][i];
-            n_few += counts[0][i], n_many += counts[1][i];
-        }
+    for (int s = 1; s < 32; s <<= 1) {
+        const int x = __shfl_up_sync(~0u, before, s);
+        if (lane >= s) before += x;
+    }
+    if (lane == 31) counts[0][wid] = before & 0xffff, counts[1][wid] = before >> 16;
+    __syncthreads();
+    const int cf = counts[0][lane], cy = counts[1][lane];
+    const int n_few = __reduce_add_sync(~0u, cf), n_many = __reduce_add_sync(~0u, cy);
+    int at_few = __reduce_add_sync(~0u, lane < wid ? cf : 0) + (before & 0xffff) - f;
+    int at_many = __reduce_add_sync(~0u, lane < wid ? cy : 0) + (before >> 16) - y;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (n[i] > 0 && n[i] <= kFew) few[at_few++] = (uint16_t)(at + i);
-            if (n[i] > kFew) many[at_many++] = (uint16_t)(at + i);
-        }
+    for (int i = 0; i < 8; ++i) {
+        if (n[i] > 0 && n[i] <= kFew) list[at_few++] = (uint16_t)(first + i);
+        if (n[i] > kFew) list[kMaxParts - 1 - at_many++] = (uint16_t)(first + i);
     }
     __syncthreads();
-    const int n_rows = p.n_kv * p.tiles, units = p.piece_rows * kSlices;
-    auto place = [&](int row, int head, bool& real) -> size_t {   // of the output row
-        const int b = row / n_rows, h = row % n_rows, tile = h % p.tiles;
-        real = head < min(16, p.group - tile * 16);
-        return (size_t)b * p.n_q + h / p.tiles * p.group + tile * 16 + head;
-    };
-    auto piece = [&](int w, int k) { return p.pieces + (size_t)(2 * (w + k) + (k == 0)) * p.piece_floats; };
-    auto finish = [&](size_t at, int col, float a, float top, float l) {
-        if (col < p.dim) ((Act*)p.out)[at * p.dim + col] = sb_from_float<Act>(a / l);
-        if (p.lse && col == 0) p.lse[at] = 0.69314718055994531f * (top + (log2f(l) - up));
+
+    const int n_rows = p.n_kv * p.tiles, tiles_d = dp / 16, units = (p.piece_rows + 7) / 8 * tiles_d;
+    const int g = lane >> 2, quad = lane & 3;
+    auto finish = [&](int row, int unit, const Joined& j) {
+        const int b = row / n_rows, h = row % n_rows, tile = h % p.tiles, heads = min(16, p.group - tile * 16);
+        const int t = unit % tiles_d;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int head = unit / tiles_d * 8 + 2 * quad + i;
+            if (head >= heads) continue;
+            const size_t at = (size_t)b * p.n_q + h / p.tiles * p.group + tile * 16 + head;
+            Act* dst = (Act*)p.out + at * p.dim + t * 16 + g;
+            if (t * 16 < p.dim) dst[0] = sb_from_float<Act>((i ? j.x.y : j.x.x) / j.l[i]);
+            if (t * 16 + 8 < p.dim) dst[8] = sb_from_float<Act>((i ? j.x.w : j.x.z) / j.l[i]);
+            if (p.lse && t == 0 && g == 0) p.lse[at] = 0.69314718055994531f * (j.top[i] + (log2f(j.l[i]) - up));
+        }
     };
 
     // ---- rows of more than kFew pieces
     for (int u = blockIdx.x; u < n_many * units; u += gridDim.x) {
-        const int w = many[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
-        const int row = p.cut_row[w], n = p.cut_pieces[w];
-        bool real;
-        const size_t at = place(row, head, real);
-        if (!real) continue;
-        // this warp's pieces: wid, wid + 8, ..; 32 at a time, one per lane
-        float top = -INFINITY, l = 0.f, a = 0.f;
-        for (int k0 = wid; k0 < n; k0 += kJoinThreads) {
-            const int k = k0 + lane * kJoinWarps;
-            const float2 ml = k < n ? *(const float2*)(piece(w, k) + 2 * head) : make_float2(-INFINITY, 0.f);
-            float t = fmaxf(top, ml.x);
-#pragma unroll
-            for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, s));
-            const float base = t == -INFINITY ? 0.f : t, old = exp2_fast(top - base), f = exp2_fast(ml.x - base);
-            top = t;
-            l = l * old + f * ml.y;   // of this lane's pieces
-            a *= old;
-            const float* src = piece(w, 1) - p.piece_floats * 2 + 32 + head * DP + col;   // piece k of the others
-            const int here = min(32, (n - k0 + kJoinWarps - 1) / kJoinWarps);
-            for (int i0 = 0; i0 < here; i0 += kBatch) {
-                float x[kBatch];
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const int k = k0 + (i0 + i) * kJoinWarps;
-                    x[i] = k < n ? src[(size_t)k * 2 * p.piece_floats + (k == 0 ? p.piece_floats : 0)] : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) a += __shfl_sync(~0u, f, i0 + i) * x[i];
-            }
-        }
-#pragma unroll
-        for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
-        if (lane == 0) red[0][wid] = top, red[1][wid] = l;
-        sums[wid][lane] = a;
+        const int part = list[kMaxParts - 1 - u / units], unit = u % units;
+        const int pieces = p.cut_pieces[part], row = p.cut_row[part];
+        const bool real = unit / tiles_d * 8 + 2 * quad < p.piece_rows;
+        sums[wid][lane] = join_pieces(p.pieces, p.piece_floats, part, pieces, wid, kJoinWarps,
+                                      2 * (unit / tiles_d * 8 + 2 * quad), kPieceHead + (unit * 32 + lane) * 4, real);
         __syncthreads();
         if (wid == 0) {
-            top = red[0][0];
-            for (int i = 1; i < kJoinWarps; ++i) top = fmaxf(top, red[0][i]);
-            const float base = top == -INFINITY ? 0.f : top;
-            a = l = 0.f;
-            for (int i = 0; i < kJoinWarps; ++i) {
-                const float f = exp2_fast(red[0][i] - base);
-                l += f * red[1][i];
-                a += f * sums[i][lane];
+            Joined j = sums[0][lane];
+            for (int i = 1; i < kJoinWarps; ++i) {
+                const Joined& k = sums[i][lane];
+                join_add(j, make_float4(k.top[0], k.l[0], k.top[1], k.l[1]), k.x);
             }
-            finish(at, col, a, top, l);
+            finish(row, unit, j);
         }
         __syncthreads();
     }
 
     // ---- the others
     for (int u = blockIdx.x * kJoinWarps + wid; u < n_few * units; u += gridDim.x * kJoinWarps) {
-        const int w = few[u / units], head = u / kSlices % p.piece_rows, col = u % kSlices * 32 + lane;
-        const int row = p.cut_row[w], n = p.cut_pieces[w];
-        bool real;
-        const size_t at = place(row, head, real);
-        if (!real) continue;
-        const float2 ml = lane < n ? *(const float2*)(piece(w, lane) + 2 * head) : make_float2(-INFINITY, 0.f);
-        float top = ml.x;
-#pragma unroll
-        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-        const float f = exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
-        float l = lane < n ? f * ml.y : 0.f, a = 0.f;
-#pragma unroll
-        for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
-        for (int k0 = 0; k0 < n; k0 += kBatch) {
-            float x[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) x[i] = k0 + i < n ? piece(w, k0 + i)[32 + head * DP + col] : 0.f;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) a += __shfl_sync(~0u, f, k0 + i) * x[i];
-        }
-        finish(at, col, a, top, l);
+        const int part = list[u / units], unit = u % units;
+        const int pieces = p.cut_pieces[part], row = p.cut_row[part];
+        const bool real = unit / tiles_d * 8 + 2 * quad < p.piece_rows;
+        finish(row, unit, join_pieces(p.pieces, p.piece_floats, part, pieces, 0, 1,
+                                      2 * (unit / tiles_d * 8 + 2 * quad), kPieceHead + (unit * 32 + lane) * 4, real));
     }
 }
 
@@ -1099,12 +1088,13 @@ int sm_count() {
 }
 int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 int most_warps(int dim) { return dim <= 128 ? 8 : dim <= 192 ? 5 : 4; }   // Shape<>::kWarps
-int piece_floats(int group, int dim) { return 64 + std::min(group, 16) * tile_width(dim); }
+int piece_floats(int group, int dim) { return kPieceHead + (group <= 8 ? 8 : 16) * tile_width(dim); }
 // The workspace: the header, the parts' cut rows, their pieces, the warps' sums.
 struct Layout {
-    size_t cut_pieces, cut_row, pieces, sums, bytes;
+    size_t parts, cut_pieces, cut_row, pieces, sums, bytes;
     Layout(int group, int dim) {
-        const size_t warps = (size_t)sm_count() * most_warps(dim), parts = (3 * warps + 7) / 8 * 8;
+        const size_t warps = (size_t)sm_count() * most_warps(dim);
+        parts = (3 * warps + 7) / 8 * 8;
         const size_t piece = piece_floats(group, dim) * sizeof(float);
         cut_pieces = 256;
         cut_row = cut_pieces + parts * sizeof(uint16_t);
@@ -1145,19 +1135,19 @@ bool cache_map(CUtensorMap* map, const void* base, int type, const AttendParams&
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class Cache, int DP, int QP, bool HALF>
+template <class Cache, int DP, int QP, int NT>
 int launch(AttendParams p, cudaStream_t st) {
     using S = Shape<DP>;
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
     constexpr bool kF16 = std::is_same<Cache, __half>::value;
-    const int q_rows = HALF ? 0 : std::min(p.group, 16) * QP;
+    const int q_rows = NT == 1 ? 0 : std::min(p.group, 16) * QP;
     const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16) + kQueue * sizeof(int4);
-    const size_t seqs = 12 * (size_t)p.n_seqs + 8;
-    // static shared memory (the scan's warp sums) is 256 bytes
+    const size_t seqs = 8 * (size_t)p.n_seqs + 4;
+    // static shared memory (the scan's warp sums) is 128 bytes
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
     static bool opted = false;
     if (!opted) {
-        if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              kSmemLimit - 1024), "attend shared memory"))
             return -1;
         opted = true;
@@ -1189,30 +1179,30 @@ int launch(AttendParams p, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, HALF>, (const AttendParams)p, (const CUtensorMap)kmap,
+    if (!sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend<Cache, DP, QP, NT>, (const AttendParams)p, (const CUtensorMap)kmap,
                                        (const CUtensorMap)vmap), "attend launch"))
         return -1;
     if (!cuts) return 0;
-    cfg.gridDim = 2 * sm_count();
+    cfg.gridDim = sm_count();
     cfg.blockDim = kJoinThreads;
     cfg.dynamicSmemBytes = 0;
-    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act, DP>, (const AttendParams)p, up_of(kF16)), "attend join launch")
+    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act>, (const AttendParams)p, DP, up_of(kF16)), "attend join launch")
                ? 0 : -1;
 }
 
-template <class Cache, int QP, bool HALF>
+template <class Cache, int QP, int NT>
 int launch_dim(const AttendParams& p, cudaStream_t st) {
     switch (tile_width(p.dim)) {
-    case 64: return launch<Cache, 64, QP, HALF>(p, st);
-    case 96: return launch<Cache, 96, QP, HALF>(p, st);
-    case 128: return launch<Cache, 128, QP, HALF>(p, st);
-    case 192: return launch<Cache, 192, QP, HALF>(p, st);
-    default: return launch<Cache, 256, QP, HALF>(p, st);
+    case 64: return launch<Cache, 64, QP, NT>(p, st);
+    case 96: return launch<Cache, 96, QP, NT>(p, st);
+    case 128: return launch<Cache, 128, QP, NT>(p, st);
+    case 192: return launch<Cache, 192, QP, NT>(p, st);
+    default: return launch<Cache, 256, QP, NT>(p, st);
     }
 }
 template <class Cache, int QP>
 int launch_group(const AttendParams& p, cudaStream_t st) {
-    return p.group <= 8 ? launch_dim<Cache, QP, true>(p, st) : launch_dim<Cache, QP, false>(p, st);
+    return p.group <= 8 ? launch_dim<Cache, QP, 1>(p, st) : launch_dim<Cache, QP, 2>(p, st);
 }
 
 }  // namespace
@@ -1249,7 +1239,7 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     }
     if (n_seqs == 0) return 0;
     if (!d_q || !d_lens || !d_out || (table_width && (!d_k_cache || !d_v_cache || !d_block_table)) ||
-        ((uintptr_t)d_q | q_seq_stride | q_head_stride | (uintptr_t)d_out) % ab ||
+        ((uintptr_t)d_q | q_seq_stride | q_head_stride) % ab || (uintptr_t)d_out % 4 ||
         ((uintptr_t)d_k_cache | (uintptr_t)d_v_cache | k_page_stride | k_slot_stride | k_head_stride | v_page_stride |
          v_slot_stride | v_head_stride) % 16 ||
         ((uintptr_t)d_block_table | (uintptr_t)d_lens | (uintptr_t)d_lse | table_stride) % 4) {
@@ -1281,15 +1271,24 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     const Layout lay(p.group, head_dim);
     uint8_t* ws = (uint8_t*)d_workspace;
     p.head = (Header*)ws;
+    p.max_parts = (int)lay.parts;
     p.cut_pieces = (uint16_t*)(ws + lay.cut_pieces);
     p.cut_row = (int*)(ws + lay.cut_row);
     p.pieces = (float*)(ws + lay.pieces);
     p.sums = (float*)(ws + lay.sums);
     const int slot = sb_timing_begin("attend_paged", st);
     int rc = 0;
-    for (int b = 0; b < n_seqs && rc == 0; b += kMaxSeqs) {
+    // the list of a launch has fewer than 2^31 places
+    const long long most = (long long)n_kv_heads * p.tiles * ((long long)table_width * page_size / kStep + 2 + kRowCost);
+    if (most > 0x7fffffffll) {
+        sb_set_error("attend: %d pages of %d per sequence are too many for %d key-value heads", table_width, page_size,
+                     n_kv_heads);
+        return -1;
+    }
+    const int per_launch = (int)std::min<long long>(kMaxSeqs, 0x7fffffffll / most);
+    for (int b = 0; b < n_seqs && rc == 0; b += per_launch) {
         AttendParams a = p;
-        a.n_seqs = std::min(kMaxSeqs, n_seqs - b);
+        a.n_seqs = std::min(per_launch, n_seqs - b);
         a.q += (size_t)b * q_seq_stride;
         a.table += (size_t)b * p.table_stride;
         a.lens += b;
