@@ -117,10 +117,18 @@ __device__ inline bool bar_wait(uint32_t bar, uint32_t parity) {
     }
     return false;
 }
-__device__ inline void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int slot, int head, int page) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
-                 "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(slot), "r"(head), "r"(page)
-                 : "memory");
+// The rows pass through L2 once: they are the first to go there, so that the
+// pieces, the tables and the queries stay.
+__device__ inline unsigned long long pass_through() {
+    unsigned long long policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ inline void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int slot, int head, int page,
+                                 unsigned long long policy) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+                 "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(slot), "r"(head),
+                 "r"(page), "l"(policy) : "memory");
 }
 __device__ inline void ldsm4(uint32_t* r, uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -285,6 +293,7 @@ struct Loader {
     const Parts& parts;
     const int lane;
     const uint32_t ring, bars;
+    const unsigned long long policy;
     int4* queue;
     Cursor c;
     bool more = true, asked = false, values = false;   // values: the next slot is the step's values
@@ -295,7 +304,7 @@ struct Loader {
 
     __device__ Loader(const AttendParams& p_, const CUtensorMap* km, const CUtensorMap* vm, const Seqs& s_, const Parts& parts_,
                       int lane_, uint32_t ring_, uint32_t bars_, int4* queue_, const Cursor& c_)
-        : p(p_), kmap(km), vmap(vm), seqs(s_), parts(parts_), lane(lane_), ring(ring_), bars(bars_), queue(queue_), c(c_) {
+        : p(p_), kmap(km), vmap(vm), seqs(s_), parts(parts_), lane(lane_), ring(ring_), bars(bars_), policy(pass_through()), queue(queue_), c(c_) {
         begin_part();
     }
     __device__ int entry_of(int key) const {
@@ -404,7 +413,7 @@ struct Loader {
             const CUtensorMap* map = values ? vmap : kmap;
             const int kv = p.tiles == 1 ? c.h : c.h / p.tiles;
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) tile_load(dst + t * S::kTileBytes, map, bar, 64 * t, row, kv, page);
+            for (int t = 0; t < S::kTiles; ++t) tile_load(dst + t * S::kTileBytes, map, bar, 64 * t, row, kv, page, policy);
         }
         if (values) advance();
         values = !values;
@@ -700,26 +709,41 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             if (!(n & 1)) {
                 row_bad |= (loader.bad >> slot) & 1;
                 // ---- scores of 32 keys and the tile's heads
-                float c[2][NT][4] = {};
+                // fragments are read a block ahead of the MMAs, which then find
+                // their factors ready and as many sums apart as hide their latency
+                float ch[2][2][NT][4] = {};   // two chains over the dimensions
+                uint32_t kf[2][2][2][4];      // [buffer][16 dimensions][16 keys]
+                auto load_keys = [&](int d) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    uint32_t kf[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        ldsm4(kf[h], ((at + k_lane) ^ ((d & 3) << 5)) + (d >> 2) * S::kTileBytes + h * 2048);
-#pragma unroll
-                    for (int s = 0; s < QP; ++s) {
-                        uint32_t qb[4];
-                        if constexpr (NT == 1)
-                            qb[0] = qf[d][s], qb[1] = qf[d][QP + s];
-                        else
-                            ldsm4(qb, q_lane + s * rows * kQRow + d * 32);
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
+                            ldsm4(kf[d / 2 & 1][i][h], ((at + k_lane) ^ (((d + i) & 3) << 5)) + ((d + i) >> 2) * S::kTileBytes + h * 2048);
+                };
+                load_keys(0);
 #pragma unroll
-                            for (int u = 0; u < NT; ++u) mma16816<Cache>(c[h][u], kf[h], qb[2 * u], qb[2 * u + 1]);
+                for (int d = 0; d < ND; d += 2) {
+                    if (d + 2 < ND) load_keys(d + 2);
+#pragma unroll
+                    for (int s = 0; s < QP; ++s) {
+                        uint32_t qb[2][4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if constexpr (NT == 1)
+                                qb[i][0] = qf[d + i][s], qb[i][1] = qf[d + i][QP + s];
+                            else
+                                ldsm4(qb[i], q_lane + s * rows * kQRow + (d + i) * 32);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int u = 0; u < NT; ++u)
+                                    mma16816<Cache>(ch[i][h][u], kf[d / 2 & 1][i][h], qb[i][2 * u], qb[i][2 * u + 1]);
                     }
                 }
+                float (&c)[2][NT][4] = ch[0];
 
                 // ---- the running softmax
                 bool move = false;
@@ -730,7 +754,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float& s = c[h][u][i];
-                            s *= unscale[2 * u + i % 2];
+                            s = (s + ch[1][h][u][i]) * unscale[2 * u + i % 2];
                             if (edge) {
                                 const int key = key0 + 16 * h + g + i / 2 * 8;
                                 if (key < cc.lo || key >= cc.len) s = -INFINITY;
@@ -786,17 +810,28 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                     __syncwarp();
                 }
                 // ---- values, transposed, times weights
+                constexpr int kAhead = ND % 4 == 0 ? 4 : 2;   // tiles of 16 columns per block
+                uint32_t vf[2][kAhead][4];
+                auto load_values = [&](int blk) {   // blocks of the first 16 keys, then of the others
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int t = 0; t < ND; ++t) {
-                        uint32_t vf[4];
-                        ldsm4t(vf, ((at + v_lane) ^ ((t & 3) << 5)) + (t >> 2) * S::kTileBytes + h * 2048);
-#pragma unroll
-                        for (int u = 0; u < NT; ++u)
-#pragma unroll
-                            for (int s = 0; s < PP; ++s) mma16816<Cache>(acc[u][t], vf, wf[h][u][s][0], wf[h][u][s][1]);
+                    for (int i = 0; i < kAhead; ++i) {
+                        const int t = blk * kAhead % ND + i, h = blk * kAhead / ND;
+                        ldsm4t(vf[blk & 1][i], ((at + v_lane) ^ ((t & 3) << 5)) + (t >> 2) * S::kTileBytes + h * 2048);
                     }
+                };
+                load_values(0);
+#pragma unroll
+                for (int blk = 0; blk < 2 * ND / kAhead; ++blk) {
+                    if (blk + 1 < 2 * ND / kAhead) load_values(blk + 1);
+                    const int h = blk * kAhead / ND;
+#pragma unroll
+                    for (int s = 0; s < PP; ++s)
+#pragma unroll
+                        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                            for (int u = 0; u < NT; ++u)
+                                mma16816<Cache>(acc[u][blk * kAhead % ND + i], vf[blk & 1][i], wf[h][u][s][0], wf[h][u][s][1]);
+                }
 
                 // ---- the MMA's sums to the rounded ones
                 if (--fold == 0) {
@@ -941,7 +976,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 // columns, as a lane holds them in a piece. Latency is all there is to it, so a
 // unit is joined by one warp where its row has few pieces and by the 32 warps of
 // a CTA where it has more, with kBatch pieces' loads in flight together.
-constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32, kFew = 16, kBatch = 4;
+constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32, kFew = 32, kBatch = 4;
 
 // The weighted sum of pieces first, first + every, .. below n, in this lane's
 // (column, head) places, with its heads' reference and sum.
