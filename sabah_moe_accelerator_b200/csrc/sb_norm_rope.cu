@@ -28,7 +28,7 @@ struct NormRopeParams {
     size_t q_token, q_head, k_token, k_head, v_token, v_head;   // bytes
     int n_q, n_kv, n_tokens, dim;
     const float *q_weight, *k_weight;
-    float eps;
+    float eps, over_dim;
     const float2* table;
     int n_positions, rope, pairs_mode;
     const int32_t* positions;
@@ -44,10 +44,6 @@ struct NormRopeParams {
     int rows, blocks;   // rows of a token; warp tasks of a token
 };
 
-template <class T, int W>
-struct Chunk {
-    T v[W];
-};
 template <class T, int W>
 __device__ inline void load_chunk(const T* p, float* f) {
     if constexpr (W == 4 && sizeof(T) == 4) {
@@ -79,56 +75,29 @@ __device__ inline void store_chunk(T* p, const float* f) {
 
 // LPR lanes per row, NP chunk pairs of W values per lane, ITER rows per lane group
 template <class Act, class Cache, int W, int LPR, int NP, int ITER>
-__global__ void __launch_bounds__(kWarps * 32) k_norm_rope(NormRopeParams p) {
+__global__ void __launch_bounds__(kWarps * 32) k_norm_rope(const __grid_constant__ NormRopeParams p) {
     constexpr int kRows = 32 / LPR;
-    const long long task = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const unsigned task = blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR;
-    const int t = (int)(task / p.blocks);
+    const int t = (int)(task / (unsigned)p.blocks);
     if (t >= p.n_tokens) return;
-    const int row0 = (int)(task % p.blocks) * kRows * ITER + grp;
+    const int row0 = (int)(task - (unsigned)t * (unsigned)p.blocks) * kRows * ITER + grp;
     const int half = p.rope / 2;
 
-    // where this lane's chunk pairs lie in a row, and their cosines
+    // where this lane's chunk pairs lie in a row
     int at[NP][2];
-    float c[NP][W], s[NP][W];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
         const int cp = sub + n * LPR;
-        const bool turned = cp * 2 * W < p.rope;
-        at[n][0] = p.pairs_mode || !turned ? cp * 2 * W : cp * W;
-        at[n][1] = p.pairs_mode || !turned ? cp * 2 * W + W : cp * W + half;
-        if (cp * 2 * W >= p.dim) at[n][0] = -1;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            c[n][i] = 1.f;
-            s[n][i] = 0.f;
-            if (!turned) continue;
-            const int pair = cp * W + i;
-            const int axis = p.pair_axis ? p.pair_axis[pair] : 0;
-            const int pos = axis < p.n_axes ? p.positions[(size_t)axis * p.n_tokens + t] : -1;
-            if (pos < 0 || pos >= p.n_positions) {
-                c[n][i] = s[n][i] = __int_as_float(0x7fc00000);
-                atomicExch(p.err, SB_DERR_BAD_INDEX);
-            } else {
-                const float2 cs = __ldg(p.table + (size_t)pos * half + pair);
-                c[n][i] = cs.x;
-                s[n][i] = cs.y;
-            }
-        }
+        const bool split = !p.pairs_mode && cp * 2 * W < p.rope;
+        at[n][0] = cp * 2 * W >= p.dim ? -1 : split ? cp * W : cp * 2 * W;
+        at[n][1] = split ? cp * W + half : cp * 2 * W + W;
     }
-    long long slot = p.slots ? p.slots[t] : -1;
-    if (slot >= (long long)p.n_slots) {
-        if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
-        slot = -1;
-    }
-    const unsigned page = slot < 0 ? 0 : (unsigned)slot / p.page_size;
-    const unsigned in_page = slot < 0 ? 0 : (unsigned)slot % p.page_size;
-
+    // all of the task's rows are on their way before anything waits
     float x[ITER][NP][2][W];
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
         const int r = row0 + it * kRows;
-        if (r >= p.rows) continue;
         const uint8_t* src = r < p.n_q            ? p.q + (size_t)t * p.q_token + (size_t)r * p.q_head
                              : r < p.n_q + p.n_kv ? p.k + (size_t)t * p.k_token + (size_t)(r - p.n_q) * p.k_head
                                                   : p.v + (size_t)t * p.v_token + (size_t)(r - p.n_q - p.n_kv) * p.v_head;
@@ -136,13 +105,63 @@ __global__ void __launch_bounds__(kWarps * 32) k_norm_rope(NormRopeParams p) {
         for (int n = 0; n < NP; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (at[n][0] >= 0)
+                if (r < p.rows && at[n][0] >= 0)
                     load_chunk<Act, W>((const Act*)src + at[n][h], x[it][n][h]);
                 else
 #pragma unroll
                     for (int i = 0; i < W; ++i) x[it][n][h][i] = 0.f;
             }
     }
+    long long slot = p.slots ? p.slots[t] : -1;
+    // the cosines of this lane's pairs, once for all of its rows
+    float c[NP][W], s[NP][W];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int pair0 = (sub + n * LPR) * W;
+        const bool turned = pair0 * 2 < p.rope;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            c[n][i] = 1.f;
+            s[n][i] = 0.f;
+        }
+        if (!turned) continue;
+        if (p.pair_axis == nullptr) {
+            const int pos = p.positions[t];
+            const bool out = pos < 0 || pos >= p.n_positions;
+            if (out) atomicExch(p.err, SB_DERR_BAD_INDEX);
+            float cs[2 * W];
+            const float* src = (const float*)(p.table + (size_t)(out ? 0 : pos) * half + pair0);
+            if constexpr (W == 4) {
+                load_chunk<float, W>(src, cs);
+                load_chunk<float, W>(src + W, cs + W);
+            } else {
+                cs[0] = __ldg(src), cs[1] = __ldg(src + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                c[n][i] = out ? __int_as_float(0x7fc00000) : cs[2 * i];
+                s[n][i] = out ? __int_as_float(0x7fc00000) : cs[2 * i + 1];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int axis = p.pair_axis[pair0 + i];
+                const int pos = axis < p.n_axes ? p.positions[(size_t)axis * p.n_tokens + t] : -1;
+                const bool out = pos < 0 || pos >= p.n_positions;
+                if (out) atomicExch(p.err, SB_DERR_BAD_INDEX);
+                const float2 cs = __ldg(p.table + (size_t)(out ? 0 : pos) * half + pair0 + i);
+                c[n][i] = out ? __int_as_float(0x7fc00000) : cs.x;
+                s[n][i] = out ? __int_as_float(0x7fc00000) : cs.y;
+            }
+        }
+    }
+    if (slot >= (long long)p.n_slots) {
+        if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
+        slot = -1;
+    }
+    const unsigned page = slot < 0 ? 0 : (unsigned)slot / p.page_size;
+    const unsigned in_page = slot < 0 ? 0 : (unsigned)slot - page * p.page_size;
+
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
         const int r = row0 + it * kRows;
@@ -155,11 +174,11 @@ __global__ void __launch_bounds__(kWarps * 32) k_norm_rope(NormRopeParams p) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < W; ++i) sum += here ? x[it][n][h][i] * x[it][n][h][i] : 0.f;
+                for (int i = 0; i < W; ++i) sum += x[it][n][h][i] * x[it][n][h][i];
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
         if (!here) continue;
-        const float inv = rsqrtf(sum / p.dim + p.eps);
+        const float inv = rsqrtf(sum * p.over_dim + p.eps);
         const int kv = is_v ? r - p.n_q - p.n_kv : r - p.n_q;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
@@ -220,16 +239,27 @@ void launch(NormRopeParams p, cudaStream_t st) {
     k_norm_rope<Act, Cache, W, LPR, NP, ITER><<<(unsigned)((tasks + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(p);
 }
 
+// Four rows per lane group once the rows of one would fill the chip twice over
+// (148 SMs x 64 warps): the cosines, positions and indexes are then a fourth of
+// the work, where few rows want all the warps there are.
+template <class Act, class Cache, int LPR>
+void launch_wide(const NormRopeParams& p, cudaStream_t st) {
+    if ((long long)p.n_tokens * p.rows * LPR / 32 > 2 * 148 * 64)
+        launch<Act, Cache, 4, LPR, 1, 4>(p, st);
+    else
+        launch<Act, Cache, 4, LPR, 1, 1>(p, st);
+}
+
 template <class Act, class Cache>
 void launch_shape(const NormRopeParams& p, bool wide, cudaStream_t st) {
     if (!wide)
         launch<Act, Cache, 1, 32, kMaxDim / 64, 1>(p, st);
     else if (p.dim <= 64)
-        launch<Act, Cache, 4, 8, 1, 1>(p, st);
+        launch_wide<Act, Cache, 8>(p, st);
     else if (p.dim <= 128)
-        launch<Act, Cache, 4, 16, 1, 1>(p, st);
+        launch_wide<Act, Cache, 16>(p, st);
     else
-        launch<Act, Cache, 4, 32, 1, 1>(p, st);
+        launch_wide<Act, Cache, 32>(p, st);
 }
 
 }  // namespace
@@ -267,6 +297,10 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
         return -1;
     }
     const int rows = n_q_heads + n_kv_heads * (cache ? 2 : 1);
+    if ((long long)n_tokens * rows > 0x7fffffffll) {
+        sb_set_error("norm_rope: %d tokens of %d rows are too many for one call", n_tokens, rows);
+        return -1;
+    }
     if (rows == 0) return 0;
     if ((n_q_heads && (!d_q || !d_q_out)) || (n_kv_heads && (!d_k || (!cache && !d_k_out)))) {
         sb_set_error("invalid norm_rope arguments (a null row or output pointer)");
@@ -282,7 +316,7 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
                      v_page_stride | v_slot_stride | v_cache_head_stride;
     }
     f32_bits = (uintptr_t)d_q_weight | (uintptr_t)d_k_weight;
-    if (act_bits % ab || cache_bits % 2 || f32_bits % 4 || (uintptr_t)d_table % 8 || (uintptr_t)d_positions % 4 ||
+    if (act_bits % ab || cache_bits % 2 || f32_bits % 4 || (uintptr_t)d_table % 4 || (uintptr_t)d_positions % 4 ||
         (uintptr_t)d_slots % 8) {
         sb_set_error("invalid norm_rope arguments (a pointer or stride is not a whole number of elements)");
         return -1;
@@ -293,7 +327,7 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
     p.k_token = k_token_stride, p.k_head = k_head_stride;
     p.v_token = v_token_stride, p.v_head = v_head_stride;
     p.n_q = n_q_heads, p.n_kv = n_kv_heads, p.n_tokens = n_tokens, p.dim = head_dim;
-    p.q_weight = d_q_weight, p.k_weight = d_k_weight, p.eps = eps;
+    p.q_weight = d_q_weight, p.k_weight = d_k_weight, p.eps = eps, p.over_dim = 1.f / head_dim;
     p.table = (const float2*)d_table, p.n_positions = n_positions, p.rope = rope_dim, p.pairs_mode = pairs_mode;
     p.positions = d_positions, p.pair_axis = d_pair_axis, p.n_axes = n_axes;
     p.q_out = (uint8_t*)d_q_out, p.k_out = (uint8_t*)d_k_out;
@@ -304,7 +338,7 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
     p.slots = d_slots, p.err = err, p.rows = rows;
     // four values at a time where rows, pairs and pointers allow it
     const bool wide = head_dim % 8 == 0 && rope_dim % 8 == 0 && act_bits % (4 * ab) == 0 && cache_bits % 8 == 0 &&
-                      f32_bits % 16 == 0;
+                      (f32_bits | (uintptr_t)d_table) % 16 == 0;
     const int slot = sb_timing_begin("qk_norm_rope", st);
     const bool bf = cache ? cache_type == SB_BF16 : true;
     if (act_type == SB_F32)

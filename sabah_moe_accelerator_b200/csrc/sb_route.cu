@@ -9,8 +9,15 @@
 //
 // The choice compares logits, not probabilities: exp would round neighbours
 // together. One warp holds a token's logits in registers as order-preserving
-// 32-bit keys; n_used times the warp takes the largest key (redux.sync) and,
-// among the lanes that hold it, the lowest expert.
+// 32-bit keys, read 16 bytes at a time where rows allow it.
+//
+// Bound: for many tokens the instructions that a logit costs, else latency, so
+// the choice is made without n_used rounds over all logits. The n_used-th
+// largest of the 32 lanes' largest keys is a key that at least n_used logits
+// reach, and few more do (about 13 of 512 for the 10 largest). Those are
+// gathered one per lane, and each lane counts how many beat its own: its rank.
+// Where more than 32 logits reach the bound (many equal ones), the warp takes
+// the largest n_used times instead.
 #include <cuda_bf16.h>
 
 #include "sb_act.cuh"
@@ -42,77 +49,135 @@ __device__ inline float key_value(uint32_t k) {
     return k == 1 ? __int_as_float(0x7fc00000) : __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
-// NV: logits per lane (n_experts <= 32 * NV); expert e is lane e % 32's
-template <class Act, int NV>
-__global__ void __launch_bounds__(kWarps * 32) k_route(RouteParams p) {
-    const int lane = threadIdx.x & 31, t = blockIdx.x * kWarps + (threadIdx.x >> 5);
+// NV: logits per lane (n_experts <= 32 * NV), V of them side by side
+template <class Act, int NV, int V>
+__global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ RouteParams p) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, t = blockIdx.x * kWarps + wid;
+    __shared__ uint2 picked[kWarps][32];
     if (t >= p.n_tokens) return;
     const Act* row = (const Act*)(p.x + (size_t)t * p.row_stride);
+    auto expert = [&](int i) { return (i / V * 32 + lane) * V + i % V; };
     uint32_t key[NV];
     uint32_t top = 0;
     bool nan = false;
 #pragma unroll
+    for (int c = 0; c < NV / V; ++c) {
+        struct alignas(V * sizeof(Act)) Chunk { Act x[V]; };
+        const int e = expert(c * V);
+        Chunk u;
+        if (e < p.n_experts) u = *(const Chunk*)(row + e);
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[c * V + i] = e < p.n_experts ? order_key(sb_to_float(u.x[i])) : 0;
+    }
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = e < p.n_experts ? order_key(sb_to_float(row[e])) : 0;
         nan |= key[i] == 1;
         top = max(top, key[i]);
     }
     nan = __any_sync(~0u, nan);
-    const float m = key_value(__reduce_max_sync(~0u, top));
-    float all = 0.f;
+    const uint32_t first = __reduce_max_sync(~0u, top);
+    const float m = key_value(first);
+    float total = 0.f;   // of all, where the weights are over all experts
     if (!p.renorm) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (key[i]) all += __expf(key_value(key[i]) - m);
+            if (key[i]) total += __expf(key_value(key[i]) - m);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
     }
-    float mine = 0.f, chosen = 0.f;   // lane j keeps choice j
-    int my_id = 0;
-    for (int j = 0; j < p.n_used; ++j) {
-        uint32_t best = 0;
-        int at = 0;
+
+    // a key that at least n_used logits reach, and who reaches it
+    uint32_t bound = first, left = top;
+    for (int lanes = 0;;) {
+        lanes += __popc(__ballot_sync(~0u, left == bound));
+        if (lanes >= p.n_used) break;
+        if (left == bound) left = 0;
+        const uint32_t k = __reduce_max_sync(~0u, left);
+        if (k == 0) {   // fewer lanes with logits than choices: all of them count
+            bound = 1;
+            break;
+        }
+        bound = k;
+    }
+    int n = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = i;
-            }
-        const uint32_t k = __reduce_max_sync(~0u, best);
-        const int e = __reduce_min_sync(~0u, best == k ? lane + 32 * at : 0x7fffffff);
-        if (lane == (e & 31)) {
+    for (int i = 0; i < NV; ++i) {
+        const unsigned who = __ballot_sync(~0u, key[i] >= bound);
+        const int at = n + __popc(who & ((1u << lane) - 1));
+        if (key[i] >= bound && at < 32) picked[wid][at] = make_uint2(key[i], expert(i));
+        n += __popc(who);
+    }
+    uint32_t mine = 0;   // this lane's choice: its key, expert and rank
+    int my_id = 0, rank = p.n_used;
+    if (n <= 32) {
+        __syncwarp();
+        if (lane < n) {
+            const uint2 u = picked[wid][lane];
+            mine = u.x, my_id = u.y, rank = 0;
+        }
+        for (int j = 0; j < n; ++j) {
+            const uint32_t k = __shfl_sync(~0u, mine, j);
+            const int e = __shfl_sync(~0u, my_id, j);
+            rank += k > mine || (k == mine && e < my_id);
+        }
+    } else {
+        for (int j = 0; j < p.n_used; ++j) {
+            uint32_t best = 0;
+            int at = 0;   // the lowest expert of the lane's largest keys: expert() grows with i
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (i == (e >> 5)) key[i] = 0;
+                if (key[i] > best) {
+                    best = key[i];
+                    at = expert(i);
+                }
+            const uint32_t k = __reduce_max_sync(~0u, best);
+            const int e = __reduce_min_sync(~0u, best == k ? at : 0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (expert(i) == e) key[i] = 0;
+            if (lane == j) mine = k, my_id = e, rank = j;
         }
-        const float v = expf(key_value(k) - m);
-        chosen += v;
-        if (lane == j) {
-            mine = v;
-            my_id = e;
-        }
+    }
+    const bool chosen = mine && rank < p.n_used;
+    const float v = chosen ? expf(key_value(mine) - m) : 0.f;
+    if (p.renorm) {
+        total = v;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
     }
     // a row with a NaN has NaN weights (its ids stay in range); a row whose
     // logits are all -inf chooses nothing: zero weights
-    float w = p.scale * (mine / (p.renorm ? chosen : all));
+    float w = p.scale * (v / total);
     if (m == -INFINITY) w = 0.f;
     if (nan) w = __int_as_float(0x7fc00000);
-    if (lane < p.n_used) {
-        p.ids[(size_t)t * p.n_used + lane] = my_id;
-        p.w[(size_t)t * p.n_used + lane] = w;
+    if (chosen) {
+        p.ids[(size_t)t * p.n_used + rank] = my_id;
+        p.w[(size_t)t * p.n_used + rank] = w;
     }
 }
 
+template <class Act, int NV>
+void launch_width(const RouteParams& p, bool wide, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(Act) < NV ? 16 / sizeof(Act) : NV;
+    const int grid = (p.n_tokens + kWarps - 1) / kWarps;
+    if (wide && p.n_experts % V == 0)
+        k_route<Act, NV, V><<<grid, kWarps * 32, 0, st>>>(p);
+    else
+        k_route<Act, NV, 1><<<grid, kWarps * 32, 0, st>>>(p);
+}
 template <class Act>
 void launch_route(const RouteParams& p, cudaStream_t st) {
-    const int grid = (p.n_tokens + kWarps - 1) / kWarps;
+    const bool wide = ((uintptr_t)p.x | p.row_stride) % 16 == 0;
     if (p.n_experts <= 128)
-        k_route<Act, 4><<<grid, kWarps * 32, 0, st>>>(p);
+        launch_width<Act, 4>(p, wide, st);
+    else if (p.n_experts <= 256)
+        launch_width<Act, 8>(p, wide, st);
     else if (p.n_experts <= 512)
-        k_route<Act, 16><<<grid, kWarps * 32, 0, st>>>(p);
+        launch_width<Act, 16>(p, wide, st);
+    else if (p.n_experts <= 1024)
+        launch_width<Act, 32>(p, wide, st);
     else
-        k_route<Act, 64><<<grid, kWarps * 32, 0, st>>>(p);
+        launch_width<Act, 64>(p, wide, st);
 }
 
 }  // namespace

@@ -99,32 +99,29 @@ def moe_block_ids(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, ids:
 
 
 # ---------------------------------------------------------------------------
-# the step around the experts: attention over a paged cache, the router
+# the step around the experts: attention over a paged cache, the router. Inputs
+# are checked (ValueError); outputs that are not given come from torch's
+# allocator on the stream that the kernel runs on: the current one, or `stream`.
 # ---------------------------------------------------------------------------
-_ACT = {torch.float32: rt.ACT_F32, torch.float16: rt.ACT_F16, torch.bfloat16: rt.ACT_BF16}
+_native = None
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _empty(shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
-    """Device memory that belongs to the stream the kernel runs on."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
-
-
-def _cache_shape(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor) -> tuple:
-    """Shape and byte strides of a cache [pages, page_size, kv_heads, head_dim]."""
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "caches: two of [pages, page_size, kv_heads, head_dim]")
-    _need(k_cache.dtype == v_cache.dtype and k_cache.dtype in (torch.float16, torch.bfloat16), "caches: f16 or bf16")
-    _need(k_cache.device == v_cache.device == like.device, "caches: on the device of the other tensors")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    _need(k_cache.numel() == 0 or (ks[3] == 1 and vs[3] == 1), "caches: head_dim must be dense")
-    return k_cache.shape, (2 * ks[0], 2 * ks[1], 2 * ks[2]), (2 * vs[0], 2 * vs[1], 2 * vs[2])
+def _ops():
+    """The native side of these calls (csrc/sb_torch.cpp): argument checks, outputs, the current
+    stream. Bound to the loaded runtime once."""
+    global _native
+    if _native is None:
+        L = rt.lib()
+        try:
+            from . import _torch_ops
+        except ImportError as e:
+            raise rt.RuntimeUnavailable("could not load _torch_ops.so (%s): build it with make -C "
+                                        "sabah_moe_accelerator_b200/csrc" % e)
+        _torch_ops.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.sabah_qk_norm_rope, L.sabah_attend_paged, L.sabah_attend_paged_workspace, L.sabah_route_topk,
+            L.sabah_rt_last_error)), rt.SabahCudaError)
+        _native = _torch_ops
+    return _native
 
 
 def rope_table(n_positions: int, rope_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -151,67 +148,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, q_wei
     f16 or bf16 and the int64 row of each token (negative: none); returns q_out.
     Without a cache v is not read, and (q_out, k_out) is returned.
     """
-    T, n_q, D = q.shape
-    _need(k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, "k: [tokens, kv_heads, head_dim] beside q")
-    n_kv = k.shape[1]
-    act = _ACT.get(q.dtype)
-    _need(act is not None and k.dtype == q.dtype, "q and k: both f32, f16 or bf16")
-    _need(q.is_cuda and k.device == q.device, "q and k: on one CUDA device")
-    _need(pairing == "halves" or pairing == "pairs", 'pairing: "halves" or "pairs"')
-    eb = q.element_size()
-    qs, ks, vs = q.stride(), k.stride(), (0, 0, 1)
-    _need(q.numel() == 0 or qs[2] == 1, "q: head_dim must be dense")
-    _need(k.numel() == 0 or ks[2] == 1, "k: head_dim must be dense")
-    for w in (q_weight, k_weight):
-        _need(w is None or (w.shape == (D,) and w.dtype == torch.float32 and w.is_contiguous()
-                            and w.device == q.device), "norm weights: dense float32 [head_dim] or None")
-    n_pos = rope = axes = 0
-    if table is not None:
-        _need(table.dim() == 3 and table.shape[2] == 2 and table.dtype == torch.float32 and table.is_contiguous()
-              and table.device == q.device, "table: dense float32 [positions, rope_dim / 2, 2]")
-        n_pos, rope = table.shape[0], 2 * table.shape[1]
-        _need(positions is not None and positions.dtype == torch.int32 and positions.is_contiguous()
-              and positions.shape[-1:] == (T,) and positions.dim() <= 2 and positions.device == q.device,
-              "positions: dense int32 [tokens] or [axes, tokens]")
-        axes = positions.shape[0] if positions.dim() == 2 else 1
-        _need(pair_axis is None or (pair_axis.shape == (rope // 2,) and pair_axis.dtype == torch.uint8
-                                    and pair_axis.is_contiguous() and pair_axis.device == q.device),
-              "pair_axis: dense uint8 [rope_dim / 2]")
-    kc = vc = (0, 0, 0)
-    n_pages = page_size = ctype = 0
-    k_cache = v_cache = slots = None
-    if cache is not None:
-        k_cache, v_cache, slots = cache
-        shape, kc, vc = _cache_shape(k_cache, v_cache, q)
-        n_pages, page_size = shape[0], shape[1]
-        _need(shape[2] == n_kv and shape[3] == D, "caches: kv_heads and head_dim as k's")
-        _need(v is not None and v.shape == k.shape and v.dtype == k.dtype and v.device == k.device, "v: as k")
-        vs = v.stride()
-        _need(v.numel() == 0 or vs[2] == 1, "v: head_dim must be dense")
-        _need(slots.shape == (T,) and slots.dtype == torch.int64 and slots.is_contiguous()
-              and slots.device == q.device, "slots: dense int64 [tokens]")
-        ctype = _ACT[k_cache.dtype]
-    elif k_out is None:
-        k_out = _empty((T, n_kv, D), q.dtype, q, stream)
-    if q_out is None:
-        q_out = _empty((T, n_q, D), q.dtype, q, stream)
-    _need(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous() and q_out.device == q.device,
-          "q_out: dense, as q")
-    _need(k_out is None or (k_out.shape == k.shape and k_out.dtype == k.dtype and k_out.is_contiguous()
-                            and k_out.device == k.device), "k_out: dense, as k")
-    rc = rt.lib().sabah_qk_norm_rope(
-        q.data_ptr(), eb * qs[0], eb * qs[1], n_q, k.data_ptr(), eb * ks[0], eb * ks[1],
-        None if cache is None else v.data_ptr(), eb * vs[0], eb * vs[1], n_kv, T, D, act,
-        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-        None if table is None else table.data_ptr(), n_pos, rope, pairing == "pairs",
-        None if table is None else positions.data_ptr(), axes,
-        None if table is None or pair_axis is None else pair_axis.data_ptr(), q_out.data_ptr(),
-        None if k_out is None else k_out.data_ptr(),
-        None if cache is None else k_cache.data_ptr(), kc[0], kc[1], kc[2],
-        None if cache is None else v_cache.data_ptr(), vc[0], vc[1], vc[2], n_pages, page_size, ctype,
-        None if cache is None else slots.data_ptr(), _stream(stream))
-    rt.check(rc, "sabah_qk_norm_rope")
-    return q_out if cache is not None else (q_out, k_out)
+    if pairing != "halves" and pairing != "pairs":
+        raise ValueError('pairing: "halves" or "pairs"')
+    k_cache, v_cache, slots = cache if cache is not None else (None, None, None)
+    args = (q, k, v, q_weight, k_weight, table, positions, eps, pairing == "pairs", pair_axis, k_cache, v_cache, slots,
+            q_out, k_out)
+    if stream is None:
+        return (_native or _ops()).norm_rope(*args)
+    with torch.cuda.stream(stream):
+        return _ops().norm_rope(*args)
 
 
 def attend_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -228,39 +173,11 @@ def attend_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     workspace: uint8 memory of rt.lib().sabah_attend_paged_workspace(q_heads,
     kv_heads, D) bytes, by default from torch's allocator for each call.
     """
-    B, H, D = q.shape
-    act = _ACT.get(q.dtype)
-    (n_pages, page_size, n_kv, cd), kc, vc = _cache_shape(k_cache, v_cache, q)
-    _need(act is not None and (act == rt.ACT_F32 or q.dtype == k_cache.dtype), "q: f32 or the cache's type")
-    _need(cd == D and n_kv > 0 and H % n_kv == 0, "q heads: a multiple of the cache's, of one head_dim")
-    _need(q.is_cuda, "q: on a CUDA device")
-    qs, eb = q.stride(), q.element_size()
-    _need(q.numel() == 0 or qs[2] == 1, "q: head_dim must be dense")
-    _need(block_table.dim() == 2 and block_table.shape[0] == B and block_table.dtype == torch.int32
-          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == q.device,
-          "block_table: int32 [sequences, pages per sequence]")
-    _need(lens.shape == (B,) and lens.dtype == torch.int32 and lens.is_contiguous() and lens.device == q.device,
-          "lens: dense int32 [sequences]")
-    if out is None:
-        out = _empty((B, H, D), q.dtype, q, stream)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == q.device,
-              "out: dense, as q")
-    _need(lse is None or (lse.shape == (B, H) and lse.dtype == torch.float32 and lse.is_contiguous()
-                          and lse.device == q.device), "lse: dense float32 [sequences, q_heads]")
-    L = rt.lib()
-    if workspace is None:
-        workspace = _empty(L.sabah_attend_paged_workspace(H, n_kv, D), torch.uint8, q, stream)
-    else:
-        _need(workspace.is_contiguous() and workspace.device == q.device, "workspace: dense, on q's device")
-    rc = L.sabah_attend_paged(
-        q.data_ptr(), eb * qs[0], eb * qs[1], act, k_cache.data_ptr(), kc[0], kc[1], kc[2],
-        v_cache.data_ptr(), vc[0], vc[1], vc[2], _ACT[k_cache.dtype], n_pages, page_size, block_table.data_ptr(),
-        4 * block_table.stride(0), block_table.shape[1], lens.data_ptr(), B, H, n_kv, D,
-        D ** -0.5 if scale is None else scale, window, out.data_ptr(), None if lse is None else lse.data_ptr(),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
-    rt.check(rc, "sabah_attend_paged")
-    return out
+    args = (q, k_cache, v_cache, block_table, lens, scale, window, out, lse, workspace)
+    if stream is None:
+        return (_native or _ops()).attend(*args)
+    with torch.cuda.stream(stream):
+        return _ops().attend(*args)
 
 
 def route_topk(logits: torch.Tensor, n_used: int, *, renorm: bool = True, scale: float = 1.0,
@@ -270,18 +187,7 @@ def route_topk(logits: torch.Tensor, n_used: int, *, renorm: bool = True, scale:
     The n_used largest logits per token, ties to the lower index, in descending
     order; w is their softmax times scale, over the chosen (renorm) or all experts.
     """
-    T, E = logits.shape
-    act = _ACT.get(logits.dtype)
-    _need(act is not None and logits.is_cuda, "logits: f32, f16 or bf16 on a CUDA device")
-    _need(logits.numel() == 0 or E == 1 or logits.stride(1) == 1, "logits: experts must be dense")
-    if ids is None:
-        ids = _empty((T, n_used), torch.int32, logits, stream)
-    if w is None:
-        w = _empty((T, n_used), torch.float32, logits, stream)
-    for t, dt in ((ids, torch.int32), (w, torch.float32)):
-        _need(t.shape == (T, n_used) and t.dtype == dt and t.is_contiguous() and t.device == logits.device,
-              "ids and w: dense int32 and float32 [tokens, n_used]")
-    rc = rt.lib().sabah_route_topk(logits.data_ptr(), logits.element_size() * logits.stride(0), act, T, E, n_used,
-                                   renorm, scale, ids.data_ptr(), w.data_ptr(), _stream(stream))
-    rt.check(rc, "sabah_route_topk")
-    return ids, w
+    if stream is None:
+        return (_native or _ops()).route(logits, n_used, renorm, scale, ids, w)
+    with torch.cuda.stream(stream):
+        return _ops().route(logits, n_used, renorm, scale, ids, w)
