@@ -10,11 +10,13 @@
 // The cosines come from a table: pos * frequency in fp32 would lose a radian's
 // third decimal at positions of 1e5.
 //
-// Bound: DRAM, each row read once and written once. A row is a lane group of
-// LPR lanes; a lane owns both halves of its pairs (W consecutive pairs, as two
-// chunks of W values), so the rotation needs no exchange and only the sum of
-// squares is shuffled. A warp takes several rows of one token and reads the
-// token's cosines once for all of them.
+// Bound: DRAM, each row read once and written once, with the instructions per
+// row not far behind. A row is a lane group of LPR lanes; a lane owns both
+// halves of its pairs (W consecutive pairs, as two chunks of W values), so the
+// rotation needs no exchange and only the sum of squares is shuffled. A warp
+// takes several rows of one token and one kind (queries, keys or values), reads
+// the token's cosines once for all of them and multiplies them by the weights:
+// a turned value is then two products and one by the norm.
 #include "sb_act.cuh"
 #include "sb_kernels.h"
 
@@ -41,37 +43,21 @@ struct NormRopeParams {
     unsigned n_slots;
     const int64_t* slots;
     int* err;
-    int rows, blocks;   // rows of a token; warp tasks of a token
+    int q_blocks, kv_blocks, blocks;   // warp tasks of a token: for queries, for keys or values, in all
 };
 
+// W consecutive values, loaded and stored at once
 template <class T, int W>
-__device__ inline void load_chunk(const T* p, float* f) {
-    if constexpr (W == 4 && sizeof(T) == 4) {
-        const float4 u = *(const float4*)p;
-        f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w;
-    } else if constexpr (W == 4) {
-        const uint2 u = *(const uint2*)p;
-        const T* h = (const T*)&u;
+struct alignas(sizeof(T) * W) Chunk {
+    T v[W];
+    __device__ void load(const T* p) { *this = *(const Chunk*)p; }
+    __device__ static void store(T* p, const float* f) {
+        Chunk c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = sb_to_float(h[i]);
-    } else {
-        f[0] = sb_to_float(*p);
+        for (int i = 0; i < W; ++i) c.v[i] = sb_from_float<T>(f[i]);
+        *(Chunk*)p = c;
     }
-}
-template <class T, int W>
-__device__ inline void store_chunk(T* p, const float* f) {
-    if constexpr (W == 4 && sizeof(T) == 4) {
-        *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
-    } else if constexpr (W == 4) {
-        uint2 u;
-        T* h = (T*)&u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = sb_from_float<T>(f[i]);
-        *(uint2*)p = u;
-    } else {
-        *p = sb_from_float<T>(f[0]);
-    }
-}
+};
 
 // LPR lanes per row, NP chunk pairs of W values per lane, ITER rows per lane group
 template <class Act, class Cache, int W, int LPR, int NP, int ITER>
@@ -81,7 +67,15 @@ __global__ void __launch_bounds__(kWarps * 32) k_norm_rope(const __grid_constant
     const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR;
     const int t = (int)(task / (unsigned)p.blocks);
     if (t >= p.n_tokens) return;
-    const int row0 = (int)(task - (unsigned)t * (unsigned)p.blocks) * kRows * ITER + grp;
+    int block = (int)(task - (unsigned)t * (unsigned)p.blocks);
+    const int kind = block < p.q_blocks ? 0 : block < p.q_blocks + p.kv_blocks ? 1 : 2;   // queries, keys, values
+    block -= kind == 0 ? 0 : kind == 1 ? p.q_blocks : p.q_blocks + p.kv_blocks;
+    const int row0 = block * kRows * ITER + grp, rows = kind == 0 ? p.n_q : p.n_kv;
+    const size_t head = kind == 0 ? p.q_head : kind == 1 ? p.k_head : p.v_head;
+    const uint8_t* src = kind == 0   ? p.q + (size_t)t * p.q_token
+                         : kind == 1 ? p.k + (size_t)t * p.k_token
+                                     : p.v + (size_t)t * p.v_token;
+    src += row0 * head;
     const int half = p.rope / 2;
 
     // where this lane's chunk pairs lie in a row
@@ -94,138 +88,138 @@ __global__ void __launch_bounds__(kWarps * 32) k_norm_rope(const __grid_constant
         at[n][1] = split ? cp * W + half : cp * 2 * W + W;
     }
     // all of the task's rows are on their way before anything waits
-    float x[ITER][NP][2][W];
+    Chunk<Act, W> raw[ITER][NP][2];
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-        const int r = row0 + it * kRows;
-        const uint8_t* src = r < p.n_q            ? p.q + (size_t)t * p.q_token + (size_t)r * p.q_head
-                             : r < p.n_q + p.n_kv ? p.k + (size_t)t * p.k_token + (size_t)(r - p.n_q) * p.k_head
-                                                  : p.v + (size_t)t * p.v_token + (size_t)(r - p.n_q - p.n_kv) * p.v_head;
+    for (int it = 0; it < ITER; ++it)
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (r < p.rows && at[n][0] >= 0)
-                    load_chunk<Act, W>((const Act*)src + at[n][h], x[it][n][h]);
+            for (int h = 0; h < 2; ++h)
+                if (row0 + it * kRows < rows && at[n][0] >= 0)
+                    raw[it][n][h].load((const Act*)(src + it * kRows * head) + at[n][h]);
                 else
 #pragma unroll
-                    for (int i = 0; i < W; ++i) x[it][n][h][i] = 0.f;
-            }
+                    for (int i = 0; i < W; ++i) raw[it][n][h].v[i] = sb_from_float<Act>(0.f);
+
+    // where the rows go
+    uint8_t* cache = nullptr;
+    size_t cache_head = 0;
+    if (kind != 0 && p.slots) {
+        const long long slot = p.slots[t];
+        if (slot >= (long long)p.n_slots) {
+            if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
+        } else if (slot >= 0) {
+            const unsigned page = (unsigned)slot / (unsigned)p.page_size, in_page = (unsigned)slot - page * p.page_size;
+            cache_head = kind == 1 ? p.kc_head : p.vc_head;
+            cache = (kind == 1 ? p.k_cache + page * p.kc_page + in_page * p.kc_slot
+                               : p.v_cache + page * p.vc_page + in_page * p.vc_slot) + row0 * cache_head;
+        }
     }
-    long long slot = p.slots ? p.slots[t] : -1;
-    // the cosines of this lane's pairs, once for all of its rows
-    float c[NP][W], s[NP][W];
+    if (kind == 2) {
+        if (cache)
+#pragma unroll
+            for (int it = 0; it < ITER; ++it)
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (row0 + it * kRows >= rows || at[n][0] < 0) continue;
+                        float f[W];
+#pragma unroll
+                        for (int i = 0; i < W; ++i) f[i] = sb_to_float(raw[it][n][h].v[i]);
+                        Chunk<Cache, W>::store((Cache*)(cache + it * kRows * cache_head) + at[n][h], f);
+                    }
+        return;
+    }
+    Act* dst = (Act*)(kind == 0 ? p.q_out : p.k_out);
+    if (dst) dst += ((size_t)t * rows + row0) * p.dim;
+
+    // the turn of this lane's pairs (a, b) -> (a ca - b sb, a sa + b cb), with
+    // the weights in it; a value that is not turned has (weight, 0, 0, weight)
+    const float* weight = kind == 0 ? p.q_weight : p.k_weight;
+    float ca[NP][W], sb[NP][W], sa[NP][W], cb[NP][W];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
         const int pair0 = (sub + n * LPR) * W;
         const bool turned = pair0 * 2 < p.rope;
+        float cs[2 * W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            c[n][i] = 1.f;
-            s[n][i] = 0.f;
-        }
-        if (!turned) continue;
-        if (p.pair_axis == nullptr) {
+        for (int i = 0; i < W; ++i) cs[2 * i] = 1.f, cs[2 * i + 1] = 0.f;
+        if (turned && p.pair_axis == nullptr) {
             const int pos = p.positions[t];
             const bool out = pos < 0 || pos >= p.n_positions;
             if (out) atomicExch(p.err, SB_DERR_BAD_INDEX);
-            float cs[2 * W];
-            const float* src = (const float*)(p.table + (size_t)(out ? 0 : pos) * half + pair0);
-            if constexpr (W == 4) {
-                load_chunk<float, W>(src, cs);
-                load_chunk<float, W>(src + W, cs + W);
-            } else {
-                cs[0] = __ldg(src), cs[1] = __ldg(src + 1);
-            }
+            const float* from = (const float*)(p.table + (size_t)(out ? 0 : pos) * half + pair0);
+            Chunk<float, W> u[2];
+            u[0].load(from), u[1].load(from + W);
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                c[n][i] = out ? __int_as_float(0x7fc00000) : cs[2 * i];
-                s[n][i] = out ? __int_as_float(0x7fc00000) : cs[2 * i + 1];
-            }
-        } else {
+            for (int i = 0; i < 2 * W; ++i) cs[i] = out ? __int_as_float(0x7fc00000) : u[i / W].v[i % W];
+        } else if (turned) {
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const int axis = p.pair_axis[pair0 + i];
                 const int pos = axis < p.n_axes ? p.positions[(size_t)axis * p.n_tokens + t] : -1;
                 const bool out = pos < 0 || pos >= p.n_positions;
                 if (out) atomicExch(p.err, SB_DERR_BAD_INDEX);
-                const float2 cs = __ldg(p.table + (size_t)(out ? 0 : pos) * half + pair0 + i);
-                c[n][i] = out ? __int_as_float(0x7fc00000) : cs.x;
-                s[n][i] = out ? __int_as_float(0x7fc00000) : cs.y;
+                const float* from = (const float*)(p.table + (size_t)(out ? 0 : pos) * half + pair0 + i);
+                cs[2 * i] = out ? __int_as_float(0x7fc00000) : __ldg(from);
+                cs[2 * i + 1] = out ? __int_as_float(0x7fc00000) : __ldg(from + 1);
             }
         }
+        Chunk<float, W> w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (weight && at[n][0] >= 0)
+                w[h].load(weight + at[n][h]);
+            else
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[h].v[i] = 1.f;
+        // the lane's 2 W values in memory order; pair i is (i, i + W), or (2i, 2i + 1) in pairs mode
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const bool next = p.pairs_mode && W > 1;
+            const float wa = next ? w[2 * i / W].v[2 * i % W] : w[0].v[i];
+            const float wb = next ? w[(2 * i + 1) / W].v[(2 * i + 1) % W] : w[1].v[i];
+            ca[n][i] = wa * cs[2 * i], sa[n][i] = wa * cs[2 * i + 1];
+            sb[n][i] = wb * cs[2 * i + 1], cb[n][i] = wb * cs[2 * i];
+        }
     }
-    if (slot >= (long long)p.n_slots) {
-        if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
-        slot = -1;
-    }
-    const unsigned page = slot < 0 ? 0 : (unsigned)slot / p.page_size;
-    const unsigned in_page = slot < 0 ? 0 : (unsigned)slot - page * p.page_size;
 
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
-        const int r = row0 + it * kRows;
-        const bool here = r < p.rows;
-        const bool is_q = r < p.n_q, is_v = r >= p.n_q + p.n_kv;
-        const float* weight = is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
-        float sum = 0.f;
+        float x[NP][2 * W], sum = 0.f;
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < W; ++i) sum += x[it][n][h][i] * x[it][n][h][i];
+            for (int i = 0; i < 2 * W; ++i) {
+                x[n][i] = sb_to_float(raw[it][n][i / W].v[i % W]);
+                sum += x[n][i] * x[n][i];
+            }
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (!here) continue;
-        const float inv = rsqrtf(sum * p.over_dim + p.eps);
-        const int kv = is_v ? r - p.n_q - p.n_kv : r - p.n_q;
+        if (row0 + it * kRows >= rows) continue;
+        const float inv = weight ? rsqrtf(sum * p.over_dim + p.eps) : 1.f;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if (at[n][0] < 0) continue;
-            float y[2][W];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float w[W];
-                if (weight) load_chunk<float, W>(weight + at[n][h], w);
-#pragma unroll
-                for (int i = 0; i < W; ++i) y[h][i] = weight ? x[it][n][h][i] * inv * w[i] : x[it][n][h][i];
-            }
-            if (!is_v && (sub + n * LPR) * 2 * W < p.rope) {
-                float z[2][W];
-                if (p.pairs_mode && W > 1) {   // (2i, 2i + 1): neighbours in the lane's 2 W values
-#pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        const float a = (&y[0][0])[2 * i], b = (&y[0][0])[2 * i + 1];
-                        (&z[0][0])[2 * i] = a * c[n][i] - b * s[n][i];
-                        (&z[0][0])[2 * i + 1] = a * s[n][i] + b * c[n][i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        z[0][i] = y[0][i] * c[n][i] - y[1][i] * s[n][i];
-                        z[1][i] = y[0][i] * s[n][i] + y[1][i] * c[n][i];
-                    }
-                }
+            float y[2 * W];
+            if (p.pairs_mode && W > 1) {
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
-                    y[0][i] = z[0][i];
-                    y[1][i] = z[1][i];
+                    y[2 * i] = (x[n][2 * i] * ca[n][i] - x[n][2 * i + 1] * sb[n][i]) * inv;
+                    y[2 * i + 1] = (x[n][2 * i] * sa[n][i] + x[n][2 * i + 1] * cb[n][i]) * inv;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    y[i] = (x[n][i] * ca[n][i] - x[n][i + W] * sb[n][i]) * inv;
+                    y[i + W] = (x[n][i] * sa[n][i] + x[n][i + W] * cb[n][i]) * inv;
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (is_q) {
-                    store_chunk<Act, W>((Act*)p.q_out + ((size_t)t * p.n_q + r) * p.dim + at[n][h], y[h]);
-                    continue;
-                }
-                if (!is_v && p.k_out)
-                    store_chunk<Act, W>((Act*)p.k_out + ((size_t)t * p.n_kv + kv) * p.dim + at[n][h], y[h]);
-                if (slot >= 0) {
-                    uint8_t* dst = is_v ? p.v_cache + page * p.vc_page + in_page * p.vc_slot + kv * p.vc_head
-                                        : p.k_cache + page * p.kc_page + in_page * p.kc_slot + kv * p.kc_head;
-                    store_chunk<Cache, W>((Cache*)dst + at[n][h], y[h]);
-                }
+                if (dst) Chunk<Act, W>::store(dst + it * kRows * p.dim + at[n][h], y + h * W);
+                if (cache) Chunk<Cache, W>::store((Cache*)(cache + it * kRows * cache_head) + at[n][h], y + h * W);
             }
         }
     }
@@ -234,7 +228,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_norm_rope(const __grid_constant
 template <class Act, class Cache, int W, int LPR, int NP, int ITER>
 void launch(NormRopeParams p, cudaStream_t st) {
     const int per_task = 32 / LPR * ITER;
-    p.blocks = (p.rows + per_task - 1) / per_task;
+    p.q_blocks = (p.n_q + per_task - 1) / per_task;
+    p.kv_blocks = (p.n_kv + per_task - 1) / per_task;
+    p.blocks = p.q_blocks + p.kv_blocks * (p.slots ? 2 : 1);
     const long long tasks = (long long)p.n_tokens * p.blocks;
     k_norm_rope<Act, Cache, W, LPR, NP, ITER><<<(unsigned)((tasks + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(p);
 }
@@ -244,7 +240,7 @@ void launch(NormRopeParams p, cudaStream_t st) {
 // the work, where few rows want all the warps there are.
 template <class Act, class Cache, int LPR>
 void launch_wide(const NormRopeParams& p, cudaStream_t st) {
-    if ((long long)p.n_tokens * p.rows * LPR / 32 > 2 * 148 * 64)
+    if ((long long)p.n_tokens * (p.n_q + 2 * p.n_kv) * LPR / 32 > 2 * 148 * 64)
         launch<Act, Cache, 4, LPR, 1, 4>(p, st);
     else
         launch<Act, Cache, 4, LPR, 1, 1>(p, st);
@@ -335,7 +331,7 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
     p.kc_page = k_page_stride, p.kc_slot = k_slot_stride, p.kc_head = k_cache_head_stride;
     p.vc_page = v_page_stride, p.vc_slot = v_slot_stride, p.vc_head = v_cache_head_stride;
     p.page_size = cache ? page_size : 1, p.n_slots = cache ? (unsigned)n_pages * (unsigned)page_size : 0;
-    p.slots = d_slots, p.err = err, p.rows = rows;
+    p.slots = d_slots, p.err = err;
     // four values at a time where rows, pairs and pointers allow it
     const bool wide = head_dim % 8 == 0 && rope_dim % 8 == 0 && act_bits % (4 * ab) == 0 && cache_bits % 8 == 0 &&
                       (f32_bits | (uintptr_t)d_table) % 16 == 0;

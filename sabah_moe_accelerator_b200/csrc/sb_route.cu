@@ -38,15 +38,17 @@ struct RouteParams {
     float* w;
 };
 
-// Larger float <=> larger key; 0 is free for "taken", NaN ranks below -inf.
+// Larger float <=> larger key. 0 is free for "taken" and "none"; a NaN is
+// below -inf once sink_nan() has seen it.
 __device__ inline uint32_t order_key(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if (f != f) return 1;
-    if (f == 0.f) return 0x80000000u;   // -0 ties with +0
-    return (u >> 31) ? ~u : u | 0x80000000u;
+    const int u = __float_as_int(f + 0.f);   // -0 ties with +0
+    return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
 }
 __device__ inline float key_value(uint32_t k) {
     return k == 1 ? __int_as_float(0x7fc00000) : __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+__device__ inline uint32_t sink_nan(uint32_t k) {   // beyond the keys of +-inf lie the NaNs
+    return k > 0xff800000u || (k && k < 0x007fffffu) ? 1 : k;
 }
 
 // NV: logits per lane (n_experts <= 32 * NV), V of them side by side
@@ -58,8 +60,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
     const Act* row = (const Act*)(p.x + (size_t)t * p.row_stride);
     auto expert = [&](int i) { return (i / V * 32 + lane) * V + i % V; };
     uint32_t key[NV];
-    uint32_t top = 0;
-    bool nan = false;
+    float odd = 0.f;   // a NaN once a NaN or an infinity went in
 #pragma unroll
     for (int c = 0; c < NV / V; ++c) {
         struct alignas(V * sizeof(Act)) Chunk { Act x[V]; };
@@ -67,14 +68,25 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
         Chunk u;
         if (e < p.n_experts) u = *(const Chunk*)(row + e);
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[c * V + i] = e < p.n_experts ? order_key(sb_to_float(u.x[i])) : 0;
+        for (int i = 0; i < V; ++i) {
+            const float x = e < p.n_experts ? sb_to_float(u.x[i]) : 0.f;
+            key[c * V + i] = e < p.n_experts ? order_key(x) : 0;
+            odd += x * 0.f;
+        }
     }
+    bool nan = __any_sync(~0u, odd != 0.f);
+    if (nan) {   // only then the keys are looked at one by one
+        nan = false;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        nan |= key[i] == 1;
-        top = max(top, key[i]);
+        for (int i = 0; i < NV; ++i) {
+            key[i] = sink_nan(key[i]);
+            nan |= key[i] == 1;
+        }
+        nan = __any_sync(~0u, nan);
     }
-    nan = __any_sync(~0u, nan);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = max(top, key[i]);
     const uint32_t first = __reduce_max_sync(~0u, top);
     const float m = key_value(first);
     float total = 0.f;   // of all, where the weights are over all experts
@@ -99,13 +111,21 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
         }
         bound = k;
     }
-    int n = 0;
+    int here = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const unsigned who = __ballot_sync(~0u, key[i] >= bound);
-        const int at = n + __popc(who & ((1u << lane) - 1));
-        if (key[i] >= bound && at < 32) picked[wid][at] = make_uint2(key[i], expert(i));
-        n += __popc(who);
+    for (int i = 0; i < NV; ++i) here += key[i] >= bound;
+    int upto = here;   // in the lanes before and this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    const int n = __shfl_sync(~0u, upto, 31);
+    if (n <= 32) {
+        uint2* next = &picked[wid][upto - here];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (key[i] >= bound) *next++ = make_uint2(key[i], expert(i));
     }
     uint32_t mine = 0;   // this lane's choice: its key, expert and rank
     int my_id = 0, rank = p.n_used;
@@ -116,9 +136,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
             mine = u.x, my_id = u.y, rank = 0;
         }
         for (int j = 0; j < n; ++j) {
-            const uint32_t k = __shfl_sync(~0u, mine, j);
-            const int e = __shfl_sync(~0u, my_id, j);
-            rank += k > mine || (k == mine && e < my_id);
+            const uint2 u = picked[wid][j];
+            rank += u.x > mine || (u.x == mine && (int)u.y < my_id);
         }
     } else {
         for (int j = 0; j < p.n_used; ++j) {
