@@ -21,8 +21,9 @@
 // and the rest is small parts that warps take as they finish, because SMs do
 // not all get the same share of the bandwidth. Warps never wait for one
 // another; each streams its own keys and values through its own ring in shared
-// memory, filled by TMA: boxes of as many rows as divide both a page and 16, 64
-// columns wide in the 128-byte swizzle that lets ldmatrix meet no bank twice.
+// memory, filled by TMA: boxes of as many rows as divide both a page and 16, in
+// tiles of 64 columns in the 128-byte swizzle that lets ldmatrix meet no bank
+// twice; one box has all tiles of 16 rows where whole tiles make up a row.
 // Rows of a box past the window's ends are masked (keys) or zeroed (values),
 // so that nothing they hold counts. A row of the list that ends in a
 // part is left as (m, l, unnormalised out) in the workspace, and a second,
@@ -59,7 +60,7 @@ constexpr int kWhole = 4;        // rows of at most this many steps are never cu
 constexpr int kMinSteps = 2;     // and a part is at least this long
 constexpr int kRowCost = 1;      // what a row costs besides its steps, in steps
 constexpr int kShare = 16;       // steps per warp from which the last 3/16 are shared out
-constexpr int kMaxWarps = 148 * 2 * 8, kMaxParts = 3 * kMaxWarps;
+constexpr int kMaxWarps = 148 * 8, kMaxParts = 3 * kMaxWarps;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr float kLazy = 4.f;     // how far, in powers of two, a score may exceed the reference
 
@@ -78,6 +79,7 @@ struct AttendParams {
     size_t k_page, k_slot, k_head, v_page, v_slot, v_head;   // bytes
     int n_pages, page_size, page_shift;   // shift: log2(page_size), or -1
     int box;                // rows of a TMA box: a power of two to 16 that divides the page
+    int box_tiles;          // its tiles of 64 columns: all of a row's, or one
     const int32_t* table;
     size_t table_stride;    // elements
     int table_width;
@@ -126,9 +128,9 @@ __device__ inline unsigned long long pass_through() {
 }
 __device__ inline void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int slot, int head, int page,
                                  unsigned long long policy) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-                 "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(slot), "r"(head),
-                 "r"(page), "l"(policy) : "memory");
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+                 "[%0], [%1, {%3, %4, %8, %5, %6}], [%2], %7;" ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(slot), "r"(head),
+                 "r"(page), "l"(policy), "r"(0) : "memory");
 }
 __device__ inline void ldsm4(uint32_t* r, uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -177,11 +179,11 @@ __device__ inline bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; 
 
 // ------------------------------------------------------------ shapes
 // DP: head size rounded up to a tile width. A slot of a ring is the keys or the
-// values of a step, as kTiles tiles of 32 rows x 64 columns (128 swizzled bytes).
+// values of a step: twice kTiles tiles of 16 rows x 64 columns (128 swizzled bytes).
 template <int DP>
 struct Shape {
     static constexpr int kTiles = (DP + 63) / 64;
-    static constexpr int kTileBytes = kStep * 128, kSlot = kTiles * kTileBytes;
+    static constexpr int kTileBytes = 16 * 128, kHalf = kTiles * kTileBytes, kSlot = 2 * kHalf;
     static constexpr int kSlots = DP <= 64 ? 6 : 3;
     static constexpr int kWarps = DP <= 128 ? 8 : DP <= 192 ? 5 : 4;
 };
@@ -199,20 +201,26 @@ __device__ inline int window_start(int len, int window) { return window > 0 ? ma
 __device__ inline int seq_steps(int len, int window) {
     return len <= 0 ? 1 : (len + kStep - 1) / kStep - window_start(len, window) / kStep;
 }
+// a / b; the integer division is a long subroutine, and most numbers here are small
+__device__ inline int div_fast(int a, int b) {
+    if (a >= 1 << 22) return (int)((unsigned)a / (unsigned)b);
+    int q = (int)__fdividef((float)a, (float)b);   // within one of the quotient
+    q -= q * b > a;
+    return q + (a - q * b >= b);
+}
 // The parts: n_own of `own` places, one per warp, then shared ones of `small`.
 struct Parts {
     int cost, own, own_end, small, n_own, n;
     __device__ Parts(int cost_, int warps, bool share) : cost(cost_) {
-        own = max((int)((unsigned)(cost + warps - 1) / (unsigned)warps), kMinSteps);
+        own = max(div_fast(cost + warps - 1, warps), kMinSteps);
         if (share && own >= kShare) {
             own = own * 13 / 16;
             n_own = warps;
             own_end = own * warps;
-            const unsigned rest = cost - own_end;
-            small = max((int)((rest + 2 * warps - 1) / (2 * warps)), kMinSteps);
-            n = n_own + (int)((rest + small - 1) / small);
+            small = max(div_fast(cost - own_end + 2 * warps - 1, 2 * warps), kMinSteps);
+            n = n_own + div_fast(cost - own_end + small - 1, small);
         } else {
-            n = n_own = (int)((unsigned)(cost + own - 1) / (unsigned)own);
+            n = n_own = div_fast(cost + own - 1, own);
             own_end = cost;
             small = 1;
         }
@@ -220,7 +228,7 @@ struct Parts {
     __device__ int begin(int i) const { return i < n_own ? i * own : own_end + (i - n_own) * small; }
     __device__ int end(int i) const { return i < n_own ? min((i + 1) * own, own_end) : min(own_end + (i + 1 - n_own) * small, cost); }
     __device__ int of(int at) const {
-        return at < own_end ? (int)((unsigned)at / (unsigned)own) : n_own + (int)((unsigned)(at - own_end) / (unsigned)small);
+        return at < own_end ? div_fast(at, own) : n_own + div_fast(at - own_end, small);
     }
 };
 
@@ -266,9 +274,9 @@ __device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, i
         a += last * hop;
     }
     c.b = a;
-    const unsigned at = from - s.pre[a] * n_rows, cost = s.pre[a + 1] - s.pre[a];
-    c.h = (int)(at / cost);
-    const int j = (int)(at - c.h * cost);
+    const int at = from - s.pre[a] * n_rows, cost = s.pre[a + 1] - s.pre[a];
+    c.h = div_fast(at, cost);
+    const int j = at - c.h * cost;
     c.row_at = from - j;
     enter_row(c, s, p, j);
     // a whole row is its first step's part's; past a row's steps are its idle places
@@ -406,14 +414,16 @@ struct Loader {
             __syncwarp();
             dirty &= ~(1u << slot);
         }
-        const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kSlot + lane * p.box * 128;
+        const int first_row = lane * p.box;
+        const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kSlot + first_row / 16 * S::kHalf + first_row % 16 * 128;
         const unsigned boxes = __popc(__ballot_sync(~0u, page >= 0));
         if (lane == 0) bar_expect(bar, boxes * p.box * (128 * S::kTiles));
         if (page >= 0) {
             const CUtensorMap* map = values ? vmap : kmap;
             const int kv = p.tiles == 1 ? c.h : c.h / p.tiles;
-#pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) tile_load(dst + t * S::kTileBytes, map, bar, 64 * t, row, kv, page, policy);
+#pragma unroll 1
+            for (int t = 0; t < S::kTiles; t += p.box_tiles)
+                tile_load(dst + t * S::kTileBytes, map, bar, 64 * t, row, kv, page, policy);
         }
         if (values) advance();
         values = !values;
@@ -561,7 +571,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     Cursor cc = enter_part(seqs, p, parts.begin(w), parts.end(w), w, lane);
     if (cc.b < 0) return;
 
-    // ---- queries on their way, then keys and values
+    // ---- table entries and queries on their way, then keys and values
     const int g = lane >> 2, quad = lane & 3;
     Act qx[NT == 1 ? ND : 1][4];   // the row's query values 16 d + 2 quad + {0, 1, 8, 9}, as they are
     auto fetch_queries = [&](const Cursor& c) {
@@ -569,12 +579,13 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             const Act* src = (const Act*)(p.q + c.b * p.q_seq + (c.h * p.group + min(g, p.group - 1)) * p.q_head);
             if (p.q_pairs) {
                 struct alignas(2 * sizeof(Act)) Pair { Act a, b; };
+                const bool full = p.dim == DP;   // then every offset is a constant
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int at = 16 * d + 2 * quad + i * 8;
-                        const Pair u = *(const Pair*)(src + (at < p.dim ? at : 0));
+                        const int at = 16 * d + i * 8;
+                        const Pair u = *(const Pair*)(src + 2 * quad + (full || at < p.dim ? at : 0));
                         qx[d][2 * i] = u.a, qx[d][2 * i + 1] = u.b;
                     }
             } else {
@@ -588,10 +599,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             }
         }
     };
-    fetch_queries(cc);
     uint8_t* ring_mem = smem + wid * S::kSlots * S::kSlot;
     const uint32_t ring = smem_addr(ring_mem);
     Loader<DP> loader(p, &kmap, &vmap, seqs, parts, lane, ring, bars, queue, cc);
+    fetch_queries(cc);
 #pragma unroll 1
     for (int i = 0; i < S::kSlots; ++i) loader.issue(i);
 
@@ -718,7 +729,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
-                            ldsm4(kf[d / 2 & 1][i][h], ((at + k_lane) ^ (((d + i) & 3) << 5)) + ((d + i) >> 2) * S::kTileBytes + h * 2048);
+                            ldsm4(kf[d / 2 & 1][i][h], ((at + k_lane) ^ (((d + i) & 3) << 5)) + ((d + i) >> 2) * S::kTileBytes + h * S::kHalf);
                 };
                 load_keys(0);
 #pragma unroll
@@ -802,9 +813,13 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             } else {
                 if (edge) {   // zeros for the values outside the window
                     uint8_t* mem = ring_mem + slot * S::kSlot;
-                    for (int i = lane; i < S::kSlot / 16; i += 32) {
-                        const int key = key0 + (i >> 3) % kStep;
-                        if (key < cc.lo || key >= cc.len) *(uint4*)(mem + i * 16) = make_uint4(0, 0, 0, 0);
+                    const int row = lane >> 3;   // 4 rows of a tile at a time
+                    for (int r = row; r < kStep; r += 4) {
+                        if (key0 + r >= cc.lo && key0 + r < cc.len) continue;
+#pragma unroll
+                        for (int t = 0; t < S::kTiles; ++t)
+                            *(uint4*)(mem + r / 16 * S::kHalf + t * S::kTileBytes + r % 16 * 128 + (lane & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
                     }
                     loader.dirty |= 1u << slot;
                     __syncwarp();
@@ -816,7 +831,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll
                     for (int i = 0; i < kAhead; ++i) {
                         const int t = blk * kAhead % ND + i, h = blk * kAhead / ND;
-                        ldsm4t(vf[blk & 1][i], ((at + v_lane) ^ ((t & 3) << 5)) + (t >> 2) * S::kTileBytes + h * 2048);
+                        ldsm4t(vf[blk & 1][i], ((at + v_lane) ^ ((t & 3) << 5)) + (t >> 2) * S::kTileBytes + h * S::kHalf);
                     }
                 };
                 load_values(0);
@@ -974,9 +989,12 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 // Pieces of a cut row, in the order of the keys: weights from their m and l,
 // then the weighted sum. A unit is 8 query heads of a cut row and 16 of its
 // columns, as a lane holds them in a piece. Latency is all there is to it, so a
-// unit is joined by one warp where its row has few pieces and by the 32 warps of
+// unit is joined by one warp where its row has few pieces, by 8 or by the 32 of
 // a CTA where it has more, with kBatch pieces' loads in flight together.
-constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32, kFew = 32, kBatch = 4;
+constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32;
+constexpr int kBatch = 4, kGroup = 8;                          // pieces in flight per warp; warps for some pieces
+constexpr int kFew = 3 * kBatch, kSome = 2 * kGroup * kBatch;   // most pieces for one warp, for kGroup
+constexpr int kChunk = 512;                                    // pieces whose weights are in shared memory
 
 // The weighted sum of pieces first, first + every, .. below n, in this lane's
 // (column, head) places, with its heads' reference and sum.
@@ -984,21 +1002,29 @@ struct Joined {
     float top[2], l[2];
     float4 x;
 };
-__device__ inline void join_add(Joined& j, const float4 ml, const float4 x) {   // ml: (m, l) of both heads
-    const float m[2] = {ml.x, ml.z}, l[2] = {ml.y, ml.w};
-    float old[2], f[2];
+__device__ inline float base_of(float top) { return top == -INFINITY ? 0.f : top; }
+// adds n parts to j: the common reference first, then exps that do not wait for one another
+template <int N>
+__device__ inline void join_add(Joined& j, const float4 (&ml)[N], const float4 (&x)[N]) {   // ml: (m, l) of both heads
+    float top[2] = {j.top[0], j.top[1]};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float t = fmaxf(j.top[i], m[i]), base = t == -INFINITY ? 0.f : t;
-        old[i] = exp2_fast(j.top[i] - base), f[i] = exp2_fast(m[i] - base);
-        j.top[i] = t;
-        j.l[i] = j.l[i] * old[i] + l[i] * f[i];
+    for (int i = 0; i < N; ++i) top[0] = fmaxf(top[0], ml[i].x), top[1] = fmaxf(top[1], ml[i].z);
+    const float base[2] = {base_of(top[0]), base_of(top[1])};
+    const float old[2] = {exp2_fast(j.top[0] - base[0]), exp2_fast(j.top[1] - base[1])};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) j.l[h] *= old[h], j.top[h] = top[h];
+    j.x.x *= old[0], j.x.y *= old[1], j.x.z *= old[0], j.x.w *= old[1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float f = exp2_fast(ml[i].x - base[0]), g = exp2_fast(ml[i].z - base[1]);
+        j.l[0] += ml[i].y * f, j.l[1] += ml[i].w * g;
+        j.x.x += x[i].x * f, j.x.y += x[i].y * g, j.x.z += x[i].z * f, j.x.w += x[i].w * g;
     }
-    j.x.x = j.x.x * old[0] + x.x * f[0], j.x.y = j.x.y * old[1] + x.y * f[1];
-    j.x.z = j.x.z * old[0] + x.z * f[0], j.x.w = j.x.w * old[1] + x.w * f[1];
 }
-__device__ inline Joined join_pieces(const float* base, int piece_floats, int part, int n, int first, int every, int heads_at,
-                                     int unit_at, bool real) {
+__device__ inline const float* piece_at(const AttendParams& p, int part, int k) {
+    return p.pieces + (size_t)(2 * (part + k) + (k == 0)) * p.piece_floats;
+}
+__device__ inline Joined join_pieces(const AttendParams& p, int part, int n, int first, int every, int heads_at, int unit_at, bool real) {
     Joined j{{-INFINITY, -INFINITY}, {0.f, 0.f}, make_float4(0.f, 0.f, 0.f, 0.f)};
     for (int k0 = first; k0 < n; k0 += every * kBatch) {
         float4 ml[kBatch], x[kBatch];
@@ -1008,59 +1034,66 @@ __device__ inline Joined join_pieces(const float* base, int piece_floats, int pa
             ml[i] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
             x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (k < n && real) {
-                const float* src = base + (size_t)(2 * (part + k) + (k == 0)) * piece_floats;
+                const float* src = piece_at(p, part, k);
                 ml[i] = *(const float4*)(src + heads_at);
                 x[i] = *(const float4*)(src + unit_at);
             }
         }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (k0 + i * every < n) join_add(j, ml[i], x[i]);
+        join_add<kBatch>(j, ml, x);
     }
     return j;
 }
 
 template <class Act>
 __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, int dp, float up) {
-    __shared__ uint16_t list[kMaxParts];   // the parts that begin a cut row: few pieces from the front, many from the end
+    // the parts that begin a cut row, with its pieces, and the row: those of few
+    // pieces, then of some, then of many
+    __shared__ uint2 list[kMaxParts];
     __shared__ int counts[2][kJoinWarps];
-    __shared__ Joined sums[kJoinWarps][32];
+    __shared__ union {
+        Joined sums[kJoinWarps / 2][32];
+        struct {
+            float weight[8][kChunk];
+            float red[8][4];   // 8 heads, 4 warps each
+        };
+    } sh;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0) p.head->ready = 0;   // for a next call of the same number (a graph's)
 
-    // ---- the cut rows, in the order of the parts that begin them: 8 parts per thread
-    static_assert(kMaxParts <= kJoinThreads * 8, "one pass");
-    const int first = threadIdx.x * 8;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (first < p.max_parts) raw = *(const uint4*)(p.cut_pieces + first);   // the array is padded to 8
-    const int n_parts = p.head->n_parts;
-    uint16_t n[8];
-    memcpy(n, &raw, 16);
-    int f = 0, y = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (first + i >= n_parts) n[i] = 0;
-        f += n[i] > 0 && n[i] <= kFew, y += n[i] > kFew;
+    // ---- the cut rows, in the order of the parts that begin them: 4 parts per thread
+    static_assert(kMaxParts <= kJoinThreads * 4, "one pass");
+    const int first = threadIdx.x * 4;
+    uint2 raw = make_uint2(0, 0);
+    int4 raw_rows = make_int4(0, 0, 0, 0);
+    if (first < p.max_parts) {   // the arrays are padded to 8
+        raw = *(const uint2*)(p.cut_pieces + first);
+        raw_rows = *(const int4*)(p.cut_row + first);
     }
-    int before = f | y << 16;   // of both, in the lanes before and this one
+    const int n_parts = p.head->n_parts;
+    const int row_of[4] = {raw_rows.x, raw_rows.y, raw_rows.z, raw_rows.w};
+    const unsigned n[4] = {raw.x & 0xffff, raw.x >> 16, raw.y & 0xffff, raw.y >> 16};
+    auto kind = [&](int i) { return first + i >= n_parts || n[i] == 0 ? -1 : n[i] <= kFew ? 0 : n[i] <= kSome ? 1 : 2; };
+    int a = 0, b = 0;   // few and some in one number; many
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a += kind(i) == 0 ? 1 : kind(i) == 1 ? 1 << 16 : 0, b += kind(i) == 2;
+    int a_to = a, b_to = b;   // in the lanes before and this one
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-        const int x = __shfl_up_sync(~0u, before, s);
-        if (lane >= s) before += x;
+        const int x = __shfl_up_sync(~0u, a_to, s), y = __shfl_up_sync(~0u, b_to, s);
+        if (lane >= s) a_to += x, b_to += y;
     }
-    if (lane == 31) counts[0][wid] = before & 0xffff, counts[1][wid] = before >> 16;
+    if (lane == 31) counts[0][wid] = a_to, counts[1][wid] = b_to;
     __syncthreads();
-    const int cf = counts[0][lane], cy = counts[1][lane];
-    const int n_few = __reduce_add_sync(~0u, cf), n_many = __reduce_add_sync(~0u, cy);
-    int at_few = __reduce_add_sync(~0u, lane < wid ? cf : 0) + (before & 0xffff) - f;
-    int at_many = __reduce_add_sync(~0u, lane < wid ? cy : 0) + (before >> 16) - y;
+    const int ca = counts[0][lane], cb = counts[1][lane];
+    const int a_all = __reduce_add_sync(~0u, ca), b_all = __reduce_add_sync(~0u, cb);
+    a_to += __reduce_add_sync(~0u, lane < wid ? ca : 0) - a, b_to += __reduce_add_sync(~0u, lane < wid ? cb : 0) - b;
+    const int count[3] = {a_all & 0xffff, a_all >> 16, b_all};
+    int to[3] = {a_to & 0xffff, count[0] + (a_to >> 16), count[0] + count[1] + b_to};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (n[i] > 0 && n[i] <= kFew) list[at_few++] = (uint16_t)(first + i);
-        if (n[i] > kFew) list[kMaxParts - 1 - at_many++] = (uint16_t)(first + i);
-    }
+    for (int i = 0; i < 4; ++i)
+        if (kind(i) >= 0) list[kind(i) == 0 ? to[0]++ : kind(i) == 1 ? to[1]++ : to[2]++] = make_uint2((first + i) | n[i] << 16, row_of[i]);
     __syncthreads();
 
     const int n_rows = p.n_kv * p.tiles, tiles_d = dp / 16, units = (p.piece_rows + 7) / 8 * tiles_d;
@@ -1080,32 +1113,125 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
         }
     };
 
-    // ---- rows of more than kFew pieces
-    for (int u = blockIdx.x; u < n_many * units; u += gridDim.x) {
-        const int part = list[kMaxParts - 1 - u / units], unit = u % units;
-        const int pieces = p.cut_pieces[part], row = p.cut_row[part];
+    auto join = [&](uint2 cut, int unit, int from, int every) {
         const bool real = unit / tiles_d * 8 + 2 * quad < p.piece_rows;
-        sums[wid][lane] = join_pieces(p.pieces, p.piece_floats, part, pieces, wid, kJoinWarps,
-                                      2 * (unit / tiles_d * 8 + 2 * quad), kPieceHead + (unit * 32 + lane) * 4, real);
-        __syncthreads();
-        if (wid == 0) {
-            Joined j = sums[0][lane];
-            for (int i = 1; i < kJoinWarps; ++i) {
-                const Joined& k = sums[i][lane];
-                join_add(j, make_float4(k.top[0], k.l[0], k.top[1], k.l[1]), k.x);
+        return join_pieces(p, cut.x & 0xffff, cut.x >> 16, from, every, 2 * (unit / tiles_d * 8 + 2 * quad),
+                           kPieceHead + (unit * 32 + lane) * 4, real);
+    };
+    // ---- rows of many pieces, by the CTA: weights of all heads first, then the sums
+    for (int u = blockIdx.x; u < count[2] * units; u += gridDim.x) {
+        const uint2 cut = list[count[0] + count[1] + u / units];
+        const int part = cut.x & 0xffff, pieces = cut.x >> 16, unit = u % units, h0 = unit / tiles_d * 8;
+        const bool real = h0 + 2 * quad < p.piece_rows;
+        const int head = wid / 4, slot = threadIdx.x % 128;   // of the weights: a head, and every 128th piece
+        float top = -INFINITY, l = 0.f;                       // of that head
+        Joined j{{0.f, 0.f}, {0.f, 0.f}, make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int k0 = 0; k0 < pieces; k0 += kChunk) {
+            float2 ml[kChunk / 128];
+            float t = top;
+#pragma unroll
+            for (int i = 0; i < kChunk / 128; ++i) {
+                const int k = k0 + slot + 128 * i;
+                ml[i] = k < pieces && h0 + head < p.piece_rows ? *(const float2*)(piece_at(p, part, k) + 2 * (h0 + head))
+                                                               : make_float2(-INFINITY, 0.f);
+                t = fmaxf(t, ml[i].x);
             }
-            finish(row, unit, j);
+#pragma unroll
+            for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, s));
+            __syncthreads();
+            if (lane == 0) sh.red[head][wid % 4] = t;
+            __syncthreads();
+            t = fmaxf(fmaxf(sh.red[head][0], sh.red[head][1]), fmaxf(sh.red[head][2], sh.red[head][3]));
+            const float old = exp2_fast(top - base_of(t));
+            top = t;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < kChunk / 128; ++i) {
+                const float f = exp2_fast(ml[i].x - base_of(t));
+                sh.weight[head][slot + 128 * i] = f;
+                l += f * ml[i].y;
+            }
+            __syncthreads();
+            // the sums so far, at the new reference
+            float now[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                now[i] = fmaxf(fmaxf(sh.red[2 * quad + i][0], sh.red[2 * quad + i][1]), fmaxf(sh.red[2 * quad + i][2], sh.red[2 * quad + i][3]));
+                const float f = k0 ? exp2_fast(j.top[i] - base_of(now[i])) : 0.f;
+                j.top[i] = now[i];
+                if (i == 0) j.x.x *= f, j.x.z *= f;
+                if (i == 1) j.x.y *= f, j.x.w *= f;
+            }
+            const int end = min(kChunk, pieces - k0);
+            for (int i0 = wid; i0 < end; i0 += kJoinWarps * 2 * kBatch) {
+                float4 x[2 * kBatch];
+#pragma unroll
+                for (int i = 0; i < 2 * kBatch; ++i) {
+                    const int k = i0 + i * kJoinWarps;
+                    x[i] = k < end && real ? *(const float4*)(piece_at(p, part, k0 + k) + kPieceHead + (unit * 32 + lane) * 4)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * kBatch; ++i) {
+                    const int k = min(i0 + i * kJoinWarps, kChunk - 1);
+                    const float f = sh.weight[2 * quad][k], g = sh.weight[2 * quad + 1][k];
+                    if (i0 + i * kJoinWarps < end)
+                        j.x.x += x[i].x * f, j.x.y += x[i].y * g, j.x.z += x[i].z * f, j.x.w += x[i].w * g;
+                }
+            }
         }
+        // the heads' sums, then the warps' columns
+#pragma unroll
+        for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(~0u, l, s);
         __syncthreads();
+        if (lane == 0) sh.red[head][wid % 4] = l;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            j.l[i] = (sh.red[2 * quad + i][0] + sh.red[2 * quad + i][1]) + (sh.red[2 * quad + i][2] + sh.red[2 * quad + i][3]);
+        __syncthreads();
+        for (int half = kJoinWarps / 2; half; half /= 2) {
+            if (wid >= half && wid < 2 * half) sh.sums[wid - half][lane].x = j.x;
+            __syncthreads();
+            if (wid < half) {
+                const float4 x = sh.sums[wid][lane].x;
+                j.x.x += x.x, j.x.y += x.y, j.x.z += x.z, j.x.w += x.w;
+            }
+            __syncthreads();
+        }
+        if (wid == 0) finish(cut.y, unit, j);
     }
-
-    // ---- the others
-    for (int u = blockIdx.x * kJoinWarps + wid; u < n_few * units; u += gridDim.x * kJoinWarps) {
-        const int part = list[u / units], unit = u % units;
-        const int pieces = p.cut_pieces[part], row = p.cut_row[part];
-        const bool real = unit / tiles_d * 8 + 2 * quad < p.piece_rows;
-        finish(row, unit, join_pieces(p.pieces, p.piece_floats, part, pieces, 0, 1,
-                                      2 * (unit / tiles_d * 8 + 2 * quad), kPieceHead + (unit * 32 + lane) * 4, real));
+    // ---- of some: by groups of warps; two groups share a place for their sums, in turn
+    {
+        const int group = wid / kGroup, per = kJoinWarps / kGroup;
+        for (int u0 = blockIdx.x * per; u0 < count[1] * units; u0 += gridDim.x * per) {
+            const int u = u0 + group;
+            const bool here = u < count[1] * units;
+            Joined j;
+            uint2 cut = make_uint2(0, 0);
+            if (here) cut = list[count[0] + u / units], j = join(cut, u % units, wid % kGroup, kGroup);
+            for (int turn = 0; turn < 2; ++turn) {
+                const bool on = here && group % 2 == turn;
+                if (on) sh.sums[group / 2 * kGroup + wid % kGroup][lane] = j;
+                __syncthreads();
+                if (on && wid % kGroup == 0) {
+                    float4 ml[kGroup - 1], x[kGroup - 1];
+#pragma unroll
+                    for (int i = 1; i < kGroup; ++i) {
+                        const Joined& k = sh.sums[group / 2 * kGroup + i][lane];
+                        ml[i - 1] = make_float4(k.top[0], k.l[0], k.top[1], k.l[1]), x[i - 1] = k.x;
+                    }
+                    join_add<kGroup - 1>(j, ml, x);
+                    finish(cut.y, u % units, j);
+                }
+                __syncthreads();
+            }
+        }
+    }
+    // ---- of few
+    for (int u = blockIdx.x * kJoinWarps + wid; u < count[0] * units; u += gridDim.x * kJoinWarps) {
+        const uint2 cut = list[u / units];
+        finish(cut.y, u % units, join(cut, u % units, 0, 1));
     }
 }
 
@@ -1156,15 +1282,19 @@ EncodeTiled encode_tiled() {
     }
     return fn;
 }
-// [pages][heads][slots][dim] with a box of p.box slots x 64 columns
+// [pages][heads][tiles of 64 columns][slots][columns] with a box of p.box slots and
+// p.box_tiles tiles; with one tile the columns are the whole head and TMA fills
+// with zeros what lies past it
 bool cache_map(CUtensorMap* map, const void* base, int type, const AttendParams& p, size_t page, size_t slot, size_t head) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+    const bool all = p.box_tiles > 1;
+    const cuuint64_t dims[5] = {(cuuint64_t)(all ? 64 : p.dim), (cuuint64_t)p.page_size, (cuuint64_t)p.box_tiles,
+                                (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
     // the stride of a dimension of one is never used, whatever the caller's
-    const cuuint64_t strides[3] = {p.page_size == 1 ? 16 : slot, p.n_kv == 1 ? 16 : head, p.n_pages == 1 ? 16 : page};
-    const cuuint32_t box[4] = {64, (cuuint32_t)p.box, 1, 1}, ones[4] = {1, 1, 1, 1};
-    return encode(map, type == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+    const cuuint64_t strides[4] = {p.page_size == 1 ? 16 : slot, 128, p.n_kv == 1 ? 16 : head, p.n_pages == 1 ? 16 : page};
+    const cuuint32_t box[5] = {64, (cuuint32_t)p.box, (cuuint32_t)p.box_tiles, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    return encode(map, type == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                   const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1190,6 +1320,7 @@ int launch(AttendParams p, cudaStream_t st) {
     const int type = kF16 ? SB_F16 : SB_BF16;
     p.box = 16;
     while (p.page_size % p.box) p.box /= 2;
+    p.box_tiles = p.box == 16 && p.dim == S::kTiles * 64 ? S::kTiles : 1;
     CUtensorMap kmap{}, vmap{};
     if (p.n_pages > 0 && (!cache_map(&kmap, p.k, type, p, p.k_page, p.k_slot, p.k_head) ||
                           !cache_map(&vmap, p.v, type, p, p.v_page, p.v_slot, p.v_head))) {

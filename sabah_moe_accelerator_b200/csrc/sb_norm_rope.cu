@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kMaxDim = 256, kMaxAxes = 4;
 
 struct NormRopeParams {
@@ -61,7 +61,7 @@ struct alignas(sizeof(T) * W) Chunk {
 
 // LPR lanes per row, NP chunk pairs of W values per lane, ITER rows per lane group
 template <class Act, class Cache, int W, int LPR, int NP, int ITER>
-__global__ void __launch_bounds__(kWarps * 32) k_norm_rope(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_constant__ NormRopeParams p) {
     constexpr int kRows = 32 / LPR;
     const unsigned task = blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR;

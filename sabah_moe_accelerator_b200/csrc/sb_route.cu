@@ -16,6 +16,8 @@
 // largest of the 32 lanes' largest keys is a key that at least n_used logits
 // reach, and few more do (about 13 of 512 for the 10 largest). Those are
 // gathered one per lane, and each lane counts how many beat its own: its rank.
+// 16-bit logits are compared two to a register, and (key, expert) of a gathered
+// one fits 32 bits, which the warp sorts.
 // Where more than 32 logits reach the bound (many equal ones), the warp takes
 // the largest n_used times instead.
 #include <cuda_bf16.h>
@@ -38,8 +40,8 @@ struct RouteParams {
     float* w;
 };
 
-// Larger float <=> larger key. 0 is free for "taken" and "none"; a NaN is
-// below -inf once sink_nan() has seen it.
+// Larger float <=> larger key. 0 stands for "taken" and "none"; a NaN is below
+// -inf once sink_nan() has seen it (until then it may have any key, 0 too).
 __device__ inline uint32_t order_key(float f) {
     const int u = __float_as_int(f + 0.f);   // -0 ties with +0
     return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
@@ -48,7 +50,7 @@ __device__ inline float key_value(uint32_t k) {
     return k == 1 ? __int_as_float(0x7fc00000) : __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 __device__ inline uint32_t sink_nan(uint32_t k) {   // beyond the keys of +-inf lie the NaNs
-    return k > 0xff800000u || (k && k < 0x007fffffu) ? 1 : k;
+    return k > 0xff800000u || k < 0x007fffffu ? 1 : k;
 }
 
 // NV: logits per lane (n_experts <= 32 * NV), V of them side by side
@@ -79,7 +81,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
         nan = false;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            key[i] = sink_nan(key[i]);
+            if (expert(i) < p.n_experts) key[i] = sink_nan(key[i]);
             nan |= key[i] == 1;
         }
         nan = __any_sync(~0u, nan);
@@ -175,12 +177,143 @@ __global__ void __launch_bounds__(kWarps * 32) k_route(const __grid_constant__ R
     }
 }
 
+// descending over the lanes
+__device__ inline uint32_t sort_lanes(uint32_t v, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k / 2; j; j >>= 1) {
+            const uint32_t x = __shfl_xor_sync(~0u, v, j);
+            v = ((lane & k) == 0) == ((lane & j) == 0) ? max(v, x) : min(v, x);
+        }
+    return v;
+}
+
+// 16-bit logits in rows of whole 16-byte chunks: as above, in 16-bit keys
+template <class Act, int NV>
+__global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_route16(const __grid_constant__ RouteParams p) {
+    constexpr bool kF16 = std::is_same<Act, __half>::value;
+    using Act2 = typename std::conditional<kF16, __half2, __nv_bfloat162>::type;
+    using Mask = typename std::conditional<NV <= 32, uint32_t, unsigned long long>::type;   // a bit per logit
+    constexpr uint32_t kInf = kF16 ? 0xfc00 : 0xff80, kNegInf = kF16 ? 0x03ff : 0x007f;   // keys of +-inf
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, t = blockIdx.x * kWarps + wid;
+    __shared__ uint32_t picked[kWarps][32];
+    if (t >= p.n_tokens) return;
+    const uint4* row = (const uint4*)(p.x + (size_t)t * p.row_stride);
+    auto expert = [&](int i) { return (i / 8 * 32 + lane) * 8 + i % 8; };
+    auto value = [&](uint32_t k) {
+        const uint16_t u = k >> 15 ? k & 0x7fff : ~k;
+        return k == 1 ? __int_as_float(0x7fc00000) : sb_to_float(*(const Act*)&u);
+    };
+    uint4 raw[NV / 8];
+#pragma unroll
+    for (int c = 0; c < NV / 8; ++c)
+        raw[c] = expert(8 * c) < p.n_experts ? __ldg(row + c * 32 + lane) : make_uint4(0, 0, 0, 0);
+    uint32_t key[NV / 2];   // two each; pairs beyond the experts stay 0
+    Act2 odd = Act2(sb_from_float<Act>(0.f), sb_from_float<Act>(0.f));
+    const Act2 zero = odd;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) {
+        const uint32_t u = ((const uint32_t*)raw)[i];
+        odd = __hfma2(*(const Act2*)&u, zero, odd);        // a NaN once a NaN or an infinity went in
+        const Act2 plus = __hadd2(*(const Act2*)&u, zero);   // -0 ties with +0
+        const uint32_t v = *(const uint32_t*)&plus;
+        key[i] = expert(2 * i) < p.n_experts ? v ^ ((v >> 15 & 0x10001u) * 0x7fffu + 0x80008000u) : 0;
+    }
+    bool nan = __any_sync(~0u, *(const uint32_t*)&odd & 0x7fff7fffu);
+    if (nan) {   // only then the keys are looked at one by one
+        nan = false;
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i) {
+            if (expert(2 * i) >= p.n_experts) continue;
+            uint32_t lo = key[i] & 0xffff, hi = key[i] >> 16;
+            if (lo > kInf || lo < kNegInf) lo = 1, nan = true;
+            if (hi > kInf || hi < kNegInf) hi = 1, nan = true;
+            key[i] = hi << 16 | lo;
+        }
+        nan = __any_sync(~0u, nan);
+    }
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) top = __vmaxu2(top, key[i]);
+    const uint32_t sorted = sort_lanes(max(top & 0xffff, top >> 16), lane);
+    const uint32_t bound = max(__shfl_sync(~0u, sorted, p.n_used - 1), 1u);   // 1: fewer lanes with logits than choices
+    const float m = value(__shfl_sync(~0u, sorted, 0));
+    float total = 0.f;   // of all, where the weights are over all experts
+    if (!p.renorm) {
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i)
+            if (key[i]) total += __expf(value(key[i] & 0xffff) - m) + __expf(value(key[i] >> 16) - m);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    }
+    // who reaches the bound, as (key, 65535 - expert): larger is earlier
+    Mask mask = 0;
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) {
+        if ((key[i] & 0xffff) >= bound) mask |= Mask(1) << (2 * i);
+        if (key[i] >= bound << 16) mask |= Mask(1) << (2 * i + 1);
+    }
+    const int here = __popcll(mask);
+    int upto = here;   // in the lanes before and this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    const int n = __shfl_sync(~0u, upto, 31);
+    uint32_t mine = 0;
+    if (n <= 32) {
+        uint32_t* next = &picked[wid][upto - here];
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i) {
+            if (mask >> (2 * i) & 1) *next++ = key[i] << 16 | (0xffff - expert(2 * i));
+            if (mask >> (2 * i + 1) & 1) *next++ = (key[i] & 0xffff0000u) | (0xffff - expert(2 * i + 1));
+        }
+        __syncwarp();
+        mine = sort_lanes(lane < n ? picked[wid][lane] : 0, lane);
+    } else {
+        mask = 0;   // taken
+        for (int j = 0; j < p.n_used; ++j) {
+            uint32_t best = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t k = i & 1 ? key[i / 2] & 0xffff0000u : key[i / 2] << 16;
+                if (k && !(mask >> i & 1)) best = max(best, k | (0xffff - expert(i)));
+            }
+            const uint32_t k = __reduce_max_sync(~0u, best);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (expert(i) == 0xffff - (int)(k & 0xffff)) mask |= Mask(1) << i;
+            if (lane == j) mine = k;
+        }
+    }
+    const bool chosen = lane < p.n_used;
+    const float v = chosen ? expf(value(mine >> 16) - m) : 0.f;
+    if (p.renorm) {
+        total = v;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    }
+    float w = p.scale * (v / total);
+    if (m == -INFINITY) w = 0.f;   // the same rules as above
+    if (nan) w = __int_as_float(0x7fc00000);
+    if (chosen) {
+        p.ids[(size_t)t * p.n_used + lane] = 0xffff - (int)(mine & 0xffff);
+        p.w[(size_t)t * p.n_used + lane] = w;
+    }
+}
+
 template <class Act, int NV>
 void launch_width(const RouteParams& p, bool wide, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(Act) < NV ? 16 / sizeof(Act) : NV;
     const int grid = (p.n_tokens + kWarps - 1) / kWarps;
-    if (wide && p.n_experts % V == 0)
-        k_route<Act, NV, V><<<grid, kWarps * 32, 0, st>>>(p);
+    if constexpr (sizeof(Act) == 2)
+        if (wide && p.n_experts % 8 == 0) {
+            k_route16<Act, (NV < 8 ? 8 : NV)><<<grid, kWarps * 32, 0, st>>>(p);
+            return;
+        }
+    if (sizeof(Act) == 4 && wide && p.n_experts % 4 == 0)
+        k_route<Act, NV, 4><<<grid, kWarps * 32, 0, st>>>(p);
     else
         k_route<Act, NV, 1><<<grid, kWarps * 32, 0, st>>>(p);
 }
