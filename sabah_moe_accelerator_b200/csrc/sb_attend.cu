@@ -15,22 +15,21 @@
 // would be padding, and tcgen05's 128 rows would be 87-99% of it.
 //
 // The work is a list of steps of 32 keys over all (sequence, key-value head)
-// rows, cut into equal parts whatever the lengths: one long sequence spreads
-// over the whole chip, and many short ones stay whole within a warp. Each warp
-// has one part of its own; where parts are long they cover 13/16 of the list,
-// and the rest is small parts that warps take as they finish, because SMs do
-// not all get the same share of the bandwidth. Warps never wait for one
-// another; each streams its own keys and values through its own ring in shared
-// memory, filled by TMA: boxes of as many rows as divide both a page and 16, in
-// tiles of 64 columns in the 128-byte swizzle that lets ldmatrix meet no bank
-// twice; one box has all tiles of 16 rows where whole tiles make up a row.
-// Rows of a box past the window's ends are masked (keys) or zeroed (values),
-// so that nothing they hold counts. A row of the list that ends in a
-// part is left as (m, l, unnormalised out) in the workspace, and a second,
-// small launch (a programmatic dependent of the first) joins the pieces of each
-// cut row in the order of its keys, so results do not depend on who took which
-// part. Rows of at most kWhole steps are never cut; where the block table
-// cannot hold a longer sequence the second launch is left out.
+// rows, cut into equal parts, one per warp, whatever the lengths: one long
+// sequence spreads over the whole chip, and many short ones stay whole within a
+// warp. Warps never wait for one another; each streams its own keys and values
+// through its own ring in shared memory, filled by TMA: boxes of as many rows as
+// divide both a page and 16, in tiles of 64 columns in the 128-byte swizzle that
+// lets ldmatrix meet no bank twice; one box has all tiles of 16 rows where whole
+// tiles make up a row. Rows of a box past the window's ends are masked (keys) or
+// zeroed (values), so that nothing they hold counts. A row of the list that ends
+// in another part is left as (m, l, unnormalised out) in the workspace, and a
+// second, small launch (a programmatic dependent of the first) joins the pieces
+// of each cut row in the order of its keys. Rows of at most kWhole steps are
+// never cut; where the block table cannot hold a longer sequence the second
+// launch is left out. (Smaller last parts, taken by the warps that finish first,
+// measured slower: 106 us against 98 on 64 ragged sequences of to 8192 keys,
+// 8 key-value heads of 128: a part's start and end cost more than the waiting.)
 //
 // Precision: scores, m, l and out are fp32. The MMA takes 16-bit factors, so
 // fp32 queries and the softmax weights are split into a sum of 16-bit parts
@@ -46,7 +45,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "sb_act.cuh"
 #include "sb_kernels.h"
@@ -57,19 +55,11 @@ constexpr int kMaxDim = 256;
 constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in shared memory
 constexpr int kStep = 32;        // keys per step
 constexpr int kWhole = 4;        // rows of at most this many steps are never cut
-constexpr int kMinSteps = 2;     // and a part is at least this long
-constexpr int kRowCost = 1;      // what a row costs besides its steps, in steps
-constexpr int kShare = 16;       // steps per warp from which the last 3/16 are shared out
-constexpr int kMaxWarps = 148 * 8, kMaxParts = 3 * kMaxWarps;
+constexpr int kMinSteps = 1;     // and a part is at least this long
+constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps
+constexpr int kMaxWarps = 148 * 8;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr float kLazy = 4.f;     // how far, in powers of two, a score may exceed the reference
-
-// The head of the workspace; the arrays of the parts follow.
-struct Header {
-    unsigned long long ready;    // the call's number, once `next` is zero
-    int next;                    // the next shared part
-    int n_parts;
-};
 
 struct AttendParams {
     const uint8_t* q;
@@ -90,14 +80,11 @@ struct AttendParams {
     uint8_t* out;
     float* lse;
     int* err;
-    int share;              // parts may be shared out
-    unsigned long long call;
-    Header* head;
-    uint16_t* cut_pieces;   // per part: the pieces of the row cut in it (0: none)
+    uint16_t* cut_pieces;   // per warp: the pieces of the row that is cut at its part's end (0: none)
     int* cut_row;           // and which row
-    float* pieces;          // per part two: the row it enters in the middle of, the row it leaves early
+    float* pieces;          // per warp two: the row it enters in the middle of, the row it leaves early
     float* sums;            // per warp one: its rounded sums, where registers have no room for them
-    int piece_floats, piece_rows, max_parts;
+    int piece_floats, piece_rows;
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -208,36 +195,11 @@ __device__ inline int div_fast(int a, int b) {
     q -= q * b > a;
     return q + (a - q * b >= b);
 }
-// The parts: n_own of `own` places, one per warp, then shared ones of `small`.
-struct Parts {
-    int cost, own, own_end, small, n_own, n;
-    __device__ Parts(int cost_, int warps, bool share) : cost(cost_) {
-        own = max(div_fast(cost + warps - 1, warps), kMinSteps);
-        if (share && own >= kShare) {
-            own = own * 13 / 16;
-            n_own = warps;
-            own_end = own * warps;
-            small = max(div_fast(cost - own_end + 2 * warps - 1, 2 * warps), kMinSteps);
-            n = n_own + div_fast(cost - own_end + small - 1, small);
-        } else {
-            n = n_own = div_fast(cost + own - 1, own);
-            own_end = cost;
-            small = 1;
-        }
-    }
-    __device__ int begin(int i) const { return i < n_own ? i * own : own_end + (i - n_own) * small; }
-    __device__ int end(int i) const { return i < n_own ? min((i + 1) * own, own_end) : min(own_end + (i + 1 - n_own) * small, cost); }
-    __device__ int of(int at) const {
-        return at < own_end ? div_fast(at, own) : n_own + div_fast(at - own_end, small);
-    }
-};
-
 // A place in the list; each warp has one that loads and one that computes.
 struct Cursor {
     int b, h;            // sequence, row of it (key-value head and tile)
     int j, end, steps;   // step in the row, where the part leaves it, the row's steps
     int len, lo;
-    int part;
     int row_at, until;   // the row's first place in the list, the part's end
 };
 // starts the row at c.b, c.h, from its step j on
@@ -259,11 +221,10 @@ __device__ inline bool next_row(Cursor& c, const Seqs& s, const AttendParams& p)
     enter_row(c, s, p, 0);
     return true;
 }
-// the first step of a part; b = -1 where the part has none of its own
-__device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, int from, int until, int part, int lane) {
+// the first step of the part [from, until); b = -1 where it has none of its own
+__device__ inline Cursor enter_part(const Seqs& s, const AttendParams& p, int from, int until, int lane) {
     const int n_rows = p.n_kv * p.tiles;
     Cursor c;
-    c.part = part;
     c.until = until;
     int a = 0, span = p.n_seqs;   // the last sequence that starts at or before `from` is in [a, a + span)
     while (span > 1) {            // 32 probes at a time
@@ -289,31 +250,30 @@ __device__ __noinline__ Cursor enter_part(const Seqs s, const AttendParams& p, i
 // been read. Block table entries are held 32 to a register, one per lane, and
 // the register after the current one is always on its way, as are the first
 // entries of this sequence (the next key-value head starts there again) and of
-// the next. Row starts go to the computing side through a small queue.
-constexpr int kQueue = 8;   // row starts between the two: at most one per two slots, and one
-
+// the next.
 template <int DP>
 struct Loader {
     using S = Shape<DP>;
     const AttendParams& p;
     const CUtensorMap *kmap, *vmap;
     const Seqs& seqs;
-    const Parts& parts;
     const int lane;
     const uint32_t ring, bars;
     const unsigned long long policy;
-    int4* queue;
     Cursor c;
-    bool more = true, asked = false, values = false;   // values: the next slot is the step's values
-    int claimed = 0, pushed = 0;
+    bool more = true, values = false;   // values: the next slot is the step's values
     uint32_t bad = 0, dirty = 0;        // bits per slot: the step met a page out of range; zeros were stored to it
     int first, cur, next, start, ahead; // cur: table entries first ..; next: the 32 after them
     int page = -1, row = 0;             // lane i: where box i of the step lies; page -1: it is not loaded
 
-    __device__ Loader(const AttendParams& p_, const CUtensorMap* km, const CUtensorMap* vm, const Seqs& s_, const Parts& parts_,
-                      int lane_, uint32_t ring_, uint32_t bars_, int4* queue_, const Cursor& c_)
-        : p(p_), kmap(km), vmap(vm), seqs(s_), parts(parts_), lane(lane_), ring(ring_), bars(bars_), policy(pass_through()), queue(queue_), c(c_) {
-        begin_part();
+    __device__ Loader(const AttendParams& p_, const CUtensorMap* km, const CUtensorMap* vm, const Seqs& s_, int lane_,
+                      uint32_t ring_, uint32_t bars_, const Cursor& c_)
+        : p(p_), kmap(km), vmap(vm), seqs(s_), lane(lane_), ring(ring_), bars(bars_), policy(pass_through()), c(c_) {
+        first = entry_of((c.lo / kStep + c.j) * kStep);
+        cur = entries(c.b, first);
+        next = entries(c.b, first + 32);
+        start = first_entries(c.b);
+        ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
     }
     __device__ int entry_of(int key) const {
         return p.page_shift >= 0 ? key >> p.page_shift : (int)((unsigned)key / (unsigned)p.page_size);
@@ -328,63 +288,18 @@ struct Loader {
         const int lo = window_start(max(seqs.len[b], 0), p.window);
         return entries(b, entry_of(lo / kStep * kStep));
     }
-    __device__ void push() {
-        queue[pushed++ % kQueue] = make_int4(c.b, c.h, c.j, c.part);   // every lane writes, and reads its own
-    }
-    __device__ void begin_part() {
-        first = entry_of((c.lo / kStep + c.j) * kStep);
-        cur = entries(c.b, first);
-        next = entries(c.b, first + 32);
-        start = first_entries(c.b);
-        ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
-        push();
-    }
-    // A shared part's number is asked for some steps before it is needed. The
-    // count starts at zero once a warp of the first CTA has said so; a warp
-    // that does not see that yet leaves the parts to others, to that CTA's
-    // warps at least, which have seen it before they start (and have parts of
-    // their own: one of at least kShare * 13 / 16 places holds a row's start).
-    __device__ void ask() {
-        asked = true;
-        claimed = kMaxParts;
-        if (lane == 0) {
-            unsigned long long r;
-            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(r) : "l"(&p.head->ready) : "memory");
-            if (r == p.call) claimed = atomicAdd(&p.head->next, 1);
-        }
-    }
     __device__ void advance() {
-        ++c.j;
-        if (parts.n > parts.n_own && !asked && c.until - c.row_at - c.j <= 2) ask();
-        if (c.j < c.end) return;
+        if (++c.j < c.end) return;
         const int b = c.b;
         more = next_row(c, seqs, p);
-        if (more) {
-            if (c.b != b) {
-                start = ahead;
-                ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
-            }
-            first = entry_of(c.lo / kStep * kStep);
-            cur = start;
-            next = entries(c.b, first + 32);
-            push();
-            return;
+        if (!more) return;
+        if (c.b != b) {
+            start = ahead;
+            ahead = c.b + 1 < p.n_seqs ? first_entries(c.b + 1) : -1;
         }
-        while (parts.n > parts.n_own) {
-            if (!asked) ask();
-            asked = false;
-            const int i = __shfl_sync(~0u, claimed, 0);
-            if (i >= parts.n - parts.n_own) break;
-            const int part = parts.n_own + i;
-            if (lane == 0) p.cut_pieces[part] = 0;
-            const Cursor at = enter_part(seqs, p, parts.begin(part), parts.end(part), part, lane);
-            if (at.b >= 0) {
-                c = at;
-                more = true;
-                begin_part();
-                break;
-            }
-        }
+        first = entry_of(c.lo / kStep * kStep);
+        cur = start;
+        next = entries(c.b, first + 32);
     }
     // fills a slot with the next keys or values
     __device__ void issue(int slot) {
@@ -511,8 +426,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     const int rows = min(p.group, 16), q_rows = NT == 1 ? 0 : rows * QP;
     uint8_t* q_mem = smem + n_warps * S::kSlots * S::kSlot + wid * q_rows * kQRow;
     uint8_t* tail = smem + n_warps * (S::kSlots * S::kSlot + q_rows * kQRow);
-    int4* queue = (int4*)tail + wid * kQueue;
-    tail += n_warps * kQueue * sizeof(int4);
     const uint32_t bars = smem_addr(tail) + wid * S::kSlots * 8;
     tail += n_warps * S::kSlots * 8;
     Seqs seqs{(int*)tail, (int*)tail + p.n_seqs + 1};
@@ -525,11 +438,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        p.head->next = 0;
-        asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(&p.head->ready), "l"(p.call) : "memory");
-    }
-
     // ---- the scan of the lengths
     __shared__ int warp_sum[32];
     {
@@ -564,11 +472,11 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 
     // ---- this warp's own part; neighbours in the list sit on different SMs
     const int w = wid * gridDim.x + blockIdx.x, n_rows = p.n_kv * p.tiles;
-    const Parts parts(seqs.pre[p.n_seqs] * n_rows, gridDim.x * n_warps, p.share);
-    if (w == 0 && lane == 0) p.head->n_parts = parts.n;
-    if (w >= parts.n_own) return;
+    const int cost = seqs.pre[p.n_seqs] * n_rows, all_warps = gridDim.x * n_warps;
+    const int part = max(div_fast(cost + all_warps - 1, all_warps), kMinSteps);
     if (lane == 0) p.cut_pieces[w] = 0;
-    Cursor cc = enter_part(seqs, p, parts.begin(w), parts.end(w), w, lane);
+    if (w >= div_fast(cost + part - 1, part)) return;
+    Cursor cc = enter_part(seqs, p, w * part, min(w * part + part, cost), lane);
     if (cc.b < 0) return;
 
     // ---- table entries and queries on their way, then keys and values
@@ -601,7 +509,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     };
     uint8_t* ring_mem = smem + wid * S::kSlots * S::kSlot;
     const uint32_t ring = smem_addr(ring_mem);
-    Loader<DP> loader(p, &kmap, &vmap, seqs, parts, lane, ring, bars, queue, cc);
+    Loader<DP> loader(p, &kmap, &vmap, seqs, lane, ring, bars, cc);
     fetch_queries(cc);
 #pragma unroll 1
     for (int i = 0; i < S::kSlots; ++i) loader.issue(i);
@@ -617,7 +525,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     const uint32_t k_lane = k_row * 128 + (((lane >> 4) ^ (k_row & 7)) << 4);
     const uint32_t v_lane = v_row * 128 + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
     float* sums = p.sums + (size_t)w * p.piece_floats;
-    int slot = 0, popped = 1;
+    int slot = 0;
     uint32_t parity = 0;
     for (bool live = true; live;) {
         const int tile = p.tiles == 1 ? 0 : cc.h % p.tiles, kv = p.tiles == 1 ? cc.h : cc.h / p.tiles;
@@ -890,20 +798,13 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         // ---- the end of the row, or of this part of it; the next row's queries
         // are on their way meanwhile, where there are registers for them
         const Cursor done = cc;
-        live = loader.pushed > popped;
-        if (live) {
-            const int4 s = queue[popped++ % kQueue];
-            cc.b = s.x, cc.h = s.y, cc.part = s.w;
-            cc.until = parts.end(s.w);
-            cc.row_at = seqs.pre[s.x] * n_rows + s.y * (seqs.pre[s.x + 1] - seqs.pre[s.x]);
-            enter_row(cc, seqs, p, s.z);
-            if (DP <= 128) fetch_queries(cc);
-        }
+        live = next_row(cc, seqs, p);
+        if (DP <= 128 && live) fetch_queries(cc);
         const bool whole = first_j == 0 && done.end == done.steps, none = done.len == done.lo;
-        float* piece = p.pieces + (size_t)(2 * done.part + (first_j == 0)) * p.piece_floats;
+        float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
         if (!whole && first_j == 0 && lane == 0) {
-            p.cut_row[done.part] = done.b * n_rows + done.h;
-            p.cut_pieces[done.part] = (uint16_t)(parts.of(done.row_at + done.steps - 1) - done.part + 1);
+            p.cut_row[w] = done.b * n_rows + done.h;
+            p.cut_pieces[w] = (uint16_t)(div_fast(done.row_at + done.steps - 1, part) - w + 1);
         }
         unsigned odd[2 * NT];
 #pragma unroll
@@ -1021,8 +922,8 @@ __device__ inline void join_add(Joined& j, const float4 (&ml)[N], const float4 (
         j.x.x += x[i].x * f, j.x.y += x[i].y * g, j.x.z += x[i].z * f, j.x.w += x[i].w * g;
     }
 }
-__device__ inline const float* piece_at(const AttendParams& p, int part, int k) {
-    return p.pieces + (size_t)(2 * (part + k) + (k == 0)) * p.piece_floats;
+__device__ inline const float* piece_at(const AttendParams& p, int warp, int k) {   // piece k of the row cut by this warp first
+    return p.pieces + (size_t)(2 * (warp + k) + (k == 0)) * p.piece_floats;
 }
 __device__ inline Joined join_pieces(const AttendParams& p, int part, int n, int first, int every, int heads_at, int unit_at, bool real) {
     Joined j{{-INFINITY, -INFINITY}, {0.f, 0.f}, make_float4(0.f, 0.f, 0.f, 0.f)};
@@ -1045,10 +946,10 @@ __device__ inline Joined join_pieces(const AttendParams& p, int part, int n, int
 }
 
 template <class Act>
-__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, int dp, float up) {
-    // the parts that begin a cut row, with its pieces, and the row: those of few
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ AttendParams p, int n_warps, int dp, float up) {
+    // the warps that begin a cut row, with its pieces, and the row: those of few
     // pieces, then of some, then of many
-    __shared__ uint2 list[kMaxParts];
+    __shared__ uint2 list[kMaxWarps];
     __shared__ int counts[2][kJoinWarps];
     __shared__ union {
         Joined sums[kJoinWarps / 2][32];
@@ -1060,24 +961,21 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.head->ready = 0;   // for a next call of the same number (a graph's)
 
-    // ---- the cut rows, in the order of the parts that begin them: 4 parts per thread
-    static_assert(kMaxParts <= kJoinThreads * 4, "one pass");
-    const int first = threadIdx.x * 4;
-    uint2 raw = make_uint2(0, 0);
-    int4 raw_rows = make_int4(0, 0, 0, 0);
-    if (first < p.max_parts) {   // the arrays are padded to 8
-        raw = *(const uint2*)(p.cut_pieces + first);
-        raw_rows = *(const int4*)(p.cut_row + first);
+    // ---- the cut rows, in the order of the keys: those of two warps per thread
+    static_assert(kMaxWarps <= kJoinThreads * 2, "one pass");
+    const int first = threadIdx.x * 2;
+    unsigned raw = 0;
+    int2 row_of = make_int2(0, 0);
+    if (first < n_warps) {   // the arrays are padded to 8
+        raw = *(const unsigned*)(p.cut_pieces + first);
+        row_of = *(const int2*)(p.cut_row + first);
     }
-    const int n_parts = p.head->n_parts;
-    const int row_of[4] = {raw_rows.x, raw_rows.y, raw_rows.z, raw_rows.w};
-    const unsigned n[4] = {raw.x & 0xffff, raw.x >> 16, raw.y & 0xffff, raw.y >> 16};
-    auto kind = [&](int i) { return first + i >= n_parts || n[i] == 0 ? -1 : n[i] <= kFew ? 0 : n[i] <= kSome ? 1 : 2; };
+    const unsigned n[2] = {raw & 0xffff, first + 1 < n_warps ? raw >> 16 : 0};
+    auto kind = [&](int i) { return n[i] == 0 ? -1 : n[i] <= kFew ? 0 : n[i] <= kSome ? 1 : 2; };
     int a = 0, b = 0;   // few and some in one number; many
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a += kind(i) == 0 ? 1 : kind(i) == 1 ? 1 << 16 : 0, b += kind(i) == 2;
+    for (int i = 0; i < 2; ++i) a += kind(i) == 0 ? 1 : kind(i) == 1 ? 1 << 16 : 0, b += kind(i) == 2;
     int a_to = a, b_to = b;   // in the lanes before and this one
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -1092,8 +990,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
     const int count[3] = {a_all & 0xffff, a_all >> 16, b_all};
     int to[3] = {a_to & 0xffff, count[0] + (a_to >> 16), count[0] + count[1] + b_to};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (kind(i) >= 0) list[kind(i) == 0 ? to[0]++ : kind(i) == 1 ? to[1]++ : to[2]++] = make_uint2((first + i) | n[i] << 16, row_of[i]);
+    for (int i = 0; i < 2; ++i)
+        if (kind(i) >= 0)
+            list[kind(i) == 0 ? to[0]++ : kind(i) == 1 ? to[1]++ : to[2]++] = make_uint2((first + i) | n[i] << 16, i ? row_of.y : row_of.x);
     __syncthreads();
 
     const int n_rows = p.n_kv * p.tiles, tiles_d = dp / 16, units = (p.piece_rows + 7) / 8 * tiles_d;
@@ -1250,17 +1149,15 @@ int sm_count() {
 int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 int most_warps(int dim) { return dim <= 128 ? 8 : dim <= 192 ? 5 : 4; }   // Shape<>::kWarps
 int piece_floats(int group, int dim) { return kPieceHead + (group <= 8 ? 8 : 16) * tile_width(dim); }
-// The workspace: the header, the parts' cut rows, their pieces, the warps' sums.
+// The workspace: which rows are cut, their pieces, the warps' rounded sums.
 struct Layout {
-    size_t parts, cut_pieces, cut_row, pieces, sums, bytes;
+    size_t cut_row, pieces, sums, bytes;
     Layout(int group, int dim) {
-        const size_t warps = (size_t)sm_count() * most_warps(dim);
-        parts = (3 * warps + 7) / 8 * 8;
+        const size_t warps = (size_t)sm_count() * most_warps(dim), padded = (warps + 7) / 8 * 8;
         const size_t piece = piece_floats(group, dim) * sizeof(float);
-        cut_pieces = 256;
-        cut_row = cut_pieces + parts * sizeof(uint16_t);
-        pieces = (cut_row + parts * sizeof(int) + 255) / 256 * 256;
-        sums = pieces + 2 * parts * piece;
+        cut_row = (padded * sizeof(uint16_t) + 255) / 256 * 256;
+        pieces = cut_row + (padded * sizeof(int) + 255) / 256 * 256;
+        sums = pieces + 2 * warps * piece;
         bytes = sums + warps * piece;
     }
 };
@@ -1306,7 +1203,7 @@ int launch(AttendParams p, cudaStream_t st) {
     using Act = typename std::conditional<QP == 1, Cache, float>::type;
     constexpr bool kF16 = std::is_same<Cache, __half>::value;
     const int q_rows = NT == 1 ? 0 : std::min(p.group, 16) * QP;
-    const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16) + kQueue * sizeof(int4);
+    const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16);
     const size_t seqs = 8 * (size_t)p.n_seqs + 4;
     // static shared memory (the scan's warp sums) is 128 bytes
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
@@ -1332,9 +1229,6 @@ int launch(AttendParams p, cudaStream_t st) {
     const long long longest = std::min((long long)p.table_width * p.page_size,
                                        p.window > 0 ? p.window + kStep - 1ll : 1ll << 40);
     const bool cuts = longest > kWhole * kStep;
-    static std::atomic<unsigned long long> calls{0x5361626168000001ull};
-    p.share = cuts;
-    p.call = calls.fetch_add(1);
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -1352,7 +1246,7 @@ int launch(AttendParams p, cudaStream_t st) {
     cfg.gridDim = sm_count();
     cfg.blockDim = kJoinThreads;
     cfg.dynamicSmemBytes = 0;
-    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act>, (const AttendParams)p, DP, up_of(kF16)), "attend join launch")
+    return sb_cuda_ok(cudaLaunchKernelEx(&cfg, k_attend_join<Act>, (const AttendParams)p, sm_count() * warps, DP, up_of(kF16)), "attend join launch")
                ? 0 : -1;
 }
 
@@ -1436,9 +1330,7 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     p.piece_floats = piece_floats(p.group, head_dim);
     const Layout lay(p.group, head_dim);
     uint8_t* ws = (uint8_t*)d_workspace;
-    p.head = (Header*)ws;
-    p.max_parts = (int)lay.parts;
-    p.cut_pieces = (uint16_t*)(ws + lay.cut_pieces);
+    p.cut_pieces = (uint16_t*)ws;
     p.cut_row = (int*)(ws + lay.cut_row);
     p.pieces = (float*)(ws + lay.pieces);
     p.sums = (float*)(ws + lay.sums);
