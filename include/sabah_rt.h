@@ -172,13 +172,13 @@ int sabah_qk_norm_rope(const void *d_q, size_t q_token_stride, size_t q_head_str
  * Key j is row j % page_size of page block_table[b][j / page_size], and query
  * head h reads key-value head h / (n_q_heads / n_kv_heads). The new token's own
  * key is in the cache and counted in lens[b]. head_dim is a multiple of 8 up to
- * 256. act_type is that of q and out (dense [n_seqs][n_q_heads][head_dim]): f32,
- * or the cache's type (f16 or bf16). Cache pointers and strides are multiples
- * of 16 bytes. d_lse (or NULL) gets m + ln sum p, [n_seqs][n_q_heads] floats.
- * A sequence of length 0 gives zeros and an lse of -inf. Cache rows, pages and
- * table entries outside the window are not read. A length outside
- * [0, table_width * page_size] or a page outside [0, n_pages) gives that
- * sequence NaN, and the device error word.
+ * 256. act_type is that of q and out (dense [n_seqs][n_q_heads][head_dim], 4-byte
+ * aligned): f32, or the cache's type (f16 or bf16). Cache pointers and strides
+ * are multiples of 16 bytes. d_lse (or NULL) gets m + ln sum p, [n_seqs][n_q_heads] floats.
+ * A sequence of length 0 gives zeros and an lse of -inf. Table entries outside
+ * the window are not read, and nothing that rows outside it hold counts (NaN
+ * included). A length outside [0, table_width * page_size] or a page outside
+ * [0, n_pages) gives that sequence NaN, and the device error word.
  * d_workspace holds sabah_attend_paged_workspace(...) bytes, 16-byte aligned,
  * of any content; calls that may overlap on the GPU must not share it. */
 size_t sabah_attend_paged_workspace(int n_q_heads, int n_kv_heads, int head_dim);

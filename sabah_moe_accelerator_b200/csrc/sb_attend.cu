@@ -54,7 +54,7 @@ namespace {
 constexpr int kMaxDim = 256;
 constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in shared memory
 constexpr int kStep = 32;        // keys per step
-constexpr int kWhole = 4;        // rows of at most this many steps are never cut
+constexpr int kWhole = 3;        // rows of at most this many steps are never cut
 constexpr int kMinSteps = 1;     // and a part is at least this long
 constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps
 constexpr int kMaxWarps = 148 * 8;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 
     if (lane < S::kSlots) bar_init(bars + lane * 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && p.n_pages > 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
@@ -890,12 +890,12 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 // Pieces of a cut row, in the order of the keys: weights from their m and l,
 // then the weighted sum. A unit is 8 query heads of a cut row and 16 of its
 // columns, as a lane holds them in a piece. Latency is all there is to it, so a
-// unit is joined by one warp where its row has few pieces, by 8 or by the 32 of
+// unit is joined by one warp where its row has few pieces, by 4 or by the 32 of
 // a CTA where it has more, with kBatch pieces' loads in flight together.
 constexpr int kJoinWarps = 32, kJoinThreads = kJoinWarps * 32;
-constexpr int kBatch = 4, kGroup = 8;                          // pieces in flight per warp; warps for some pieces
-constexpr int kFew = 3 * kBatch, kSome = 2 * kGroup * kBatch;   // most pieces for one warp, for kGroup
-constexpr int kChunk = 512;                                    // pieces whose weights are in shared memory
+constexpr int kBatch = 4, kGroup = 4;                      // pieces in flight per warp; warps for some pieces
+constexpr int kFew = kBatch, kSome = 2 * kGroup * kBatch;   // most pieces for one warp, for kGroup
+constexpr int kChunk = 512;                                // pieces whose weights are in shared memory
 
 // The weighted sum of pieces first, first + every, .. below n, in this lane's
 // (column, head) places, with its heads' reference and sum.
@@ -1292,13 +1292,13 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
         return -1;
     }
     if (n_pages < 0 || page_size <= 0 || table_width < 0 || window < 0 ||
-        (long long)table_width * page_size > 0x7fffffffll) {
+        (long long)table_width * page_size > 0x7fffff00ll) {   // a step past the last key is still an int
         sb_set_error("invalid attend cache (%d pages of %d, %d per sequence, window %d)", n_pages, page_size,
                      table_width, window);
         return -1;
     }
     if (n_seqs == 0) return 0;
-    if (!d_q || !d_lens || !d_out || (table_width && (!d_k_cache || !d_v_cache || !d_block_table)) ||
+    if (!d_q || !d_lens || !d_out || (table_width && !d_block_table) || (n_pages && (!d_k_cache || !d_v_cache)) ||
         ((uintptr_t)d_q | q_seq_stride | q_head_stride) % ab || (uintptr_t)d_out % 4 ||
         ((uintptr_t)d_k_cache | (uintptr_t)d_v_cache | k_page_stride | k_slot_stride | k_head_stride | v_page_stride |
          v_slot_stride | v_head_stride) % 16 ||

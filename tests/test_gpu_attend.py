@@ -333,3 +333,51 @@ def test_refusals(ops):
     torch.cuda.synchronize()
     assert rt.lib().sabah_rt_device_error() == 0
     check(ops, (q, k, v, table, lens))                           # and the next good call is good
+
+
+def test_more_sequences_than_one_launch_holds_some_of_them_long(ops):
+    """Launches of a call share the workspace one after another."""
+    lens = [(13 * i) % 60 for i in range(2500)]
+    lens[3], lens[1000], lens[1030], lens[2400] = 9000, 5000, 7001, 3333
+    check(ops, make(lens, 4, 1, 64, 16, F32, HF))
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_constant_values_keep_their_sum(ops, act, cache, dim):
+    """One warp adds up thousands of equal products: a sum that is cut off instead of rounded drifts."""
+    q, k, v, table, lens = make([3000] * 620, 4, 2, dim, 16, act, cache, q_scale=0.0)
+    v[torch.isfinite(v)] = 1.0 + 2.0 ** -6
+    out = ops.attend_paged(q, k, v, table, lens)
+    assert o.rel_l2(out, torch.full(out.shape, 1.0 + 2.0 ** -6, dtype=torch.float64)) <= o.TOL[act]
+
+
+def test_no_pages_at_all(ops):
+    z = torch.zeros(0, 16, 2, 64, dtype=BF, device="cuda")
+    q = torch.randn(3, 4, 64, device="cuda").to(BF)
+    table, lens = torch.zeros(3, 5, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    lse = torch.zeros(3, 4, device="cuda")
+    assert (ops.attend_paged(q, z, z, table, lens, lse=lse) == 0).all() and (lse == -math.inf).all()
+
+
+def test_heads_that_share_their_memory(ops):
+    q, k, v, table, lens = make([50, 900], 4, 1, 64, 16, BF, BF)
+    check(ops, (q, k.expand(-1, -1, 2, -1), v.expand(-1, -1, 2, -1), table, lens))
+
+
+def test_more_refusals(ops):
+    from sabah_moe_accelerator_b200 import rt
+    q, k, v, table, lens = make([50, 90], 4, 2, 64, 16, BF, BF)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.attend_paged(q.requires_grad_(), k, v, table, lens)
+    q = q.detach()
+    flat = torch.empty(q.numel() + 1, dtype=BF, device="cuda")
+    with pytest.raises(rt.SabahCudaError):                     # an output at an odd element
+        ops.attend_paged(q, k, v, table, lens, out=flat[1:].view(q.shape))
+    with pytest.raises(ValueError):
+        ops.attend_paged(q, k, v, table, lens, window=1 << 40)
+    wide = torch.zeros(2, 1, dtype=torch.int32, device="cuda").expand(2, 1 << 28)
+    with pytest.raises((ValueError, rt.SabahCudaError)):         # 2^32 keys per sequence
+        ops.attend_paged(q, k, v, wide, lens)
+    assert rt.lib().sabah_rt_device_error() == 0
+    check(ops, (q, k, v, table, lens))

@@ -139,3 +139,56 @@ def test_refusals(ops):
     with pytest.raises(ValueError):
         ops.route_topk(x, 4, w=torch.empty(4, 5, device="cuda"))
     check(ops, x, 4)
+
+
+@pytest.mark.parametrize("dtype", [F32, HF, BF])
+@pytest.mark.parametrize("E", [304, 512, 1024])
+def test_ties_in_whole_chunks(ops, dtype, E):
+    x = torch.zeros(7, E, dtype=dtype, device="cuda")
+    x[1, E - 40:] = 1
+    x[2, ::9] = 2
+    x[3] = torch.arange(E, device="cuda") // 50
+    x[4, 1::2] = -0.0
+    x[5, 5] = 3
+    x[5, 9:60] = 2.5
+    x[6, :33] = 1                                        # one more than lanes
+    for K in (1, 10, 32):
+        check(ops, x, K)
+        check(ops, x, K, False)
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_every_16_bit_value_ranks_where_it_belongs(ops, dtype):
+    """Subnormals, zeros and the largest values, in rows of 512."""
+    bits = torch.randperm(65536, generator=torch.Generator().manual_seed(0)).to(torch.int32)
+    x = (bits - ((bits > 32767) * 65536)).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x.float())]
+    x = x[:x.numel() // 512 * 512].view(-1, 512).cuda()
+    ids, _ = ops.route_topk(x, 32)
+    want, _ = o.route(x, 32, True)
+    assert torch.equal(ids.cpu().long(), want)
+    tiny = x.clone()
+    tiny[tiny.float().abs() > 1e-3] = 0                  # only small ones are left to choose
+    ids, _ = ops.route_topk(tiny, 32)
+    assert torch.equal(ids.cpu().long(), o.route(tiny, 32, True)[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, HF, BF])
+@pytest.mark.parametrize("E", [512, 301])
+def test_every_kind_of_nan(ops, dtype, E):
+    x = logits(6, E, dtype)
+    ints = {F32: torch.int32, HF: torch.int16, BF: torch.int16}[dtype]
+    for t, payload in enumerate((-1, torch.iinfo(ints).max)):   # all bits set, with and without the sign
+        x.view(ints)[t, 7] = payload
+        x.view(ints)[t + 2, E - 1] = payload
+    ids, w = ops.route_topk(x, 10)
+    assert w[:4].isnan().all() and not w[4:].isnan().any()
+    assert not (ids[:2] == 7).any() and not (ids[2:4] == E - 1).any() and ((ids >= 0) & (ids < E)).all()
+    x[0, 1:] = x[0, 7]                                    # one number among NaNs
+    ids, w = ops.route_topk(x, 10)
+    assert ids[0].tolist() == list(range(10)) and w[0].isnan().all()
+
+
+def test_no_gradient(ops):
+    with pytest.raises(ValueError, match="gradient"):
+        ops.route_topk(logits(2, 64, F32).requires_grad_(), 4)
