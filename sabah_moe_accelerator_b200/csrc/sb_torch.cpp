@@ -12,7 +12,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "../../include/sabah_rt.h"
 
@@ -67,7 +67,7 @@ void* stream() {
     return s ? s : (void*)1;
 }
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
-    return at::empty(sizes, like.options().dtype(type).requires_grad(false));
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);   // torch.empty without its dispatch
 }
 bool failed(int rc, const char* what) {
     if (rc == 0) return false;
