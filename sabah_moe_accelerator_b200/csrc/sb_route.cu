@@ -20,6 +20,10 @@
 // one fits 32 bits, which the warp sorts.
 // Where more than 32 logits reach the bound (many equal ones), the warp takes
 // the largest n_used times instead.
+//
+// Measured (one B200): 16384 tokens x 512 bf16 logits, the 10 largest: 13.4 us
+// (1.4 TB/s, 560 instructions a token, issue slots 71%), 35 us with n_used rounds;
+// one token: 5 us, the launch and the call.
 #include <cuda_bf16.h>
 
 #include "sb_act.cuh"
