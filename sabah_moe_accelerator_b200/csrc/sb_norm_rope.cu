@@ -18,19 +18,22 @@
 // the token's cosines once for all of them and multiplies them by the weights:
 // a turned value is then two products and one by the norm.
 //
-// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 55 us, 3.8
-// TB/s, with the issue slots 57% and 42% of the warps; the same rows only copied
-// take 35 us. What is left is the chain position -> cosines -> rows of a short
-// task, which more warps would hide and registers do not allow. Slower: 8 values
-// at a time (71 us), one or two rows per task (85, 66), tasks in a loop with the
-// next one's rows ahead (59), a CTA per token with the turn in shared memory (68).
+// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 43 us, 4.9
+// TB/s; the same rows only copied take 35 us. What is left is the chain position
+// -> cosines of a short task, which more warps would hide and registers do not
+// allow: issue slots 69%, warps 44%. The kind of row is the CTA's, so that its tests and pointers are uniform
+// (a flat index over all tasks of a token: 55 us), and place and position are read
+// before the rows (after them: 45). Slower: one, three or six rows per task (68,
+// 52, 60), 9 CTAs an SM for 8 (47); with the flat index 8 values at a time (71),
+// tasks in a loop with the next one's rows ahead (59), a CTA per token with the
+// turn in shared memory (68).
 #include "sb_act.cuh"
 #include "sb_kernels.h"
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kMaxDim = 256, kMaxAxes = 4;
+constexpr int kMaxDim = 256, kMaxAxes = 4, kMaxHeads = 16384;   // tasks of a token are a grid dimension
 
 struct NormRopeParams {
     const uint8_t *q, *k, *v;
@@ -50,7 +53,7 @@ struct NormRopeParams {
     unsigned n_slots;
     const int64_t* slots;
     int* err;
-    int q_blocks, kv_blocks, blocks;   // warp tasks of a token: for queries, for keys or values, in all
+    unsigned q_blocks, kv_blocks;   // warp tasks of a token: for queries, for keys or values
 };
 
 // W consecutive values, loaded and stored at once
@@ -70,13 +73,12 @@ struct alignas(sizeof(T) * W) Chunk {
 template <class Act, class Cache, int W, int LPR, int NP, int ITER>
 __global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_constant__ NormRopeParams p) {
     constexpr int kRows = 32 / LPR;
-    const unsigned task = blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR;
-    const int t = (int)(task / (unsigned)p.blocks);
+    // a warp per token; the kind of row and which of them are the CTA's
+    const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (t >= p.n_tokens) return;
-    int block = (int)(task - (unsigned)t * (unsigned)p.blocks);
-    const int kind = block < p.q_blocks ? 0 : block < p.q_blocks + p.kv_blocks ? 1 : 2;   // queries, keys, values
-    block -= kind == 0 ? 0 : kind == 1 ? p.q_blocks : p.q_blocks + p.kv_blocks;
+    const int kind = blockIdx.y < p.q_blocks ? 0 : blockIdx.y < p.q_blocks + p.kv_blocks ? 1 : 2;   // queries, keys, values
+    const int block = blockIdx.y - (kind == 0 ? 0 : kind == 1 ? p.q_blocks : p.q_blocks + p.kv_blocks);
     const int row0 = block * kRows * ITER + grp, rows = kind == 0 ? p.n_q : p.n_kv;
     const size_t head = kind == 0 ? p.q_head : kind == 1 ? p.k_head : p.v_head;
     const uint8_t* src = kind == 0   ? p.q + (size_t)t * p.q_token
@@ -94,7 +96,11 @@ __global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_const
         at[n][0] = cp * 2 * W >= p.dim ? -1 : split ? cp * W : cp * 2 * W;
         at[n][1] = split ? cp * W + half : cp * 2 * W + W;
     }
-    // all of the task's rows are on their way before anything waits
+    // the token's place and position, then all of the task's rows are on their
+    // way before anything waits
+    const bool plain = kind != 2 && half && !p.pair_axis;
+    const int pos = plain ? __ldg(p.positions + t) : 0;
+    const long long slot = kind != 0 && p.slots ? __ldg((const long long*)p.slots + t) : -1;
     Chunk<Act, W> raw[ITER][NP][2];
 #pragma unroll
     for (int it = 0; it < ITER; ++it)
@@ -111,16 +117,13 @@ __global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_const
     // where the rows go
     uint8_t* cache = nullptr;
     size_t cache_head = 0;
-    if (kind != 0 && p.slots) {
-        const long long slot = p.slots[t];
-        if (slot >= (long long)p.n_slots) {
-            if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
-        } else if (slot >= 0) {
-            const unsigned page = (unsigned)slot / (unsigned)p.page_size, in_page = (unsigned)slot - page * p.page_size;
-            cache_head = kind == 1 ? p.kc_head : p.vc_head;
-            cache = (kind == 1 ? p.k_cache + page * p.kc_page + in_page * p.kc_slot
-                               : p.v_cache + page * p.vc_page + in_page * p.vc_slot) + row0 * cache_head;
-        }
+    if (slot >= (long long)p.n_slots) {
+        if (lane == 0) atomicExch(p.err, SB_DERR_BAD_INDEX);
+    } else if (slot >= 0) {
+        const unsigned page = (unsigned)slot / (unsigned)p.page_size, in_page = (unsigned)slot - page * p.page_size;
+        cache_head = kind == 1 ? p.kc_head : p.vc_head;
+        cache = (kind == 1 ? p.k_cache + page * p.kc_page + in_page * p.kc_slot
+                           : p.v_cache + page * p.vc_page + in_page * p.vc_slot) + row0 * cache_head;
     }
     if (kind == 2) {
         if (cache)
@@ -153,7 +156,6 @@ __global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_const
 #pragma unroll
         for (int i = 0; i < W; ++i) cs[2 * i] = 1.f, cs[2 * i + 1] = 0.f;
         if (turned && p.pair_axis == nullptr) {
-            const int pos = p.positions[t];
             const bool out = pos < 0 || pos >= p.n_positions;
             if (out) atomicExch(p.err, SB_DERR_BAD_INDEX);
             const float* from = (const float*)(p.table + (size_t)(out ? 0 : pos) * half + pair0);
@@ -237,15 +239,15 @@ void launch(NormRopeParams p, cudaStream_t st) {
     const int per_task = 32 / LPR * ITER;
     p.q_blocks = (p.n_q + per_task - 1) / per_task;
     p.kv_blocks = (p.n_kv + per_task - 1) / per_task;
-    p.blocks = p.q_blocks + p.kv_blocks * (p.slots ? 2 : 1);
-    const long long tasks = (long long)p.n_tokens * p.blocks;
-    k_norm_rope<Act, Cache, W, LPR, NP, ITER><<<(unsigned)((tasks + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(p);
+    const dim3 grid((p.n_tokens + kWarps - 1) / kWarps, p.q_blocks + p.kv_blocks * (p.slots ? 2 : 1));
+    k_norm_rope<Act, Cache, W, LPR, NP, ITER><<<grid, kWarps * 32, 0, st>>>(p);
 }
 
 // Four rows per lane group once the rows of one would fill the chip twice over
 // (148 SMs x 64 warps): the cosines, positions and indexes are then a fourth of
-// the work (8191 tokens: 55 us; one row: 85), where few rows want all the warps
-// there are (64 tokens: 5.0 us either way, the launch).
+// the work (8191 tokens: 43 us, with one row 68; 2049 patches of 24 + 4 heads of
+// 80: 10.4 and 16.5), where few rows want all the warps there are (64 tokens: 5.0
+// us either way, the launch).
 template <class Act, class Cache, int LPR>
 void launch_wide(const NormRopeParams& p, cudaStream_t st) {
     if ((long long)p.n_tokens * (p.n_q + 2 * p.n_kv) * LPR / 32 > 2 * 148 * 64)
@@ -283,7 +285,7 @@ SABAH_API int sabah_qk_norm_rope(const void* d_q, size_t q_token_stride, size_t 
     if (!sb_op_begin(stream, &st, &err)) return -1;
     const size_t ab = sb_act_bytes(act_type), cb = sb_act_bytes(cache_type);
     const bool cache = d_slots != nullptr;
-    if (n_tokens < 0 || n_q_heads < 0 || n_kv_heads < 0 || n_q_heads > 65536 || n_kv_heads > 65536 || head_dim <= 0 ||
+    if (n_tokens < 0 || n_q_heads < 0 || n_kv_heads < 0 || n_q_heads > kMaxHeads || n_kv_heads > kMaxHeads || head_dim <= 0 ||
         head_dim > kMaxDim || head_dim % 2 || rope_dim < 0 || rope_dim > head_dim || rope_dim % 2 || !ab) {
         sb_set_error("invalid norm_rope geometry (tokens %d, heads %d / %d, head size %d of an even number to %d, "
                      "rotated %d, type %d)", n_tokens, n_q_heads, n_kv_heads, head_dim, kMaxDim, rope_dim, act_type);
