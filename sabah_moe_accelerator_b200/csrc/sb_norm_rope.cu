@@ -18,7 +18,7 @@
 // the token's cosines once for all of them and multiplies them by the weights:
 // a turned value is then two products and one by the norm.
 //
-// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 43 us, 4.9
+// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 43-45 us, 4.8
 // TB/s; the same rows only copied take 35 us. What is left is the chain position
 // -> cosines of a short task, which more warps would hide and registers do not
 // allow: issue slots 69%, warps 44%. The kind of row is the CTA's, so that its tests and pointers are uniform

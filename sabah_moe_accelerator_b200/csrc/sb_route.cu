@@ -16,14 +16,16 @@
 // largest of the 32 lanes' largest keys is a key that at least n_used logits
 // reach, and few more do (about 13 of 512 for the 10 largest). Those are
 // gathered one per lane, and each lane counts how many beat its own: its rank.
-// 16-bit logits are compared two to a register, and (key, expert) of a gathered
-// one fits 32 bits, which the warp sorts.
+// 16-bit logits are compared two to a register, the lanes' largest are sorted for
+// the bound, and (key, expert) of a gathered one fits 32 bits.
 // Where more than 32 logits reach the bound (many equal ones), the warp takes
 // the largest n_used times instead.
 //
-// Measured (one B200): 16384 tokens x 512 bf16 logits, the 10 largest: 13.4 us
-// (1.4 TB/s, 560 instructions a token, issue slots 71%), 35 us with n_used rounds;
-// one token: 5 us, the launch and the call.
+// Measured (one B200): 16384 tokens x 512 bf16 logits, the 10 largest: 12.3 us
+// (1.4 TB/s, 505 instructions a token, issue slots 69%), 35 us with n_used rounds;
+// 131,072 tokens: 76 us (1.8 TB/s; 82 with the gathered ones sorted by the warp and
+// every lane looking at all its logits to gather them); one token: 5 us, the launch
+// and the call.
 #include <cuda_bf16.h>
 
 #include "sb_act.cuh"
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
     using Mask = typename std::conditional<NV <= 32, uint32_t, unsigned long long>::type;   // a bit per logit
     constexpr uint32_t kInf = kF16 ? 0xfc00 : 0xff80, kNegInf = kF16 ? 0x03ff : 0x007f;   // keys of +-inf
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, t = blockIdx.x * kWarps + wid;
-    __shared__ uint32_t picked[kWarps][32];
+    __shared__ alignas(16) uint32_t picked[kWarps][32];
+    __shared__ uint4 kept[kWarps][NV / 8][32];   // the keys, where a lane can take one by number
     if (t >= p.n_tokens) return;
     const uint4* row = (const uint4*)(p.x + (size_t)t * p.row_stride);
     auto expert = [&](int i) { return (i / 8 * 32 + lane) * 8 + i % 8; };
@@ -223,7 +226,9 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
         odd = __hfma2(*(const Act2*)&u, zero, odd);        // a NaN once a NaN or an infinity went in
         const Act2 plus = __hadd2(*(const Act2*)&u, zero);   // -0 ties with +0
         const uint32_t v = *(const uint32_t*)&plus;
-        key[i] = expert(2 * i) < p.n_experts ? v ^ ((v >> 15 & 0x10001u) * 0x7fffu + 0x80008000u) : 0;
+        uint32_t negative;   // all ones in the halves that are
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(negative) : "r"(v));
+        key[i] = expert(2 * i) < p.n_experts ? v ^ (negative | 0x80008000u) : 0;
     }
     bool nan = __any_sync(~0u, *(const uint32_t*)&odd & 0x7fff7fffu);
     if (nan) {   // only then the keys are looked at one by one
@@ -251,6 +256,9 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
     }
+#pragma unroll
+    for (int c = 0; c < NV / 8; ++c)
+        kept[wid][c][lane] = make_uint4(key[4 * c], key[4 * c + 1], key[4 * c + 2], key[4 * c + 3]);
     // who reaches the bound, as (key, 65535 - expert): larger is earlier
     Mask mask = 0;
 #pragma unroll
@@ -267,15 +275,22 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
     }
     const int n = __shfl_sync(~0u, upto, 31);
     uint32_t mine = 0;
+    int rank = lane;
     if (n <= 32) {
         uint32_t* next = &picked[wid][upto - here];
-#pragma unroll
-        for (int i = 0; i < NV / 2; ++i) {
-            if (mask >> (2 * i) & 1) *next++ = key[i] << 16 | (0xffff - expert(2 * i));
-            if (mask >> (2 * i + 1) & 1) *next++ = (key[i] & 0xffff0000u) | (0xffff - expert(2 * i + 1));
+        for (; mask; mask &= mask - 1) {
+            const int i = sizeof(Mask) == 4 ? __ffs((int)mask) - 1 : __ffsll((long long)mask) - 1;
+            const uint32_t two = ((const uint32_t*)&kept[wid][i / 8][lane])[i % 8 / 2];
+            *next++ = (i & 1 ? two & 0xffff0000u : two << 16) | (0xffff - expert(i));
         }
+        if (lane >= n) picked[wid][lane] = 0;
         __syncwarp();
-        mine = sort_lanes(lane < n ? picked[wid][lane] : 0, lane);
+        mine = picked[wid][lane];
+        rank = mine ? 0 : p.n_used;
+        for (int j = 0; j < n; j += 4) {
+            const uint4 u = *(const uint4*)&picked[wid][j];
+            rank += (u.x > mine) + (u.y > mine) + (u.z > mine) + (u.w > mine);
+        }
     } else {
         mask = 0;   // taken
         for (int j = 0; j < p.n_used; ++j) {
@@ -292,7 +307,7 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
             if (lane == j) mine = k;
         }
     }
-    const bool chosen = lane < p.n_used;
+    const bool chosen = rank < p.n_used;
     const float v = chosen ? expf(value(mine >> 16) - m) : 0.f;
     if (p.renorm) {
         total = v;
@@ -303,20 +318,23 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 16 ? 40 / kWarps : 1) k_rou
     if (m == -INFINITY) w = 0.f;   // the same rules as above
     if (nan) w = __int_as_float(0x7fc00000);
     if (chosen) {
-        p.ids[(size_t)t * p.n_used + lane] = 0xffff - (int)(mine & 0xffff);
-        p.w[(size_t)t * p.n_used + lane] = w;
+        p.ids[(size_t)t * p.n_used + rank] = 0xffff - (int)(mine & 0xffff);
+        p.w[(size_t)t * p.n_used + rank] = w;
     }
 }
 
+// Two 16-bit logits to a register pay from 8 logits per lane on (131,072 tokens of
+// bf16, 256 experts, the 8 largest: 62 us, singly 66; 128 experts: 64, singly 56,
+// and the 2 largest of them 58 and 40).
 template <class Act, int NV>
 void launch_width(const RouteParams& p, bool wide, cudaStream_t st) {
     const int grid = (p.n_tokens + kWarps - 1) / kWarps;
-    if constexpr (sizeof(Act) == 2)
+    if constexpr (sizeof(Act) == 2 && NV > 4)
         if (wide && p.n_experts % 8 == 0) {
-            k_route16<Act, (NV < 8 ? 8 : NV)><<<grid, kWarps * 32, 0, st>>>(p);
+            k_route16<Act, NV><<<grid, kWarps * 32, 0, st>>>(p);
             return;
         }
-    if (sizeof(Act) == 4 && wide && p.n_experts % 4 == 0)
+    if (wide && p.n_experts % 4 == 0)
         k_route<Act, NV, 4><<<grid, kWarps * 32, 0, st>>>(p);
     else
         k_route<Act, NV, 1><<<grid, kWarps * 32, 0, st>>>(p);
