@@ -148,7 +148,7 @@ int sabah_rt_device_error(void);
  *   pos = positions[pair_axis ? pair_axis[i] : 0][token]
  * table is [n_positions][rope_dim / 2][2] floats, positions [n_axes][n_tokens]
  * (n_axes <= 4), pair_axis [rope_dim / 2] or NULL. head_dim is even and at most
- * 256; rope_dim is even, 0 for no rotation.
+ * 256; rope_dim is even, 0 for no rotation; at most 16384 heads of each kind.
  * q_out and k_out are dense [n_tokens][heads][head_dim] of act_type; q_out may
  * be q and k_out k where those are dense. With d_slots, k (as rotated) and v
  * (as it is) also go to row slots[t] % page_size of page slots[t] / page_size,

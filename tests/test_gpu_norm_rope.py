@@ -87,6 +87,17 @@ def test_token_counts(ops, T):
     check(ops, make(ops, T, 32 if T < 3000 else 7, 8 if T < 3000 else 1, 128, 128, BF, BF))
 
 
+@pytest.mark.parametrize("T,n_q,n_kv", [(5, 131, 9), (1, 1, 1024), (700, 50, 33)])
+def test_many_heads(ops, T, n_q, n_kv):
+    check(ops, make(ops, T, n_q, n_kv, 64, 64, BF, BF))
+
+
+@pytest.mark.parametrize("D,rope,pairing", [(64, 32, "pairs"), (80, 80, "halves"), (192, 128, "halves"), (256, 256, "pairs")])
+@pytest.mark.parametrize("act", [F32, HF])
+def test_many_rows(ops, D, rope, pairing, act):
+    check(ops, make(ops, 5003, 6, 5, D, rope, act, HF, axes=2), pairing)
+
+
 @pytest.mark.parametrize("axes", [2, 3, 4])
 @pytest.mark.parametrize("D,rope,pairing", [(80, 80, "pairs"), (128, 64, "halves"), (90, 30, "halves")])
 def test_axes(ops, axes, D, rope, pairing):
@@ -269,3 +280,13 @@ def test_refusals(ops):
     torch.cuda.synchronize()
     assert rt.lib().sabah_rt_device_error() == 0
     check(ops, a)
+
+
+def test_too_many_heads_are_refused(ops):
+    from sabah_moe_accelerator_b200 import rt
+    q = torch.zeros(1, 16385, 2, device="cuda", dtype=BF)
+    one = ops.qk_norm_rope(q[:, :16384], q[:, :16384], None, None, None, None, None)
+    assert one[0].shape == (1, 16384, 2)
+    for a, b in ((q, q[:, :4]), (q[:, :4], q)):
+        with pytest.raises(rt.SabahCudaError, match="geometry"):
+            ops.qk_norm_rope(a, b, None, None, None, None, None)

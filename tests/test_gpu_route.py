@@ -142,7 +142,7 @@ def test_refusals(ops):
 
 
 @pytest.mark.parametrize("dtype", [F32, HF, BF])
-@pytest.mark.parametrize("E", [304, 512, 1024])
+@pytest.mark.parametrize("E", [64, 124, 128, 304, 512, 1024])
 def test_ties_in_whole_chunks(ops, dtype, E):
     x = torch.zeros(7, E, dtype=dtype, device="cuda")
     x[1, E - 40:] = 1
@@ -174,7 +174,7 @@ def test_every_16_bit_value_ranks_where_it_belongs(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, HF, BF])
-@pytest.mark.parametrize("E", [512, 301])
+@pytest.mark.parametrize("E", [512, 301, 128])
 def test_every_kind_of_nan(ops, dtype, E):
     x = logits(6, E, dtype)
     ints = {F32: torch.int32, HF: torch.int16, BF: torch.int16}[dtype]
