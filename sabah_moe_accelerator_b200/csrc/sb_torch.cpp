@@ -33,19 +33,26 @@ PyObject* g_error;   // rt.SabahCudaError
         }                                             \
     } while (0)
 
-// the tensor behind an argument; null for None
-bool tensor(PyObject* o, const char* name, bool optional, at::Tensor& t) {
-    if (o == Py_None && optional) return true;
+// The tensor behind an argument, which the caller holds during the call; an
+// undefined one for None, null with the error for anything else.
+const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
+    static const at::Tensor none;
+    if (o == Py_None && optional) return &none;
     if (!THPVariable_Check(o)) {
         PyErr_Format(PyExc_ValueError, "%s: a tensor%s, not %.100s", name, optional ? " or None" : "", Py_TYPE(o)->tp_name);
-        return false;
+        return nullptr;
     }
-    t = THPVariable_Unpack(o);
-    return true;
+    return &THPVariable_Unpack(o);
 }
-#define TENSOR(t, o, optional) \
-    at::Tensor t;              \
-    if (!tensor(o, #t, optional, t)) return nullptr
+#define TENSOR(t, o, optional)                             \
+    const at::Tensor* t##_arg = tensor(o, #t, optional);   \
+    if (!t##_arg) return nullptr;                          \
+    const at::Tensor& t = *t##_arg
+// the same for an output, to be filled in where it is None
+#define OUTPUT(t, o)                                   \
+    const at::Tensor* t##_arg = tensor(o, #t, true);   \
+    if (!t##_arg) return nullptr;                      \
+    at::Tensor t = *t##_arg
 
 int act_type(const at::Tensor& t) {   // ggml's codes
     switch (t.scalar_type()) {
@@ -110,8 +117,8 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TENSOR(k_cache, a[10], true);
     TENSOR(v_cache, a[11], true);
     TENSOR(slots, a[12], true);
-    TENSOR(q_out, a[13], true);
-    TENSOR(k_out, a[14], true);
+    OUTPUT(q_out, a[13]);
+    OUTPUT(k_out, a[14]);
     const bool cache = a[12] != Py_None;
 
     NEED(q.dim() == 3 && k.dim() == 3, "q, k: [tokens, heads, head_dim]");
@@ -191,9 +198,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TENSOR(v_cache, a[2], false);
     TENSOR(block_table, a[3], false);
     TENSOR(lens, a[4], false);
-    TENSOR(out, a[7], true);
+    OUTPUT(out, a[7]);
     TENSOR(lse, a[8], true);
-    TENSOR(workspace, a[9], true);
+    OUTPUT(workspace, a[9]);
     const long window = PyLong_AsLong(a[6]);
     if (window == -1 && PyErr_Occurred()) return nullptr;
 
@@ -258,8 +265,8 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int renorm = PyObject_IsTrue(a[2]);
     const double scale = PyFloat_AsDouble(a[3]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-    TENSOR(ids, a[4], true);
-    TENSOR(w, a[5], true);
+    OUTPUT(ids, a[4]);
+    OUTPUT(w, a[5]);
     NEED(logits.dim() == 2, "logits: [tokens, experts]");
     const int64_t T = logits.size(0), E = logits.size(1), rows[] = {T, used};
     const int act = act_type(logits);
