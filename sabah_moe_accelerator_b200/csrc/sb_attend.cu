@@ -171,6 +171,8 @@ __device__ inline int exponent(float x) {
 }
 __device__ inline float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 __device__ inline bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+// the reference that a score or another reference is taken relative to
+__device__ inline float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
 // ------------------------------------------------------------ shapes
 // DP: head size rounded up to a tile width. A slot of a ring is the keys or the
@@ -369,7 +371,9 @@ __host__ __device__ inline int frag_at(int head, int col, int dp) {
 // Products of parts make NaN of what is an infinity in the formula (0 * inf,
 // inf - inf between parts). Where a row's result is not finite, its columns that
 // are not are computed again here, key by key in fp32, for this warp's keys
-// [from, to); all of them where the softmax's own sum is not finite.
+// [from, to); all of them where the softmax's own sum is not finite. A score of
+// -inf weighs nothing, also where no finite one came before it; a NaN stays one,
+// whatever the weights that follow.
 template <class Cache, class Act>
 __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int head, int from, int to, float m, float l,
                                       float up, bool whole, float* piece, int row, int dp, int lane) {
@@ -386,16 +390,16 @@ __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int 
             if (lane + 32 * i < p.dim) s += sb_to_float(q[lane + 32 * i]) * sb_to_float(k[lane + 32 * i]);
         for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
         s *= p.scale_log2;
-        const float t = fmaxf(top, s), a = top == -INFINITY ? 0.f : exp2f(top - t), e = exp2f(s - t);
+        const float t = fmaxf(top, s), a = top == -INFINITY ? 1.f : exp2f(top - t), e = exp2f(s - finite_or_zero(t));
         top = t;
         sum = sum * a + e;
         for (int i = 0; i < N; ++i)
-            if (lane + 32 * i < p.dim) o[i] = (a == 0.f ? 0.f : o[i] * a) + e * sb_to_float(v[lane + 32 * i]);
+            if (lane + 32 * i < p.dim) o[i] = o[i] * a + e * sb_to_float(v[lane + 32 * i]);
     }
     const bool all = !is_finite(l);
     const size_t at = (size_t)b * p.n_q + head;
     Act* out = (Act*)p.out + at * p.dim;
-    const float scale = all ? exp2f(up) : exp2f(top - m + up);
+    const float scale = all ? exp2f(up) : exp2f(finite_or_zero(top) - finite_or_zero(m) + up);
     for (int i = 0; i < N; ++i) {
         const int d = lane + 32 * i;
         if (d >= p.dim) break;
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                 for (int u = 0; u < NT; ++u) {
                     float base[2], sum[2] = {};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) base[i] = (m[2 * u + i] == -INFINITY ? 0.f : m[2 * u + i]) - kUp;
+                    for (int i = 0; i < 2; ++i) base[i] = finite_or_zero(m[2 * u + i]) - kUp;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
                         l_sum[x] += l[x];
                         l[x] = 0.f;
                         if constexpr (!kKeep) {   // in memory, with the reference that they were added at
-                            a[x] = folds ? exp2_fast(m_fold[x] - m[x]) : 0.f;
+                            a[x] = folds ? exp2_fast(m_fold[x] - finite_or_zero(m[x])) : 0.f;
                             m_fold[x] = m[x];
                         }
                     }
@@ -827,7 +831,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll
                 for (int s = 4; s <= 16; s <<= 1) l[x] += __shfl_xor_sync(~0u, l[x], s);
                 if (row_bad) l[x] = __int_as_float(0x7fc00000);
-                a[i] = !kKeep && folds ? exp2_fast(m_fold[x] - m[x]) : 0.f;
+                a[i] = !kKeep && folds ? exp2_fast(m_fold[x] - finite_or_zero(m[x])) : 0.f;
                 inv[i] = !whole ? 1.f : none ? 0.f : 1.f / l[x];
                 check[i] = l[x] * 0.f;   // a NaN once anything infinite or NaN went in
                 if (g == 0 && head < heads) {
@@ -913,14 +917,13 @@ struct Joined {
     float top[2], l[2];
     float4 x;
 };
-__device__ inline float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 // adds n parts to j: the common reference first, then exps that do not wait for one another
 template <int N>
 __device__ inline void join_add(Joined& j, const float4 (&ml)[N], const float4 (&x)[N]) {   // ml: (m, l) of both heads
     float top[2] = {j.top[0], j.top[1]};
 #pragma unroll
     for (int i = 0; i < N; ++i) top[0] = fmaxf(top[0], ml[i].x), top[1] = fmaxf(top[1], ml[i].z);
-    const float base[2] = {base_of(top[0]), base_of(top[1])};
+    const float base[2] = {finite_or_zero(top[0]), finite_or_zero(top[1])};
     const float old[2] = {exp2_fast(j.top[0] - base[0]), exp2_fast(j.top[1] - base[1])};
 #pragma unroll
     for (int h = 0; h < 2; ++h) j.l[h] *= old[h], j.top[h] = top[h];
@@ -1051,12 +1054,12 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
             if (lane == 0) sh.red[head][wid % 4] = t;
             __syncthreads();
             t = fmaxf(fmaxf(sh.red[head][0], sh.red[head][1]), fmaxf(sh.red[head][2], sh.red[head][3]));
-            const float old = exp2_fast(top - base_of(t));
+            const float old = exp2_fast(top - finite_or_zero(t));
             top = t;
             l *= old;
 #pragma unroll
             for (int i = 0; i < kChunk / 128; ++i) {
-                const float f = exp2_fast(ml[i].x - base_of(t));
+                const float f = exp2_fast(ml[i].x - finite_or_zero(t));
                 sh.weight[head][slot + 128 * i] = f;
                 l += f * ml[i].y;
             }
@@ -1066,7 +1069,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 now[i] = fmaxf(fmaxf(sh.red[2 * quad + i][0], sh.red[2 * quad + i][1]), fmaxf(sh.red[2 * quad + i][2], sh.red[2 * quad + i][3]));
-                const float f = k0 ? exp2_fast(j.top[i] - base_of(now[i])) : 0.f;
+                const float f = k0 ? exp2_fast(j.top[i] - finite_or_zero(now[i])) : 0.f;
                 j.top[i] = now[i];
                 if (i == 0) j.x.x *= f, j.x.z *= f;
                 if (i == 1) j.x.y *= f, j.x.w *= f;
