@@ -211,19 +211,22 @@ __global__ void __launch_bounds__(kWarps * 32, 8) k_norm_rope(const __grid_const
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if (at[n][0] < 0) continue;
+            // a value that is not turned leaves its partner's product with zero out: an
+            // infinity or NaN there is none of its business (a predicate per product; a
+            // branch for such lanes: 8191 tokens with half of each head turned 45.3 us, this 44.0)
+            const bool turned = (sub + n * LPR) * 2 * W < p.rope;
             float y[2 * W];
+            auto turn = [&](int i, int a, int b) {   // pair i, the lane's values a and b
+                float u = x[n][a] * ca[n][i], v = x[n][b] * cb[n][i];
+                if (turned) u -= x[n][b] * sb[n][i], v += x[n][a] * sa[n][i];
+                y[a] = u * inv, y[b] = v * inv;
+            };
             if (p.pairs_mode && W > 1) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    y[2 * i] = (x[n][2 * i] * ca[n][i] - x[n][2 * i + 1] * sb[n][i]) * inv;
-                    y[2 * i + 1] = (x[n][2 * i] * sa[n][i] + x[n][2 * i + 1] * cb[n][i]) * inv;
-                }
+                for (int i = 0; i < W; ++i) turn(i, 2 * i, 2 * i + 1);
             } else {
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    y[i] = (x[n][i] * ca[n][i] - x[n][i + W] * sb[n][i]) * inv;
-                    y[i + W] = (x[n][i] * sa[n][i] + x[n][i + W] * cb[n][i]) * inv;
-                }
+                for (int i = 0; i < W; ++i) turn(i, i, i + W);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
