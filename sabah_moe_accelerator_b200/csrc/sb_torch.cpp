@@ -10,6 +10,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -34,7 +35,8 @@ PyObject* g_error;   // rt.SabahCudaError
     } while (0)
 
 // The tensor behind an argument, which the caller holds during the call; an
-// undefined one for None, null with the error for anything else.
+// undefined one for None, null with the error for anything else. A wrapper (of
+// vmap, a functional transform, a dispatching subclass) has no memory of its own.
 const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
     static const at::Tensor none;
     if (o == Py_None && optional) return &none;
@@ -42,7 +44,13 @@ const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
         PyErr_Format(PyExc_ValueError, "%s: a tensor%s, not %.100s", name, optional ? " or None" : "", Py_TYPE(o)->tp_name);
         return nullptr;
     }
-    return &THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (at::isTensorSubclassLike(t)) {
+        PyErr_Format(PyExc_ValueError, "%s: a plain tensor (not inside vmap or another transform, no dispatching subclass)",
+                     name);
+        return nullptr;
+    }
+    return &t;
 }
 #define TENSOR(t, o, optional)                             \
     const at::Tensor* t##_arg = tensor(o, #t, optional);   \
@@ -75,6 +83,16 @@ void* stream() {
 }
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
     return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);   // torch.empty without its dispatch
+}
+// The ABI's call without the lock. Its arguments are values, read before the lock
+// is given up: reading a tensor may throw, and throws into Python.
+template <class F, class... A>
+int unlocked(F f, A... a) {
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(a...);
+    Py_END_ALLOW_THREADS
+    return rc;
 }
 bool failed(int rc, const char* what) {
     if (rc == 0) return false;
@@ -168,17 +186,15 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     NEED(!k_out.defined() || dense(k_out, k.scalar_type(), k.sizes(), k), "k_out: dense, as k");
     auto ptr = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
     void* st = stream();
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_norm_rope(ptr(q), eb * q.stride(0), eb * q.stride(1), (int)n_q, ptr(k), eb * k.stride(0), eb * k.stride(1),
-                     cache ? ptr(v) : nullptr, vs[0], vs[1], (int)n_kv, (int)T, (int)D, act, (const float*)ptr(q_weight),
-                     (const float*)ptr(k_weight), (float)eps, (const float*)ptr(table), (int)n_pos, (int)rope, pairs,
-                     table.defined() ? (const int32_t*)ptr(positions) : nullptr, (int)axes,
-                     table.defined() ? (const uint8_t*)ptr(pair_axis) : nullptr, ptr(q_out), ptr(k_out),
-                     cache ? ptr(k_cache) : nullptr, kc_at.page, kc_at.row, kc_at.head, cache ? ptr(v_cache) : nullptr,
-                     vc_at.page, vc_at.row, vc_at.head, cache ? (int)k_cache.size(0) : 0, cache ? (int)k_cache.size(1) : 0,
-                     cache ? act_type(k_cache) : 0, cache ? (const int64_t*)ptr(slots) : nullptr, st);
-    Py_END_ALLOW_THREADS
+    const int rc = unlocked(
+        g_norm_rope, ptr(q), eb * q.stride(0), eb * q.stride(1), (int)n_q, ptr(k), eb * k.stride(0), eb * k.stride(1),
+        cache ? ptr(v) : nullptr, vs[0], vs[1], (int)n_kv, (int)T, (int)D, act, (const float*)ptr(q_weight),
+        (const float*)ptr(k_weight), (float)eps, (const float*)ptr(table), (int)n_pos, (int)rope, pairs,
+        table.defined() ? (const int32_t*)ptr(positions) : nullptr, (int)axes,
+        table.defined() ? (const uint8_t*)ptr(pair_axis) : nullptr, ptr(q_out), ptr(k_out),
+        cache ? ptr(k_cache) : nullptr, kc_at.page, kc_at.row, kc_at.head, cache ? ptr(v_cache) : nullptr,
+        vc_at.page, vc_at.row, vc_at.head, cache ? (int)k_cache.size(0) : 0, cache ? (int)k_cache.size(1) : 0,
+        cache ? act_type(k_cache) : 0, cache ? (const int64_t*)ptr(slots) : nullptr, st);
     if (failed(rc, "sabah_qk_norm_rope")) return nullptr;
     if (cache) return THPVariable_Wrap(q_out);
     PyObject *x = THPVariable_Wrap(q_out), *y = THPVariable_Wrap(k_out);
@@ -241,15 +257,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Cache kc(k_cache), vc(v_cache);
     const size_t eb = q.element_size();
     void* st = stream();
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_attend(q.data_ptr(), eb * q.stride(0), eb * q.stride(1), act, k_cache.data_ptr(), kc.page, kc.row, kc.head,
-                  v_cache.data_ptr(), vc.page, vc.row, vc.head, act_type(k_cache), (int)k_cache.size(0), (int)k_cache.size(1),
-                  (const int32_t*)block_table.data_ptr(), 4 * (size_t)block_table.stride(0), (int)block_table.size(1),
-                  (const int32_t*)lens.data_ptr(), (int)B, (int)H, (int)n_kv, (int)D, (float)scale, (int)window,
-                  out.data_ptr(), lse.defined() ? (float*)lse.data_ptr() : nullptr, workspace.data_ptr(),
-                  workspace.numel() * workspace.element_size(), st);
-    Py_END_ALLOW_THREADS
+    const int rc = unlocked(
+        g_attend, q.data_ptr(), eb * q.stride(0), eb * q.stride(1), act, k_cache.data_ptr(), kc.page, kc.row, kc.head,
+        v_cache.data_ptr(), vc.page, vc.row, vc.head, act_type(k_cache), (int)k_cache.size(0), (int)k_cache.size(1),
+        (const int32_t*)block_table.data_ptr(), 4 * (size_t)block_table.stride(0), (int)block_table.size(1),
+        (const int32_t*)lens.data_ptr(), (int)B, (int)H, (int)n_kv, (int)D, (float)scale, (int)window,
+        out.data_ptr(), lse.defined() ? (float*)lse.data_ptr() : nullptr, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), st);
     if (failed(rc, "sabah_attend_paged")) return nullptr;
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -279,11 +293,8 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
     NEED(dense(ids, at::kInt, rows, logits) && dense(w, at::kFloat, rows, logits),
          "ids and w: dense int32 and float32 [tokens, n_used]");
     void* st = stream();
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_route(logits.data_ptr(), logits.element_size() * logits.stride(0), act, (int)T, (int)E, (int)used, renorm,
-                 (float)scale, (int32_t*)ids.data_ptr(), (float*)w.data_ptr(), st);
-    Py_END_ALLOW_THREADS
+    const int rc = unlocked(g_route, logits.data_ptr(), logits.element_size() * logits.stride(0), act, (int)T, (int)E,
+                            (int)used, renorm, (float)scale, (int32_t*)ids.data_ptr(), (float*)w.data_ptr(), st);
     if (failed(rc, "sabah_route_topk")) return nullptr;
     PyObject *x = THPVariable_Wrap(ids), *y = THPVariable_Wrap(w);
     PyObject* both = x && y ? PyTuple_Pack(2, x, y) : nullptr;
