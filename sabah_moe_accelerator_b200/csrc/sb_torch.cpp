@@ -36,7 +36,9 @@ PyObject* g_error;   // rt.SabahCudaError
 
 // The tensor behind an argument, which the caller holds during the call; an
 // undefined one for None, null with the error for anything else. A wrapper (of
-// vmap, a functional transform, a dispatching subclass) has no memory of its own.
+// vmap, a functional transform, a dispatching subclass) has no memory of its own;
+// a tensor with the negative bit, a lazy zero or a freed storage has no memory that
+// holds its values.
 const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
     static const at::Tensor none;
     if (o == Py_None && optional) return &none;
@@ -48,6 +50,10 @@ const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
     if (at::isTensorSubclassLike(t)) {
         PyErr_Format(PyExc_ValueError, "%s: a plain tensor (not inside vmap or another transform, no dispatching subclass)",
                      name);
+        return nullptr;
+    }
+    if (t.is_neg() || t._is_zerotensor() || (t.numel() && t.is_cuda() && !t.data_ptr())) {
+        PyErr_Format(PyExc_ValueError, "%s: its memory does not hold its values (a negative view, a lazy zero, a freed storage)", name);
         return nullptr;
     }
     return &t;

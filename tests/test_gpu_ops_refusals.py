@@ -67,3 +67,20 @@ def test_functional_transforms(ops, op):
         torch.func.grad(lambda t: f(t).sum())(a[name])
     call(**a)
     torch.cuda.synchronize()
+
+
+FLOATS = [(op, n) for op, n in EVERY if n not in ("positions", "slots", "block_table", "lens", "workspace", "ids")]
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_memory_that_does_not_hold_the_values(ops, op, name):
+    """A view that reads as the negative of its memory; a storage that was freed."""
+    call, a = args_of(ops)[op]
+    with pytest.raises(ValueError, match=name + ".*hold its values"):
+        call(**{**a, name: torch._neg_view(a[name])})
+    gone = a[name].clone()
+    gone.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match=name + ".*hold its values"):
+        call(**{**a, name: gone})
+    call(**a)
+    torch.cuda.synchronize()

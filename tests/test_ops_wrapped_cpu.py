@@ -77,3 +77,13 @@ def test_every_argument_is_looked_at(ops):
                 (c, c, slots)[n])
     for name, t in (("pair_axis", torch.zeros(4, dtype=torch.uint8)), ("q_out", q), ("k_out", q)):
         refused(lambda t, name=name: ops.qk_norm_rope(*args, **{name: t}), t)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_memory_that_does_not_hold_the_values_is_refused(ops, which):
+    """A view that reads as the negative of its memory; zeros without memory."""
+    f = calls(ops)[which]
+    with pytest.raises(ValueError, match="hold its values"):
+        f(torch._neg_view(torch.ones(4, 8)))
+    with pytest.raises(ValueError, match="hold its values"):
+        f(torch._efficientzerotensor((4, 8)))
