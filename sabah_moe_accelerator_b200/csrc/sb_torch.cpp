@@ -14,6 +14,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 
 #include "../../include/sabah_rt.h"
 
@@ -38,7 +39,8 @@ PyObject* g_error;   // rt.SabahCudaError
 // undefined one for None, null with the error for anything else. A wrapper (of
 // vmap, a functional transform, a dispatching subclass) has no memory of its own;
 // a tensor with the negative bit, a lazy zero or a freed storage has no memory that
-// holds its values.
+// holds its values. Nothing here has a derivative, so whatever would lose one is
+// refused too, a norm's weight or an output no less than the queries.
 const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
     static const at::Tensor none;
     if (o == Py_None && optional) return &none;
@@ -54,6 +56,14 @@ const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
     }
     if (t.is_neg() || t._is_zerotensor() || (t.numel() && t.is_cuda() && !t.data_ptr())) {
         PyErr_Format(PyExc_ValueError, "%s: its memory does not hold its values (a negative view, a lazy zero, a freed storage)", name);
+        return nullptr;
+    }
+    if (t.requires_grad() && at::GradMode::is_enabled()) {
+        PyErr_Format(PyExc_ValueError, "%s: this operator has no gradient (use torch.no_grad or detach)", name);
+        return nullptr;
+    }
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+        PyErr_Format(PyExc_ValueError, "%s: this operator has no forward gradient (unpack the dual tensor)", name);
         return nullptr;
     }
     return &t;
@@ -81,7 +91,6 @@ bool dense(const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes, cons
 }
 bool last_dense(const at::Tensor& t) { return t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1; }
 bool here(const at::Tensor& t) { return t.is_cuda() && t.device().index() == c10::cuda::current_device(); }
-bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 // the current stream; the ABI reads 0 as its own stream, so the default one is passed as cudaStreamLegacy
 void* stream() {
     void* s = c10::cuda::getCurrentCUDAStream().stream();
@@ -152,7 +161,6 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int act = act_type(q);
     NEED(act >= 0 && k.scalar_type() == q.scalar_type(), "q and k: both f32, f16 or bf16");
     NEED(here(q) && k.device() == q.device(), "q and k: on the current CUDA device");
-    NEED(!wants_grad(q) && !wants_grad(k), "q and k: this operator has no gradient (use torch.no_grad or detach)");
     NEED(last_dense(q) && last_dense(k), "q and k: head_dim must be dense");
     const int64_t row[] = {D};
     NEED(!q_weight.defined() || dense(q_weight, at::kFloat, row, q), "q_weight: dense float32 [head_dim] or None");
@@ -238,7 +246,6 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     NEED(k_cache.size(3) == D && n_kv > 0 && H % n_kv == 0, "q heads: a multiple of the cache's, of one head_dim");
     NEED(B <= 0x7fffffff && H <= 65536 && D <= 65536, "q: a dimension is too large");
     NEED(here(q), "q: on the current CUDA device");
-    NEED(!wants_grad(q), "q: this operator has no gradient (use torch.no_grad or detach)");
     NEED(last_dense(q), "q: head_dim must be dense");
     NEED(block_table.dim() == 2 && block_table.size(0) == B && block_table.size(1) <= 0x7fffffff &&
          block_table.scalar_type() == at::kInt && last_dense(block_table) && block_table.device() == q.device(),
@@ -291,7 +298,6 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t T = logits.size(0), E = logits.size(1), rows[] = {T, used};
     const int act = act_type(logits);
     NEED(act >= 0 && here(logits), "logits: f32, f16 or bf16 on the current CUDA device");
-    NEED(!wants_grad(logits), "logits: this operator has no gradient (use torch.no_grad or detach)");
     NEED(last_dense(logits), "logits: experts must be dense");
     NEED(T <= 0x7fffffff && E <= 0x7fffffff && used > 0 && used <= E, "n_used: from 1 to the number of experts");
     if (!ids.defined()) ids = empty(rows, at::kInt, logits);

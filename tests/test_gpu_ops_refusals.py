@@ -84,3 +84,18 @@ def test_memory_that_does_not_hold_the_values(ops, op, name):
         call(**{**a, name: gone})
     call(**a)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_what_would_lose_a_gradient(ops, op, name):
+    import torch.autograd.forward_ad as fw
+    call, a = args_of(ops)[op]
+    wants = {**a, name: a[name].clone().requires_grad_()}
+    with pytest.raises(ValueError, match=name + ".*no gradient"):
+        call(**wants)
+    with torch.no_grad():
+        call(**wants)
+    with fw.dual_level(), pytest.raises(ValueError, match=name + ".*no forward gradient"):
+        call(**{**a, name: fw.make_dual(a[name], torch.ones_like(a[name]))})
+    call(**a)
+    torch.cuda.synchronize()
