@@ -146,6 +146,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(a[7]);
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     const int pairs = PyObject_IsTrue(a[8]);
+    if (pairs < 0) return nullptr;
     TENSOR(pair_axis, a[9], true);
     TENSOR(k_cache, a[10], true);
     TENSOR(v_cache, a[11], true);
@@ -290,6 +291,7 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long used = PyLong_AsLong(a[1]);
     if (used == -1 && PyErr_Occurred()) return nullptr;
     const int renorm = PyObject_IsTrue(a[2]);
+    if (renorm < 0) return nullptr;
     const double scale = PyFloat_AsDouble(a[3]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
     OUTPUT(ids, a[4]);

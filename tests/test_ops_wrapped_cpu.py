@@ -87,3 +87,9 @@ def test_memory_that_does_not_hold_the_values_is_refused(ops, which):
         f(torch._neg_view(torch.ones(4, 8)))
     with pytest.raises(ValueError, match="hold its values"):
         f(torch._efficientzerotensor((4, 8)))
+
+
+def test_what_is_neither_true_nor_false(ops):
+    """renorm is asked for its truth; what it raises is what the caller gets."""
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ops.route_topk(torch.zeros(4, 8), 2, renorm=torch.zeros(2))
