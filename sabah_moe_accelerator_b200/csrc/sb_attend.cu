@@ -53,6 +53,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "sb_act.cuh"
 #include "sb_kernels.h"
@@ -1148,15 +1149,22 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
 }
 
 // ------------------------------------------------------------ launches
+// What is kept of a device holds for that device alone. A number beyond the table is asked anew.
+constexpr int kMaxDevices = 64;
+int device_index() {
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : -1;
+}
 int sm_count() {
-    static int sms = 0;
-    if (!sms) {
-        int dev = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        if (sms < 1) sms = 148;
-        sms = std::min(sms, kMaxWarps / 8);
-    }
+    static std::atomic<int> kept[kMaxDevices];
+    const int at = device_index();
+    int sms = at >= 0 ? kept[at].load(std::memory_order_relaxed) : 0;
+    if (sms) return sms;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    sms = std::min(sms < 1 ? 148 : sms, kMaxWarps / 8);
+    if (at >= 0) kept[at].store(sms, std::memory_order_relaxed);
     return sms;
 }
 int tile_width(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
@@ -1179,17 +1187,14 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
-    static EncodeTiled fn = nullptr;
-    static bool looked = false;
-    if (!looked) {
+    static const EncodeTiled fn = [] {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess &&
-            found == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiled)f;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess &&
+                        found == cudaDriverEntryPointSuccess;
         cudaGetLastError();
-        looked = true;
-    }
+        return ok ? (EncodeTiled)f : nullptr;
+    }();
     return fn;
 }
 // [pages][heads][tiles of 64 columns][slots][columns] with a box of p.box slots and
@@ -1220,12 +1225,13 @@ int launch(AttendParams p, cudaStream_t st) {
     const size_t seqs = 8 * (size_t)p.n_seqs + 4;
     // static shared memory (the scan's warp sums) is 128 bytes
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
-    static bool opted = false;
-    if (!opted) {
+    static std::atomic<bool> opted[kMaxDevices];
+    const int dev = device_index();
+    if (dev < 0 || !opted[dev].load(std::memory_order_relaxed)) {
         if (!sb_cuda_ok(cudaFuncSetAttribute(k_attend<Cache, DP, QP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              kSmemLimit - 1024), "attend shared memory"))
             return -1;
-        opted = true;
+        if (dev >= 0) opted[dev].store(true, std::memory_order_relaxed);
     }
     const int type = kF16 ? SB_F16 : SB_BF16;
     p.box = 16;
