@@ -1353,8 +1353,6 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     p.cut_row = (int*)(ws + lay.cut_row);
     p.pieces = (float*)(ws + lay.pieces);
     p.sums = (float*)(ws + lay.sums);
-    const int slot = sb_timing_begin("attend_paged", st);
-    int rc = 0;
     // the list of a launch has fewer than 2^31 places
     const long long most = (long long)n_kv_heads * p.tiles * ((long long)table_width * page_size / kStep + 2 + kRowCost);
     if (most > 0x7fffffffll) {
@@ -1363,6 +1361,8 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
         return -1;
     }
     const int per_launch = (int)std::min<long long>(kMaxSeqs, 0x7fffffffll / most);
+    const int slot = sb_timing_begin("attend_paged", st);
+    int rc = 0;
     for (int b = 0; b < n_seqs && rc == 0; b += per_launch) {
         AttendParams a = p;
         a.n_seqs = std::min(per_launch, n_seqs - b);

@@ -54,3 +54,13 @@ def test_each_device_is_set_up(host):
     assert host.fake_refused_launches() == 0
     assert sizes[1] < sizes[3] < sizes[0]
     host.fake_set_device(0)
+
+
+def test_a_refused_call_leaves_no_timing_open(host):
+    """A refusal after the checks of the arguments: the list of steps would be too long."""
+    host.fake_set_device(0)
+    open_before, launches = host.fake_open_timings(), host.fake_launches()
+    assert attend(host, kv=4096, heads=4096, width=1 << 26, page=16) == -1
+    assert b"too many" in host.fake_message()
+    assert host.fake_open_timings() == open_before and host.fake_launches() == launches
+    assert attend(host) == 0 and host.fake_open_timings() == open_before
