@@ -57,6 +57,7 @@
 
 #include "sb_act.cuh"
 #include "sb_kernels.h"
+#include "sb_split.cuh"
 
 namespace {
 
@@ -200,13 +201,6 @@ struct Seqs {
 __device__ inline int window_start(int len, int window) { return window > 0 ? max(0, len - window) : 0; }
 __device__ inline int seq_steps(int len, int window) {
     return len <= 0 ? 1 : (len + kStep - 1) / kStep - window_start(len, window) / kStep;
-}
-// a / b; the integer division is a long subroutine, and most numbers here are small
-__device__ inline int div_fast(int a, int b) {
-    if (a >= 1 << 22) return (int)((unsigned)a / (unsigned)b);
-    int q = (int)__fdividef((float)a, (float)b);   // within one of the quotient
-    q -= q * b > a;
-    return q + (a - q * b >= b);
 }
 // A place in the list; each warp has one that loads and one that computes.
 struct Cursor {
@@ -488,10 +482,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     // ---- this warp's own part; neighbours in the list sit on different SMs
     const int w = wid * gridDim.x + blockIdx.x, n_rows = p.n_kv * p.tiles;
     const int cost = seqs.pre[p.n_seqs] * n_rows, all_warps = gridDim.x * n_warps;
-    const int part = max(div_fast(cost + all_warps - 1, all_warps), kMinSteps);
+    const int part = part_of(cost, all_warps, kMinSteps);
     if (lane == 0) p.cut_pieces[w] = 0;
-    if (w >= div_fast(cost + part - 1, part)) return;
-    Cursor cc = enter_part(seqs, p, w * part, min(w * part + part, cost), lane);
+    if (w >= parts_in(cost, part)) return;
+    Cursor cc = enter_part(seqs, p, w * part, part_end(cost, part, w), lane);
     if (cc.b < 0) return;
 
     // ---- table entries and queries on their way, then keys and values
