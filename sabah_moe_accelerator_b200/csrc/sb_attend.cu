@@ -54,6 +54,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "sb_act.cuh"
 #include "sb_kernels.h"
@@ -96,6 +97,7 @@ struct AttendParams {
     float* pieces;          // per warp two: the row it enters in the middle of, the row it leaves early
     float* sums;            // per warp one: its rounded sums, where registers have no room for them
     int piece_floats, piece_rows;
+    int stalled;            // test only (SABAH_TEST_ATTEND_STALL): the warp that waits for what nothing ends; -1: none
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -107,8 +109,8 @@ __device__ inline void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Bounded: false after 2^24 tries, some tenths of a second.
-__device__ inline bool bar_wait(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < 1 << 24; ++i) {
+__device__ inline bool bar_wait(uint32_t bar, uint32_t parity, int tries = 1 << 24) {
+    for (int i = 0; i < tries; ++i) {
         uint32_t ok;
         asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
@@ -357,6 +359,11 @@ struct Loader {
 // heads and 16 columns a float4 per lane, of (column, head) = (lane / 4, 2 (lane
 // % 4)), the next head, and both at column + 8.
 constexpr int kPieceHead = 32;
+// the row c, which part w begins and does not end, for the join
+__device__ inline void cut(const AttendParams& p, const Cursor& c, int w, int part) {
+    p.cut_row[w] = c.b * p.n_kv * p.tiles + c.h;
+    p.cut_pieces[w] = (uint16_t)(div_fast(c.row_at + c.steps - 1, part) - w + 1);
+}
 __host__ __device__ inline int frag_at(int head, int col, int dp) {
     const int lane = col % 8 * 4 + head % 8 / 2;
     return ((head / 8 * (dp / 16) + col / 16) * 32 + lane) * 4 + col % 16 / 8 * 2 + head % 2;
@@ -410,6 +417,32 @@ __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int 
             piece[2 * row] = top, piece[2 * row + 1] = sum * scale;
         else if (p.lse)
             p.lse[at] = 0.69314718055994531f * (top + log2f(sum));
+    }
+}
+
+// ------------------------------------------------------------ giving up
+// A wait that never ends: the error word, then the loads in flight get their time
+// (`left` of this row's are still to be used, and the ring has no more than its
+// slots), and what this warp still owes becomes NaN: whole rows, and the sums of
+// pieces, which the join carries on to their rows.
+template <class Act>
+__device__ __noinline__ void give_up(const AttendParams& p, const Seqs& seqs, Cursor c, int first_j, int left, uint32_t bars,
+                                     int slot, uint32_t parity, int slots, int w, int part, int lane) {
+    const float nan = __int_as_float(0x7fc00000);
+    if (lane == 0) atomicExch(p.err, SB_DERR_TIMEOUT);
+    int ahead = left;
+    for (Cursor x = c; ahead < slots && next_row(x, seqs, p);) ahead += 2 * (x.end - x.j);
+    for (int i = 0; i < min(ahead, slots); ++i) bar_wait(bars + (slot + i) % slots * 8, parity ^ (slot + i >= slots));
+    for (bool live = true; live; live = next_row(c, seqs, p), first_j = 0) {
+        const int tile = c.h % p.tiles, head0 = c.h / p.tiles * p.group + tile * 16, heads = min(16, p.group - tile * 16);
+        if (first_j == 0 && c.end == c.steps) {
+            const size_t at = (size_t)c.b * p.n_q + head0;
+            for (int i = lane; i < heads * p.dim; i += 32) ((Act*)p.out)[at * p.dim + i] = sb_from_float<Act>(nan);
+            if (p.lse && lane < heads) p.lse[at + lane] = nan;
+            continue;
+        }
+        if (lane < heads) *(float2*)(p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats + 2 * lane) = make_float2(0.f, nan);
+        if (first_j == 0 && lane == 0) cut(p, c, w, part);
     }
 }
 
@@ -536,6 +569,15 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     float* sums = p.sums + (size_t)w * p.piece_floats;
     int slot = 0;
     uint32_t parity = 0;
+    if (w == p.stalled) {   // test only: a wait, with a short limit, that nothing ends
+        __shared__ uint64_t never;
+        if (lane == 0) bar_init(smem_addr(&never), 1);
+        __syncwarp();
+        if (!bar_wait(smem_addr(&never), 0, 1 << 10)) {
+            give_up<Act>(p, seqs, cc, cc.j, 2 * (cc.end - cc.j), bars, slot, parity, S::kSlots, w, part, lane);
+            return;
+        }
+    }
     for (bool live = true; live;) {
         const int tile = p.tiles == 1 ? 0 : cc.h % p.tiles, kv = p.tiles == 1 ? cc.h : cc.h / p.tiles;
         const int first_head = kv * p.group + tile * 16, heads = min(16, p.group - tile * 16);
@@ -625,10 +667,8 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         // keys on even counts, then values; one copy of the code that waits and loads
 #pragma unroll 1
         for (int n = 2 * (cc.end - cc.j); n > 0; --n) {
-            if (!bar_wait(bars + slot * 8, parity)) {   // give up, once the later loads had their time too
-                if (lane == 0) atomicExch(p.err, SB_DERR_TIMEOUT);
-                for (int i = 1; i < S::kSlots; ++i)
-                    bar_wait(bars + (slot + i) % S::kSlots * 8, parity ^ (slot + i >= S::kSlots));
+            if (!bar_wait(bars + slot * 8, parity)) {
+                give_up<Act>(p, seqs, cc, first_j, n, bars, slot, parity, S::kSlots, w, part, lane);
                 return;
             }
             const uint32_t at = ring + slot * S::kSlot;
@@ -811,10 +851,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         if (DP <= 128 && live) fetch_queries(cc);
         const bool whole = first_j == 0 && done.end == done.steps, none = done.len == done.lo;
         float* piece = p.pieces + (size_t)(2 * w + (first_j == 0)) * p.piece_floats;
-        if (!whole && first_j == 0 && lane == 0) {
-            p.cut_row[w] = done.b * n_rows + done.h;
-            p.cut_pieces[w] = (uint16_t)(div_fast(done.row_at + done.steps - 1, part) - w + 1);
-        }
+        if (!whole && first_j == 0 && lane == 0) cut(p, done, w, part);
         unsigned odd[2 * NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
@@ -1217,7 +1254,7 @@ int launch(AttendParams p, cudaStream_t st) {
     const int q_rows = NT == 1 ? 0 : std::min(p.group, 16) * QP;
     const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16);
     const size_t seqs = 8 * (size_t)p.n_seqs + 4;
-    // static shared memory (the scan's warp sums) is 128 bytes
+    // static shared memory (the scan's warp sums and a test's barrier) is under 256 bytes
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
     static std::atomic<bool> opted[kMaxDevices];
     const int dev = device_index();
@@ -1331,6 +1368,9 @@ SABAH_API int sabah_attend_paged(const void* d_q, size_t q_seq_stride, size_t q_
     p.lens = d_lens, p.n_seqs = n_seqs, p.n_q = n_q_heads, p.n_kv = n_kv_heads, p.dim = head_dim, p.window = window;
     p.scale_log2 = scale * 1.44269504088896341f;
     p.out = (uint8_t*)d_out, p.lse = d_lse, p.err = err;
+    static const bool test = std::getenv("SABAH_TEST_ATTEND_STALL") != nullptr;   // at the first call; then by call
+    const char* stall = test ? std::getenv("SABAH_TEST_ATTEND_STALL") : nullptr;
+    p.stalled = stall ? std::atoi(stall) : -1;
     if (!d_workspace || (uintptr_t)d_workspace % 16 ||
         workspace_bytes < sabah_attend_paged_workspace(n_q_heads, n_kv_heads, head_dim)) {
         sb_set_error("attend workspace of %zu bytes: %zu, 16-byte aligned, are needed", workspace_bytes,

@@ -3,11 +3,15 @@ out of the ordinary, against the formula in 64 bits."""
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import attn_oracle as o
+from conftest import ROOT
 from test_gpu_attend import BF, F32, HF, TYPES, make
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +114,54 @@ def test_nan_stays_however_little_it_weighs(ops, act, cache):
     assert want[0, :, 7].isnan().all() and want[1].isnan().all() and want[2, :, 9].isnan().all()
     for b in range(3):
         same(out[b], want[b], o.TOL[act])
+
+
+# ---------------------------------------------------------------- a wait that runs out
+STALL = "SABAH_TEST_ATTEND_STALL"
+
+
+def stall(ops, act, cache, heads, kv, dim):
+    from sabah_moe_accelerator_b200 import rt
+    short, long = [1, 40, 0, 7, 96, 33] * 40, [30000, 5, 20000]
+    for lens in (short, long, short + long):
+        t = make(lens, heads, kv, dim, 16, act, cache)
+        lse_ok = torch.empty(len(lens), heads, device="cuda")
+        want = ops.attend_paged(*t, lse=lse_ok)
+        assert torch.isfinite(want).all()
+        hurt = 0
+        for w in (0, 3, 150, 400):
+            lse, out = torch.full_like(lse_ok, 7.0), torch.full_like(want, 7.0)
+            os.environ[STALL] = str(w)
+            ops.attend_paged(*t, lse=lse, out=out)
+            torch.cuda.synchronize()
+            os.environ[STALL] = "-1"
+            code = rt.lib().sabah_rt_device_error()
+            lost = out.isnan()
+            rows = lost.all(-1)
+            assert torch.equal(rows, lost.any(-1)) and torch.equal(rows, lse.isnan())
+            assert torch.equal(out[~lost], want[~lost]) and torch.equal(lse[~rows], lse_ok[~rows])
+            assert code == (2 if rows.any() else 0)   # a warp beyond the list's parts has nothing to wait for
+            hurt += int(rows.any())
+        assert hurt >= 2
+        assert torch.equal(ops.attend_paged(*t), want)
+    assert rt.lib().sabah_rt_device_error() == 0
+
+
+def test_a_wait_that_runs_out_gives_nan_there_and_an_error():
+    """With the test switch SABAH_TEST_ATTEND_STALL=w, warp w first waits, with a short
+    limit, for what nothing ends. It gives up, lets its loads arrive and makes NaN of the
+    rows that it owes, whole or cut; every other row is what it was, the error word is
+    set, and the next call is clean. The switch is looked for at a process's first call."""
+    env = dict(os.environ, **{STALL: "-1"})
+    env["PYTHONPATH"] = os.pathsep.join((ROOT, os.path.join(ROOT, "tests"), env.get("PYTHONPATH", "")))
+    r = subprocess.run([sys.executable, os.path.abspath(__file__)], cwd=ROOT, env=env, capture_output=True, text=True,
+                       timeout=600)
+    assert r.returncode == 0 and "stall ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+if __name__ == "__main__":
+    from sabah_moe_accelerator_b200 import ops as _ops
+    _ops.init(0)
+    for _case in ((BF, BF, 16, 2, 256), (F32, HF, 8, 2, 128), (HF, HF, 40, 2, 64)):
+        stall(_ops, *_case)
+    print("stall ok")
