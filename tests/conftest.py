@@ -1,7 +1,8 @@
 """Shared fixtures. Tests marked `gpu` need a B200; everything else runs on CPU.
 
-The product library (sabah_moe_accelerator_b200/libsabah_rt.so) and the CPU
-oracle (oracle/_build/liboracle.so) are built on first use if absent.
+The product library (sabah_moe_accelerator_b200/libsabah_rt.so), its torch
+module (_torch_ops.so) and the CPU oracle (oracle/_build/liboracle.so) are built
+on first use if absent.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ if ROOT not in sys.path:
 
 PKG = os.path.join(ROOT, "sabah_moe_accelerator_b200")
 LIB = os.path.join(PKG, "libsabah_rt.so")
+TORCH_OPS = os.path.join(PKG, "_torch_ops.so")
 GOLDEN = os.path.join(ROOT, "tests", "golden", "golden.npz")
 
 
@@ -26,7 +28,7 @@ def pytest_configure(config):
 
 
 def _ensure_built():
-    if not os.path.exists(LIB):
+    if not (os.path.exists(LIB) and os.path.exists(TORCH_OPS)):
         subprocess.run(["make", "-s", "-C", os.path.join(PKG, "csrc")], check=True)
 
 
