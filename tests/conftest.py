@@ -27,6 +27,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
+# files whose tests need a build of the reference, and that build
+REFERENCE_BUILDS = {
+    "test_gpu_ref_harness.py": os.path.join(ROOT, "baseline", "_ref", "harness", "tests", "test_gpu_smoke.py"),
+    "test_gpu_ref_parity.py": os.path.join(ROOT, "oracle", "_ref", "libsabah_rt_ref.so"),
+}
+
+
+def pytest_collection_modifyitems(items):
+    """Tests whose reference build is missing fail, but last: under -x they would
+    keep the files after them from running."""
+    items.sort(key=lambda i: not os.path.exists(REFERENCE_BUILDS.get(i.path.name, ROOT)))
+
+
 def _ensure_built():
     if not (os.path.exists(LIB) and os.path.exists(TORCH_OPS)):
         subprocess.run(["make", "-s", "-C", os.path.join(PKG, "csrc")], check=True)
