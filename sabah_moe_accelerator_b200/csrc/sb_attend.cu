@@ -64,11 +64,13 @@ namespace {
 
 constexpr int kMaxDim = 256;
 constexpr int kMaxSeqs = 1024;   // per launch: the scan of the lengths sits in shared memory
-// What the split is made of, each measured against its neighbours (us a call):
+// What the split is made of, each measured against its neighbours on one kernel, us a
+// call in a graph. S: 256 sequences of 16-512 keys, 8 heads of 64, f16; L: the same
+// lengths, 16 over 2 heads of 256, bf16; M: 64 of 64-2048, 32 over 8 of 128, f32 over bf16.
 constexpr int kStep = 32;        // keys per step
-constexpr int kWhole = 3;        // rows of at most this many steps are never cut (256 sequences of 16-512 keys: 28.5; 4: 29.8, 8: 38)
-constexpr int kMinSteps = 1;     // and a part is at least this long (1000 keys, 2 rows: 17.0; 2: 19.3, 4: 25.2)
-constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps (the same 256: 31.7; 1: 33.4, 3: 32.6)
+constexpr int kWhole = 3;        // rows of at most this many steps are never cut (S 27.5, L 30.8, M 39.8; 2: 27.4, 28.7, 38.8; 4: 29.0, 31.1, 40.3; 8: 33.9, 35.9, 46.1)
+constexpr int kMinSteps = 1;     // and a part is at least this long (1000 keys, 16 over 2 heads of 128: 13.8; 2: 14.3, 4: 16.8)
+constexpr int kRowCost = 2;      // what a row costs besides its steps, in steps (S 27.5, L 30.8, M 39.8; 1: 29.1, 34.1, 42.1; 3: 29.5, 30.2, 39.4)
 constexpr int kMaxWarps = 148 * 8;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr float kLazy = 4.f;     // how far, in powers of two, a score may exceed the reference
@@ -97,7 +99,7 @@ struct AttendParams {
     float* pieces;          // per warp two: the row it enters in the middle of, the row it leaves early
     float* sums;            // per warp one: its rounded sums, where registers have no room for them
     int piece_floats, piece_rows;
-    int stalled;            // test only (SABAH_TEST_ATTEND_STALL): the warp that waits for what nothing ends; -1: none
+    int stalled;            // test only (SABAH_TEST_ATTEND_STALL): the warp whose first wait nothing ends; -1: none
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -108,9 +110,12 @@ __device__ inline void bar_init(uint32_t bar, int count) {
 __device__ inline void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Bounded: false after 2^24 tries, some tenths of a second.
-__device__ inline bool bar_wait(uint32_t bar, uint32_t parity, int tries = 1 << 24) {
-    for (int i = 0; i < tries; ++i) {
+__device__ inline void bar_expect_more(uint32_t bar, uint32_t bytes) {   // without arriving
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Bounded: false after 2^24 tries, under a second.
+__device__ inline bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < 1 << 24; ++i) {
         uint32_t ok;
         asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
@@ -150,7 +155,7 @@ __device__ inline void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ inline float exp2_fast(float x) {   // 2 ulp; exp2(-inf) = 0
+__device__ inline float exp2_fast(float x) {   // 2 ulp, less than the rounding of a score; exp2(-inf) = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
@@ -427,7 +432,10 @@ __device__ __noinline__ void redo_row(const AttendParams& p, int b, int kv, int 
 // pieces, which the join carries on to their rows.
 template <class Act>
 __device__ __noinline__ void give_up(const AttendParams& p, const Seqs& seqs, Cursor c, int first_j, int left, uint32_t bars,
-                                     int slot, uint32_t parity, int slots, int w, int part, int lane) {
+                                     int slot, uint32_t parity, int slots) {
+    // found anew, so that the kernel keeps nothing for a call that it hardly ever makes
+    const int lane = threadIdx.x & 31, n_warps = blockDim.x >> 5, w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    const int part = part_of(seqs.pre[p.n_seqs] * p.n_kv * p.tiles, gridDim.x * n_warps, kMinSteps);
     const float nan = __int_as_float(0x7fc00000);
     if (lane == 0) atomicExch(p.err, SB_DERR_TIMEOUT);
     int ahead = left;
@@ -461,6 +469,9 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     constexpr float kUp = up_of(std::is_same<Cache, __half>::value);
     // rounded sums stay in registers where there is room for them
     constexpr bool kKeep = ND * (8 * NT + (NT == 1 ? 2 * QP : 0)) <= 160;
+    // A cut-off loses up to 2^-23 of the running sum, 2 PP of them a step: before a fold
+    // 48 at most with fp32 outputs (6e-6; three parts), 128 with 16-bit ones (1.5e-5,
+    // under a tenth of f16's half unit). More folds cost time, one is 4 ND NT adds a lane.
     constexpr int kFold = QP == 1 ? 32 : 8;
     constexpr int kQRow = DP * 2 + 16;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -551,6 +562,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     };
     uint8_t* ring_mem = smem + wid * S::kSlots * S::kSlot;
     const uint32_t ring = smem_addr(ring_mem);
+    if (w == p.stalled && lane == 0) bar_expect_more(bars, 16);   // test only: bytes that no load brings
     Loader<DP> loader(p, &kmap, &vmap, seqs, lane, ring, bars, cc);
     fetch_queries(cc);
 #pragma unroll 1
@@ -569,15 +581,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     float* sums = p.sums + (size_t)w * p.piece_floats;
     int slot = 0;
     uint32_t parity = 0;
-    if (w == p.stalled) {   // test only: a wait, with a short limit, that nothing ends
-        __shared__ uint64_t never;
-        if (lane == 0) bar_init(smem_addr(&never), 1);
-        __syncwarp();
-        if (!bar_wait(smem_addr(&never), 0, 1 << 10)) {
-            give_up<Act>(p, seqs, cc, cc.j, 2 * (cc.end - cc.j), bars, slot, parity, S::kSlots, w, part, lane);
-            return;
-        }
-    }
     for (bool live = true; live;) {
         const int tile = p.tiles == 1 ? 0 : cc.h % p.tiles, kv = p.tiles == 1 ? cc.h : cc.h / p.tiles;
         const int first_head = kv * p.group + tile * 16, heads = min(16, p.group - tile * 16);
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 #pragma unroll 1
         for (int n = 2 * (cc.end - cc.j); n > 0; --n) {
             if (!bar_wait(bars + slot * 8, parity)) {
-                give_up<Act>(p, seqs, cc, first_j, n, bars, slot, parity, S::kSlots, w, part, lane);
+                give_up<Act>(p, seqs, cc, first_j, n, bars, slot, parity, S::kSlots);
                 return;
             }
             const uint32_t at = ring + slot * S::kSlot;
@@ -1254,7 +1257,7 @@ int launch(AttendParams p, cudaStream_t st) {
     const int q_rows = NT == 1 ? 0 : std::min(p.group, 16) * QP;
     const size_t per_warp = S::kSlots * (S::kSlot + 8) + (size_t)q_rows * (DP * 2 + 16);
     const size_t seqs = 8 * (size_t)p.n_seqs + 4;
-    // static shared memory (the scan's warp sums and a test's barrier) is under 256 bytes
+    // static shared memory (the scan's warp sums) takes 1024 bytes, the rings' alignment
     const int warps = (int)std::min<size_t>(S::kWarps, (kSmemLimit - 1024 - seqs) / per_warp);
     static std::atomic<bool> opted[kMaxDevices];
     const int dev = device_index();
