@@ -125,7 +125,8 @@ int sabah_moe_decode(int n_layers, const void *const *gate_banks, const void *co
                      int ff, int n_used, int n_tokens, int qt_gate, int qt_up, int qt_down, void *stream);
 
 /* Reads and clears the device error word: 1 when a kernel reading a
- * device-resident bank met an expert id outside [0, n_experts), 4 when an
+ * device-resident bank met an expert id outside [0, n_experts), 2 when a kernel
+ * gave up a wait, 3 when an expert base was not 16-byte aligned, 4 when an
  * attention-side kernel met a cache page, slot, length or position out of
  * range, else 0.
  * New in this build (the device-resident path has no synchronous id check). */
@@ -178,7 +179,9 @@ int sabah_qk_norm_rope(const void *d_q, size_t q_token_stride, size_t q_head_str
  * A sequence of length 0 gives zeros and an lse of -inf. Table entries outside
  * the window are not read, and nothing that rows outside it hold counts (NaN
  * included). A length outside [0, table_width * page_size] or a page outside
- * [0, n_pages) gives that sequence NaN, and the device error word.
+ * [0, n_pages) gives that sequence NaN, and the device error word; so does a wait
+ * for cache rows that runs out, for the heads that it belongs to. out and lse must
+ * not overlap anything that is read.
  * d_workspace holds sabah_attend_paged_workspace(...) bytes, 16-byte aligned,
  * of any content; calls that may overlap on the GPU must not share it. */
 size_t sabah_attend_paged_workspace(int n_q_heads, int n_kv_heads, int head_dim);

@@ -44,10 +44,10 @@
 // to rounded fp32 sums every kFold steps.
 //
 // Measured (one B200, the inputs in turn larger than L2): 131,071 keys of one
-// sequence, 2 heads of 256, bf16: 58 us, 4.6 TB/s, of which about 7 us pass before
+// sequence, 2 heads of 256, bf16: 59 us, 4.5 TB/s, of which about 7 us pass before
 // the first keys arrive and 6 in the join; 64 sequences of 128-8192 keys, 8
-// heads of 128, f16 with fp32 queries: 96 us, 5.3 TB/s (the steady part 7.2); 256
-// of 16-512 keys, 8 heads of 64: 29 us, 2.5 TB/s; 37 keys: 9.5 us. The start is
+// heads of 128, f16 with fp32 queries: 99 us, 5.1 TB/s (the steady part 7.2); 256
+// of 16-512 keys, 8 heads of 64: 29 us, 2.5 TB/s; 37 keys: 9.6 us. The start is
 // a chain of dependent reads (lengths, block table, rows) and code that runs for
 // the first time; what bounds the long calls is DRAM.
 #include <cuda.h>

@@ -18,15 +18,15 @@
 // the token's cosines once for all of them and multiplies them by the weights:
 // a turned value is then two products and one by the norm.
 //
-// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 43-45 us, 4.8
-// TB/s; the same rows only copied take 35 us. What is left is the chain position
-// -> cosines of a short task, which more warps would hide and registers do not
-// allow: issue slots 69%, warps 44%. The kind of row is the CTA's, so that its tests and pointers are uniform
-// (a flat index over all tasks of a token: 55 us), and place and position are read
-// before the rows (after them: 45). Slower: one, three or six rows per task (68,
-// 52, 60), 9 CTAs an SM for 8 (47); with the flat index 8 values at a time (71),
-// tasks in a loop with the next one's rows ahead (59), a CTA per token with the
-// turn in shared memory (68).
+// Measured (one B200): 8191 tokens x (32 + 8 + 8) heads of 128, bf16: 42.7 us in a
+// graph (4.8 TB/s), 45 called one by one; the same rows only copied take 35 us. What
+// is left is the chain position -> cosines of a short task, which more warps would
+// hide and registers do not allow: issue slots 69%, DRAM 46%, warps 44%. The kind of
+// row is the CTA's, so that its tests and pointers are uniform (a flat index over all
+// tasks of a token: 55 us), and place and position are read before the rows (after
+// them: 45). Slower: one, three or six rows per task (68, 52, 60), 9 CTAs an SM for 8
+// (47); with the flat index 8 values at a time (71), tasks in a loop with the next
+// one's rows ahead (59), a CTA per token with the turn in shared memory (68).
 #include "sb_act.cuh"
 #include "sb_kernels.h"
 
@@ -248,7 +248,7 @@ void launch(NormRopeParams p, cudaStream_t st) {
 
 // Four rows per lane group once the rows of one would fill the chip twice over
 // (148 SMs x 64 warps): the cosines, positions and indexes are then a fourth of
-// the work (8191 tokens: 43 us, with one row 68; 2049 patches of 24 + 4 heads of
+// the work (8191 tokens: 45 us, with one row 68; 2049 patches of 24 + 4 heads of
 // 80: 10.4 and 16.5), where few rows want all the warps there are (64 tokens: 5.0
 // us either way, the launch).
 template <class Act, class Cache, int LPR>

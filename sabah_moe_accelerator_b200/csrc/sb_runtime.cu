@@ -549,7 +549,7 @@ bool device_errors_clear() {
                      code == SB_DERR_BAD_ID ? "a kernel found an expert id outside [0, n_experts)"
                      : code == SB_DERR_MISALIGNED ? "an expert base was not 16-byte aligned"
                      : code == SB_DERR_BAD_INDEX ? "a kernel found a cache page, slot, length or position out of range"
-                     : "a kernel gave up waiting for its weight tiles", code);
+                     : "a kernel gave up waiting for its weight tiles or cache rows", code);
         return false;
     }
     return true;

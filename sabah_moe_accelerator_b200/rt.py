@@ -23,8 +23,6 @@ QTYPE = {
     "IQ3_XXS": 18, "IQ4_NL": 20, "IQ3_S": 21, "IQ2_S": 22, "IQ4_XS": 23, "Q2_0": 42,
 }
 QTYPE_NAME = {v: k for k, v in QTYPE.items()}
-# element types of activations and key-value caches (ggml's codes too)
-ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 30
 
 # (elements per block, bytes per block) (reference rt.py:26-31, plus Q6_K)
 QBLOCK = {
