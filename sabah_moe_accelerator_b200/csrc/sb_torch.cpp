@@ -10,11 +10,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/DispatchKeySet.h>
 
 #include "../../include/sabah_rt.h"
 
@@ -35,6 +35,15 @@ PyObject* g_error;   // rt.SabahCudaError
         }                                             \
     } while (0)
 
+// A tensor that stands for others, or for one laid out otherwise. A mode that is
+// active around the call (a counter of operations, say) does not make it one.
+bool wrapper(const at::Tensor& t) {
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                        c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
+                                        c10::DispatchKey::Batched});
+    return t.key_set().has_any(keys) || t.layout() != at::kStrided || t.is_nested();
+}
+
 // The tensor behind an argument, which the caller holds during the call; an
 // undefined one for None, null with the error for anything else. A wrapper (of
 // vmap, a functional transform, a dispatching subclass) has no memory of its own;
@@ -49,7 +58,7 @@ const at::Tensor* tensor(PyObject* o, const char* name, bool optional) {
         return nullptr;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (at::isTensorSubclassLike(t)) {
+    if (wrapper(t)) {
         PyErr_Format(PyExc_ValueError, "%s: a plain tensor (not inside vmap or another transform, no dispatching subclass)",
                      name);
         return nullptr;

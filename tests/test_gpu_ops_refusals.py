@@ -99,3 +99,19 @@ def test_what_would_lose_a_gradient(ops, op, name):
         call(**{**a, name: fw.make_dual(a[name], torch.ones_like(a[name]))})
     call(**a)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("op", ["norm_rope", "attend", "route"])
+def test_a_dispatch_mode_changes_nothing(ops, op):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    call, a = args_of(ops)[op]
+    want = call(**a)
+    want = [t.clone() for t in (want if isinstance(want, tuple) else (want,))]
+    with Watch():
+        got = call(**a)
+    assert all(torch.equal(x, y) for x, y in zip(got if isinstance(got, tuple) else (got,), want))

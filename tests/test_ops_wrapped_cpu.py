@@ -93,3 +93,29 @@ def test_what_is_neither_true_nor_false(ops):
     """renorm is asked for its truth; what it raises is what the caller gets."""
     with pytest.raises(RuntimeError, match="ambiguous"):
         ops.route_topk(torch.zeros(4, 8), 2, renorm=torch.zeros(2))
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_plain_tensors_under_a_dispatch_mode_are_plain(ops, which):
+    """A mode that watches torch's own operations is none of a tensor's doing."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Watch(), pytest.raises(ValueError, match="CUDA"):   # the next check speaks
+        calls(ops)[which](torch.zeros(4, 8))
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_other_layouts_are_refused(ops, which):
+    with pytest.raises(ValueError, match="plain tensor"):
+        if which == 2:
+            ops.route_topk(torch.zeros(4, 8).to_sparse(), 2)
+        else:
+            s, x = torch.zeros(2, 2, 8).to_sparse(), torch.zeros(2, 2, 8)
+            ops.qk_norm_rope(x, s, None, None, None, None, None) if which else ops.attend_paged(s, x, x, x, x)
+    functional = torch.func.functionalize(calls(ops)[which])
+    with pytest.raises(ValueError, match="plain tensor"):
+        functional(torch.zeros(4, 8))
